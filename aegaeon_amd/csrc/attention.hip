@@ -61,6 +61,7 @@
 #include <utility>
 
 #include "aegkv_internal.h"
+#include "kv4_format.h"
 
 namespace aegkv {
 namespace {
@@ -101,6 +102,9 @@ __device__ __forceinline__ int cost_units(int len) {
 // wave per SIMD.
 template <int D>
 constexpr int pipeline_depth() { return D >= 256 ? 2 : 3; }
+// Steps of the 4-bit cache in registers.
+template <int D>
+constexpr int kv4_pipeline_depth() { return 2; }
 
 // kv heads of a workgroup's group, one per wave; the 4 / heads waves of each
 // head take ranges of their own.  Four, unless that leaves one wave in 20 or
@@ -507,6 +511,169 @@ __device__ __forceinline__ void compute_block(KVRegs<D>& r, const u32x4* qv, f32
       a1 = (v[2][w] & 0xffffu) | (v[3][w] << 16);
     }
     acc[t] = E::mfma(u32x4{a0, a1, a0, a1}, bop, acc[t]);
+  }
+}
+
+// ---- the 4-bit cache (kv4_format.h) ----
+// Codes and scale bytes of one block for one lane (j, g): K token j, whose
+// words hold 8 dims each of the chunks g (and, D = 256, 4 + g); V tokens 4g ..
+// 4g + 3, dims D/16 j .. of each.  The contraction over the head dim runs in
+// the codes' order: k-step ks takes the lane's word ks, dims kv4_dim(ks, g) ..
+// + 7, of K and of the query alike.
+template <int D>
+struct KV4Regs {
+  static constexpr int KS = D / 32;  // QK k-steps: words of K codes per lane
+  static constexpr int NS = D >= 256 ? 2 : 1;
+  uint32_t k[KS], v[KS];  // D = 64: a word of V holds two tokens' four codes
+  uint32_t ks[NS];        // scale byte of the K words (each NS-th part of them)
+  uint32_t vs;            // scale bytes of the four V tokens
+};
+template <int D>
+__device__ __forceinline__ int kv4_dim(int ks, int g) {
+  return 128 * (ks >> 2) + (D == 64 ? 16 : 32) * g + 8 * (ks & 3);
+}
+
+// One block of one kv head: r is its K and V records (17 D bytes, or empty).
+template <int D>
+__device__ __forceinline__ void load_block4(KV4Regs<D>& b, __amdgpu_buffer_rsrc_t r, int lane) {
+  constexpr int REC = kv4_record_bytes(D), CODES = kv4_code_bytes(D);
+  const int j = lane & 15, g = lane >> 4;
+  if constexpr (D == 64) {
+    const u32x2 k = __builtin_amdgcn_raw_buffer_load_b64(r, 8 * lane, 0, kNt);
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, REC + 8 * lane, 0, kNt);
+    b.k[0] = k.x; b.k[1] = k.y;
+    b.v[0] = v.x; b.v[1] = v.y;
+  } else {
+#pragma unroll
+    for (int f = 0; f < D / 128; ++f) {
+      const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(r, 1024 * f + 16 * lane, 0, kNt);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, REC + 1024 * f + 16 * lane, 0, kNt);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b.k[4 * f + i] = k[i];
+        b.v[4 * f + i] = v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < KV4Regs<D>::NS; ++f)
+    b.ks[f] = __builtin_amdgcn_raw_buffer_load_b8(
+        r, CODES + ((D == 64 ? g >> 1 : g) + 4 * f) * kBlockSize + j, 0, kNt);
+  b.vs = __builtin_amdgcn_raw_buffer_load_b32(
+      r, REC + CODES + (j * (D / 16) / kKv4Group) * kBlockSize + 4 * g, 0, kNt);
+}
+
+// A step of up to kStep4 consecutive blocks of one sequence, its first token
+// tok0: the softmax update and P.V of compute_block, with one maximum and one
+// rescale test for all of them.  K and V are converted to 16 bits, where every
+// code times its scale is exact, so nothing past the conversion differs from
+// the 16-bit cache's arithmetic.  Tokens at or past `limit` are masked, and the
+// blocks whose bit in `skip` is set (unreadable ids, and those past the step).
+constexpr int kStep4 = 4;
+template <int DT, int D>
+__device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[kStep4], const u32x4* qv, f32x4* acc,
+                                              float& m, float& lsum, int tok0, int limit,
+                                              uint32_t skip, int g, float scale_log2) {
+  using E = Elem<DT>;
+  using C = Kv4Elem<DT>;
+  constexpr int KS = KV4Regs<D>::KS;
+  f32x4 sc[kStep4];
+#pragma unroll
+  for (int u = 0; u < kStep4; ++u) {
+    sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const float s = kv4_scale(r[u].ks[ks >> 2]);
+      const uint32_t w = r[u].k[ks];
+      sc[u] = E::mfma(u32x4{C::template dq<0>(w, s), C::template dq<1>(w, s),
+                            C::template dq<2>(w, s), C::template dq<3>(w, s)},
+                      qv[ks], sc[u]);
+    }
+  }
+  const int last = limit - tok0 - 4 * g;  // this lane's tokens 16 u + i below it
+  float x[kStep4][4];
+#pragma unroll
+  for (int u = 0; u < kStep4; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[u][i] = (16 * u + i < last && !(skip >> u & 1)) ? sc[u][i] * scale_log2 : -INFINITY;
+  float bm = x[0][0];
+#pragma unroll
+  for (int u = 0; u < kStep4; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bm = fmaxf(bm, x[u][i]);
+  bm = fmaxf(bm, __shfl_xor(bm, 16));
+  bm = fmaxf(bm, __shfl_xor(bm, 32));
+  if (__builtin_amdgcn_ballot_w64(bm > m + kRescaleSlack)) {  // lazy rescaling, as in compute_block
+    const float mn = fmaxf(m, bm);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);  // 0 while m = -inf
+    lsum *= alpha;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) acc[t] *= alpha;
+    m = mn;
+  }
+  const float ms = m == -INFINITY ? 0.f : m;  // -inf only while every token is masked
+#pragma unroll
+  for (int u = 0; u < kStep4; ++u) {
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(x[u][i] - ms);
+    lsum += (p[0] + p[1]) + (p[2] + p[3]);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) E::split(p[i], hi[i], lo[i]);
+    const u32x4 bop = {hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16), lo[0] | (lo[1] << 16),
+                       lo[2] | (lo[3] << 16)};
+    // tokens past the end hold stale bytes, maybe the scale byte of NaN: scale
+    // byte zero and codes zero read as zero
+    uint32_t vs = r[u].vs;
+    uint32_t v[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) v[i] = r[u].v[i];
+    if (tok0 + 16 * (u + 1) > limit) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool keep = 16 * u + c < last;
+        vs = keep ? vs : vs & ~(0xffu << (8 * c));
+        if constexpr (D == 64) {
+          v[c >> 1] = keep ? v[c >> 1] : v[c >> 1] & (c & 1 ? 0x0000ffffu : 0xffff0000u);
+        } else {
+#pragma unroll
+          for (int f = 0; f < D / 128; ++f) v[4 * f + c] = keep ? v[4 * f + c] : 0u;
+        }
+      }
+    }
+    float s[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] = kv4_scale((vs >> (8 * c)) & 0xffu);
+    // dims t and t + 1 (t even) of the four tokens -> the tokens of each dim
+    auto tile_pair = [&](int t, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+      const uint32_t e0 = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+      const uint32_t e1 = __builtin_amdgcn_perm(x3, x2, 0x05040100u);
+      const uint32_t o0 = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+      const uint32_t o1 = __builtin_amdgcn_perm(x3, x2, 0x07060302u);
+      acc[t] = E::mfma(u32x4{e0, e1, e0, e1}, bop, acc[t]);
+      acc[t + 1] = E::mfma(u32x4{o0, o1, o0, o1}, bop, acc[t + 1]);
+    };
+    if constexpr (D == 64) {
+      tile_pair(0, C::template dq<0>(v[0], s[0]), C::template dq<2>(v[0], s[1]),
+                C::template dq<0>(v[1], s[2]), C::template dq<2>(v[1], s[3]));
+      tile_pair(2, C::template dq<1>(v[0], s[0]), C::template dq<3>(v[0], s[1]),
+                C::template dq<1>(v[1], s[2]), C::template dq<3>(v[1], s[3]));
+    } else {
+#pragma unroll
+      for (int f = 0; f < D / 128; ++f) {
+        const uint32_t* w = v + 4 * f;
+        tile_pair(8 * f + 0, C::template dq<0>(w[0], s[0]), C::template dq<0>(w[1], s[1]),
+                  C::template dq<0>(w[2], s[2]), C::template dq<0>(w[3], s[3]));
+        tile_pair(8 * f + 2, C::template dq<1>(w[0], s[0]), C::template dq<1>(w[1], s[1]),
+                  C::template dq<1>(w[2], s[2]), C::template dq<1>(w[3], s[3]));
+        tile_pair(8 * f + 4, C::template dq<2>(w[0], s[0]), C::template dq<2>(w[1], s[1]),
+                  C::template dq<2>(w[2], s[2]), C::template dq<2>(w[3], s[3]));
+        tile_pair(8 * f + 6, C::template dq<3>(w[0], s[0]), C::template dq<3>(w[1], s[1]),
+                  C::template dq<3>(w[2], s[2]), C::template dq<3>(w[3], s[3]));
+      }
+    }
   }
 }
 
@@ -952,6 +1119,167 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
   flush();
 }
 
+// attend_items over the 4-bit cache: the same items, ids, pieces and records,
+// in steps of up to kStep4 blocks that end where a piece does.  The step that
+// is loaded is NSET - 1 steps ahead of the one computed, across sequences: the
+// load side keeps a sequence position of its own, and hands a step's to the
+// compute side with its registers.  Past the range a step loads nothing (empty
+// buffer ranges) and is not computed.
+template <int DT, int D, int NSET, bool PLANNED>
+__device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* s_bcum,
+                                              const int32_t* s_len, uint8_t* stage, int4* meta,
+                                              int range, int grp, int hl, int b0, int i0, int i1,
+                                              bool have_first, int id_first) {
+  constexpr int KS = D / 32;
+  constexpr int DPL = D / 16;
+  const int lane = threadIdx.x & 63;
+  const int h = grp * a.heads + hl;
+  if (h >= a.n_kv_heads) return;  // wave past the last kv head (uniform)
+  const int j = lane & 15, g = lane >> 4;
+  const bool head_ok = j < a.group;
+  const int hq = h * a.group + j;
+  const int hl0 = hl * a.group;
+
+  // ids of items [cbase, cbase + 64) and of the next 64, one lane per item
+  auto item_id = [&](int i, int bh) -> int {
+    i = min(i, i1 - 1);
+    if constexpr (PLANNED) {
+      return a.plan_ids[i];
+    } else {
+      int b = bh;
+      if (s_bcum[b + 1] <= i) b = s_bcum[b + 2] > i ? b + 1 : seq_at(s_bcum, a.batch, i);
+      return a.block_tables[(int64_t)b * a.max_blocks + (i - s_bcum[b])];
+    }
+  };
+  int id_cur = PLANNED && have_first ? id_first : item_id(i0 + lane, b0);
+  int id_nxt = item_id(i0 + 64 + lane, b0);
+  int cbase = i0;
+  auto next_seq = [&](int b) -> int {  // the next non-empty sequence (one exists)
+    ++b;
+    while (uni(s_bcum[b + 1]) == uni(s_bcum[b])) ++b;
+    return b;
+  };
+  auto load_q = [&](int b, u32x4* qv) {  // lanes past the group load its first head
+    const uint16_t* qp =
+        a.q + (int64_t)b * a.q_bstride + (int64_t)(head_ok ? hq : h * a.group) * D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qv[ks] = *reinterpret_cast<const u32x4*>(qp + kv4_dim<D>(ks, g));
+  };
+
+  // the load side: sequence bl, whose items in range end at lend; next item il
+  int bl = b0, il = i0, lend = min(uni(s_bcum[b0 + 1]), i1);
+  struct Step {
+    int n;          // blocks (0: past the range)
+    uint32_t skip;  // blocks not to attend: unreadable, or past n
+  };
+  KV4Regs<D> buf[NSET][kStep4];
+  Step st[NSET];
+  auto load_step = [&](KV4Regs<D> (&r)[kStep4], Step& s) {
+    s.n = min(kStep4, lend - il);
+    s.skip = 0;
+    if (il - cbase >= 64) {
+      id_cur = id_nxt;
+      cbase += 64;
+      id_nxt = item_id(cbase + 64 + lane, bl);
+    }
+#pragma unroll
+    for (int u = 0; u < kStep4; ++u) {
+      // item il + u of the 128 at hand
+      const int k = il + u - cbase;
+      const int id = k < 64 ? __builtin_amdgcn_readlane(id_cur, k & 63)
+                            : __builtin_amdgcn_readlane(id_nxt, k & 63);
+      const bool ok = u < s.n && id >= 0 && id < a.n_blocks;
+      if (!ok) s.skip |= 1u << u;
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id : 0) * a.blk_stride) +
+                         (int64_t)h * 17 * D;
+      load_block4<D>(r[u], byte_range(p, ok ? 17 * D : 0u), lane);
+    }
+    il += s.n;
+    if (il == lend && il < i1) {
+      bl = next_seq(bl);
+      lend = min(uni(s_bcum[bl + 1]), i1);
+    }
+  };
+
+  // the compute side
+  int bc = b0, first = uni(s_bcum[b0]), cend = lend, len = uni(s_len[b0]), ic = i0;
+  bool complete = first >= i0 && cend == uni(s_bcum[b0 + 1]);
+  u32x4 qv[KS];
+  load_q(bc, qv);
+  f32x4 acc[DPL];
+#pragma unroll
+  for (int t = 0; t < DPL; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, lsum = 0.f;
+
+  const int rec_bytes = stage_record_bytes<D>();
+  const int slot_bytes = a.group * 4 * rec_bytes;
+  uint8_t* my_rec = stage + (j * 4 + g) * rec_bytes;
+  int nstaged = 0;
+  auto flush = [&]() {
+    if constexpr (!stages_pieces<D>()) return;
+    for (int s = 0; s < nstaged; ++s) {
+      const int4 md = meta[s];
+      f32x4 o[DPL];
+      float mm, lt;
+      if (head_ok) {
+        get_record<D>(my_rec + s * slot_bytes, o, mm, lt);
+        store_piece<DT, D>(a, o, mm, lt, uni(md.x), hq, uni(md.y) != 0, uni(md.z), hl0);
+      }
+    }
+    nstaged = 0;
+  };
+  auto compute = [&](KV4Regs<D> (&r)[kStep4], const Step& s) {
+    compute_step4<DT, D>(r, qv, acc, m, lsum, (ic - first) * kBlockSize,
+                         min(len, (cend - first) * kBlockSize), s.skip, g, a.scale_log2);
+    ic += s.n;
+    if (ic == cend) {  // the piece of sequence bc in this range ends (uniform)
+      float lt = lsum + __shfl_xor(lsum, 16);
+      lt += __shfl_xor(lt, 32);
+      const int pslot = range + grp * a.batch + bc;
+      if (stages_pieces<D>() && a.stage_slots > 0) {
+        if (nstaged == a.stage_slots) flush();
+        if (head_ok) put_record<D>(my_rec + nstaged * slot_bytes, acc, m, lt);
+        if (lane == 0) meta[nstaged] = make_int4(bc, complete ? 1 : 0, pslot, 0);
+        ++nstaged;
+      } else if (head_ok) {
+        store_piece<DT, D>(a, acc, m, lt, bc, hq, complete, pslot, hl0);
+      }
+      if (ic < i1) {
+        bc = next_seq(bc);
+        first = uni(s_bcum[bc]);
+        cend = min(uni(s_bcum[bc + 1]), i1);
+        len = uni(s_len[bc]);
+        complete = cend == uni(s_bcum[bc + 1]);  // it starts in range
+        load_q(bc, qv);
+#pragma unroll
+        for (int t = 0; t < DPL; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY;
+        lsum = 0.f;
+      }
+    }
+  };
+
+  unrolled_steps<NSET>([&](auto kc) {
+    load_step(buf[decltype(kc)::value], st[decltype(kc)::value]);
+    return false;
+  });
+  bool more = true;
+  while (more) {
+    unrolled_steps<NSET>([&](auto kc) {
+      constexpr int k = decltype(kc)::value;
+      compute(buf[k], st[k]);
+      if (ic == i1) {  // every item is computed (uniform)
+        more = false;
+        return true;
+      }
+      load_step(buf[k], st[k]);
+      return false;
+    });
+  }
+  flush();
+}
+
 // Prefix sums of the batch's positions and blocks (lengths clamped to
 // max_seq_len) into LDS: s_cum[batch + 1] (cost units), s_bcum[batch + 1]
 // (blocks), s_len[batch]; with s_over, bit b set when sequence b's length
@@ -1058,7 +1386,7 @@ __device__ __forceinline__ int items_before(const int32_t* cum, const int32_t* b
   return bcum[b] + min(max(p - cum[b] - kSegmentCost, 0), bcum[b + 1] - bcum[b]);
 }
 
-template <int DT, int D, int NBUF, bool PLANNED, bool FUSED>
+template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, bool Q4>
 __global__ __launch_bounds__(64 * kWaves, D >= 256 ? 1 : 2) void
 paged_decode_attention_kernel(AttnArgs a) {
   // cum[batch + 1] (positions), len[batch], bcum[batch + 1] (blocks)
@@ -1108,7 +1436,11 @@ paged_decode_attention_kernel(AttnArgs a) {
       const int i0 = first_pass ? uni(rec[2]) : 0;
       const int b0 = first_pass ? uni(rec[3]) : uni(rec[5]);
       const int i1 = grp == uni(rec[1]) ? uni(rec[4]) : items;
-      if (i1 > i0)
+      if (i1 <= i0) continue;
+      if constexpr (Q4)
+        attend_items4<DT, D, NBUF, true>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
+                                         i0, i1, first_pass, id_first);
+      else
         attend_items<DT, D, NBUF, true, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
                                                hl, b0, i0, i1, first_pass, id_first,
                                                first_pass ? tag_first : -1, s_over, nstage,
@@ -1147,7 +1479,11 @@ paged_decode_attention_kernel(AttnArgs a) {
       if (hl == 0 && lane == 0) a.desc[range] = continued_desc(b0, grp, w0, w1, range);
       first_pass = false;
     }
-    if (i1 > i0)
+    if constexpr (Q4) {
+      if (i1 > i0)
+        attend_items4<DT, D, NBUF, false>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
+                                          i0, i1, false, 0);
+    } else if (i1 > i0)
       attend_items<DT, D, NBUF, false, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
                                               hl, b0, i0, i1, false, 0, -1, s_over, nstage,
                                               s_newseq[wave]);
@@ -1617,15 +1953,19 @@ int launch_combine(const AttnArgs& a, hipStream_t stream) {
   return AEGKV_OK;
 }
 
-template <int DT, int D, bool PLANNED, bool FUSED>
+template <int DT, int D, bool PLANNED, bool FUSED, bool Q4 = false>
 void launch_main(const AttnArgs& a, size_t lds, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, pipeline_depth<D>(), PLANNED, FUSED>),
+  constexpr int NBUF = Q4 ? kv4_pipeline_depth<D>() : pipeline_depth<D>();
+  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, Q4>),
                      dim3(a.n_wg), dim3(64 * kWaves), lds, stream, a);
 }
 
 template <int DT, int D>
-int launch_attention(const AttnArgs& a, size_t lds, hipStream_t stream) {
-  if (a.plan_wg) {
+int launch_attention(const AttnArgs& a, bool kv4, size_t lds, hipStream_t stream) {
+  if (kv4) {
+    if (a.plan_wg) launch_main<DT, D, true, false, true>(a, lds, stream);
+    else launch_main<DT, D, false, false, true>(a, lds, stream);
+  } else if (a.plan_wg) {
     if (a.knew) launch_main<DT, D, true, true>(a, lds, stream);
     else launch_main<DT, D, true, false>(a, lds, stream);
   } else {
@@ -1644,8 +1984,9 @@ int launch_attention(const AttnArgs& a, size_t lds, hipStream_t stream) {
 
 namespace aegkv {
 namespace {
-// Both entry points: `plan` (with plan_bytes) replaces the block tables when
-// given.
+// Every entry point: `plan` (with plan_bytes) replaces the block tables when
+// given; kv4: both caches are the 4-bit cache, cache_block_stride in units of
+// two bytes.
 // The new token's K/V rows of an appending call (none: key == nullptr).
 struct NewRows {
   const void* key = nullptr;
@@ -1661,7 +2002,7 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
                   int32_t max_seq_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                   int32_t block_size, float scale, int32_t dtype, int32_t n_workgroups,
                   void* workspace, uint64_t workspace_bytes, aegkv_stream_t stream,
-                  const NewRows& nr = NewRows()) {
+                  const NewRows& nr = NewRows(), bool kv4 = false) {
   if (batch < 0 || max_seq_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || max_blocks < 0 ||
       n_blocks < 0 || n_workgroups < 0)
     return AEGKV_ERR_INVALID_ARG;
@@ -1777,12 +2118,12 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
     }
     const size_t lds = lds_bytes(a, ds->max_lds);
     switch (head_dim) {
-      case 64: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 64>(a, lds, st)
-                       : launch_attention<AEGKV_DTYPE_FP16, 64>(a, lds, st); break;
-      case 128: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 128>(a, lds, st)
-                        : launch_attention<AEGKV_DTYPE_FP16, 128>(a, lds, st); break;
-      default: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 256>(a, lds, st)
-                       : launch_attention<AEGKV_DTYPE_FP16, 256>(a, lds, st); break;
+      case 64: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 64>(a, kv4, lds, st)
+                       : launch_attention<AEGKV_DTYPE_FP16, 64>(a, kv4, lds, st); break;
+      case 128: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 128>(a, kv4, lds, st)
+                        : launch_attention<AEGKV_DTYPE_FP16, 128>(a, kv4, lds, st); break;
+      default: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 256>(a, kv4, lds, st)
+                       : launch_attention<AEGKV_DTYPE_FP16, 256>(a, kv4, lds, st); break;
     }
     if (rc) return rc;
   }
@@ -2019,6 +2360,40 @@ int aegkv_paged_decode_attention_planned(void* out, int64_t out_batch_stride, co
                        cache_block_stride, n_blocks, nullptr, 0, plan, plan_bytes, seq_lens,
                        batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, block_size, scale,
                        dtype, n_workgroups, workspace, workspace_bytes, stream);
+}
+
+int aegkv_kv4_decode_attention(void* out, int64_t out_batch_stride, const void* q,
+                               int64_t q_batch_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* seq_lens, int32_t batch, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                               float scale, int32_t dtype, int32_t n_workgroups, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream) {
+  if (batch > 0 && !block_tables) return AEGKV_ERR_INVALID_ARG;
+  if (cache_block_stride & 15) return AEGKV_ERR_MISALIGNED;
+  return run_attention(out, out_batch_stride, q, q_batch_stride, cache, cache,
+                       cache_block_stride / 2, n_blocks, block_tables, max_blocks, nullptr, 0,
+                       seq_lens, batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize,
+                       scale, dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(),
+                       true);
+}
+
+int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, const void* q,
+                                       int64_t q_batch_stride, const void* cache,
+                                       int64_t cache_block_stride, int64_t n_blocks,
+                                       const void* plan, uint64_t plan_bytes,
+                                       const int32_t* seq_lens, int32_t batch,
+                                       int32_t max_seq_len, int32_t n_q_heads,
+                                       int32_t n_kv_heads, int32_t head_dim, float scale,
+                                       int32_t dtype, int32_t n_workgroups, void* workspace,
+                                       uint64_t workspace_bytes, aegkv_stream_t stream) {
+  if (batch > 0 && !plan) return AEGKV_ERR_INVALID_ARG;
+  if (cache_block_stride & 15) return AEGKV_ERR_MISALIGNED;
+  return run_attention(out, out_batch_stride, q, q_batch_stride, cache, cache,
+                       cache_block_stride / 2, n_blocks, nullptr, 0, plan, plan_bytes, seq_lens,
+                       batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize, scale,
+                       dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(), true);
 }
 
 }  // extern "C"

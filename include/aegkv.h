@@ -394,6 +394,76 @@ int aegkv_varlen_prefill_attention(void* out, int64_t out_token_stride, const vo
                                    int32_t head_dim, float scale, int32_t causal, int32_t dtype,
                                    aegkv_stream_t stream);
 
+/* ---- the 4-bit KV cache ----------------------------------------------------
+ * No counterpart in the reference, whose caches are 16-bit.  Blocks of 16
+ * tokens at 4.25 bits per value: 32 consecutive dims of a token's K or V row of
+ * a head share a scale byte.  With e the least integer for which the group's
+ * max|x| < 7 * 2^e, within [-125, 125] (bf16 rows) or [-125, 13] (fp16 rows), a
+ * value is stored as its sign and |x| / 2^e rounded to the nearest of 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 (ties to the even code, at most 6), the byte is e + 127, and
+ * the stored value is code * 2^e, exact in the rows' 16-bit type.  A group that
+ * holds an infinity or a NaN reads back as 32 NaNs (byte 255, codes 0).
+ *   A block of one layer and kv head is 17 * head_dim bytes, K's record before
+ *     V's: 8 * head_dim bytes of codes, then scale bytes [head_dim / 32][16
+ *     tokens].  A byte holds two dims, the lower in its low half.  K codes:
+ *     [chunk][16 tokens][16 bytes], a chunk being 32 consecutive dims (head_dim
+ *     64: 8 bytes, 16 dims).  V codes: [piece][4][16 lanes j][4 tokens][4 bytes],
+ *     token 4 x (second index) + (fourth), dims head_dim / 16 * j + 8 * piece
+ *     .. + 7 (head_dim 64: 2 bytes, 4 dims).
+ *   A layer's block holds its kv heads one after the other
+ *     (aegkv_kv4_block_bytes); storage [N][L][n_kv_heads][2][8.5 head_dim], so
+ *     the byte-moving entries (swap, copy, pack, scatter, defrag) and the block
+ *     manager take it as any pool with L * aegkv_kv4_block_bytes per block.
+ * head_dim 64, 128 or 256; strides of the cache in bytes, multiples of 16. */
+
+/* Bytes of one block of one layer: 17 * n_kv_heads * head_dim (or a status). */
+int64_t aegkv_kv4_block_bytes(int32_t n_kv_heads, int32_t head_dim);
+
+/* aegkv_kv_append into the 4-bit cache: key/value rows of `dtype` (strides in
+ * elements, the heads of a token dense), slots as there (negative ones and
+ * those past the pool are skipped).  The slots of one call must be distinct:
+ * rows written to one slot mix. */
+int aegkv_kv4_append(const void* key, const void* value, int64_t key_token_stride,
+                     int64_t value_token_stride, int64_t key_layer_stride,
+                     int64_t value_layer_stride, const int64_t* slot_mapping, int64_t n_tokens,
+                     void* cache, int64_t cache_block_stride, int64_t cache_layer_stride,
+                     int64_t n_blocks, int32_t n_layers, int32_t n_kv_heads, int32_t head_dim,
+                     int32_t dtype, aegkv_stream_t stream);
+
+/* aegkv_gather_tokens from the 4-bit cache: the values the codes stand for, in
+ * `dtype`, the type of the appended rows (a value past another type's range
+ * becomes an infinity or loses bits).  out_layer_stride in elements. */
+int aegkv_kv4_gather_tokens(const void* cache, int64_t cache_block_stride,
+                            int64_t cache_layer_stride, int64_t n_blocks,
+                            const int32_t* block_tables, int32_t max_blocks,
+                            const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t batch,
+                            int32_t max_seq_len, void* out_key, void* out_value,
+                            int64_t out_tokens, int64_t out_layer_stride, int32_t n_layers,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                            aegkv_stream_t stream);
+
+/* aegkv_paged_decode_attention over a layer of the 4-bit cache: its arguments,
+ * limits, workspace (aegkv_paged_decode_attention_workspace_size) and plans
+ * (aegkv_paged_decode_plan), with one cache in place of two.  q and out are of
+ * the type that the cache was written from. */
+int aegkv_kv4_decode_attention(void* out, int64_t out_batch_stride, const void* q,
+                               int64_t q_batch_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* seq_lens, int32_t batch, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                               float scale, int32_t dtype, int32_t n_workgroups, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream);
+int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, const void* q,
+                                       int64_t q_batch_stride, const void* cache,
+                                       int64_t cache_block_stride, int64_t n_blocks,
+                                       const void* plan, uint64_t plan_bytes,
+                                       const int32_t* seq_lens, int32_t batch,
+                                       int32_t max_seq_len, int32_t n_q_heads,
+                                       int32_t n_kv_heads, int32_t head_dim, float scale,
+                                       int32_t dtype, int32_t n_workgroups, void* workspace,
+                                       uint64_t workspace_bytes, aegkv_stream_t stream);
+
 /* ---- a8: node-wide block manager (host bookkeeping) ----------------------
  * Replaces the allocation and move bookkeeping of BlockManager
  * (aegaeon/aegaeon/block_manager.py:180-874).  Pure host code, no HIP calls;

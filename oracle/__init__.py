@@ -23,4 +23,7 @@ Pinning (what fixes each function independently of this file's formulas):
       scaled_dot_product_attention in float64 on the gathered K/V, plus the
       closed forms len=1 -> V0, equal keys -> mean(V), dominant logit -> V_argmax,
       GQA == MHA with repeated KV heads.
+  kv4_oracle (the 4-bit cache)             - hand-computed codes, scale bytes and
+      byte positions, every byte of a record written once
+      (tests/test_kv4.py).
 """
