@@ -22,7 +22,7 @@ LIB_PATH = PKG / "libaegkv.so"
 
 SOURCES = [
     "runtime.hip", "blocks.hip", "append.hip", "attention.hip", "inputs.hip",
-    "prefill.hip", "kv4.hip", "signals.hip", "block_manager.cpp",
+    "prefill.hip", "kv4.hip", "kv4_prefill.hip", "signals.hip", "block_manager.cpp",
 ]
 ARCH = "gfx950"
 

@@ -1,0 +1,750 @@
+// Attention of several query tokens per sequence over the paged 4-bit KV cache
+// (kv4_format.h) on gfx950: a prompt's next chunk over what is cached of it, or
+// drafted tokens.  Sequence b has queries [cu_seqlens[b], cu_seqlens[b + 1]),
+// m of them, the last of its seq_lens[b] = n cached tokens; query i attends to
+// keys j <= n - m + i (every key j < n when not causal).
+//
+// Rows.  The m queries of a sequence times the G query heads of one kv head
+// are rows r = i * G + (head in the group) that share that head's K and V.  32
+// consecutive rows are a wave's unit, W units a workgroup's tile.  A tile's
+// workgroup walks the sequence's keys 64 at a time: a wave loads one 16-token
+// block's codes into registers a tile ahead, converts them to 16 bits and
+// stores them to LDS, and every wave takes S = K.Q^T, the online softmax and
+// O += V^T.P^T of its rows from there (prefill_wave.h, 32x32x16 MFMA; P rounded
+// to 16 bits as in the prompt attention).  The conversion is shared by the
+// tile's W waves.
+//
+// Pieces.  When the batch has too few tiles to fill the chip, a tile's keys are
+// cut into pieces of a workgroup each, which write fp32 partials (O, running
+// maximum in log2 units, sum) that a second kernel merges.  The cut is the same
+// for a sequence's tiles: `splits` ranges of ceil(n_kt / splits) key tiles,
+// splits = ceil(n_kt / C), with one C for the batch that every workgroup
+// computes for itself: the batch's key tiles times row tiles divided by the
+// pieces wanted.
+#include <algorithm>
+#include <cmath>
+
+#include "aegkv_internal.h"
+#include "kv4_format.h"
+#include "prefill_wave.h"
+
+namespace aegkv {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kUnitRows = 32;   // rows of a wave
+constexpr int kTileBlocks = kPfKTile / kKv4Tokens;
+constexpr int kShortWaves4 = 4;
+constexpr int kMinSplitTiles = 4;  // least key tiles of a piece
+
+struct VarlenArgs {
+  const uint8_t* q;
+  uint8_t* out;
+  int64_t q_tok_b, o_tok_b;  // byte strides per token
+  const uint8_t* cache;
+  int64_t blk_b;             // byte stride per block
+  int64_t n_blocks;
+  const int32_t* tables;
+  int32_t max_blocks;
+  const int32_t* cu;         // [batch + 1]
+  const int32_t* seq_lens;   // [batch]
+  int32_t batch, n_kv_heads, group, max_q, max_len, causal;
+  int32_t token_bound;       // min(total query tokens, INT32_MAX)
+  FastDiv by_group;
+  float scale_log2;          // |softmax scale| * log2(e), > 0 (1 for 0)
+  int32_t scale_sign;        // of the scale: 1, -1 or 0
+  int64_t target;            // pieces wanted (0: no sequence is cut)
+  int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
+  float* part_o;             // [n_pieces][32 W][D]
+  float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
+};
+
+// What a sequence asks for, in tiles of W units.
+struct SeqWork {
+  int t0, m;        // first query token, queries (at most max_q)
+  int off;          // key position of query 0
+  int len;          // keys
+  int rows, tiles;  // rows of one kv head, row tiles
+  int n_kt;         // key tiles that its last row sees
+};
+template <int W>
+__device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
+  SeqWork s;
+  const int c0 = a.cu[b], c1 = a.cu[b + 1], n = max(a.seq_lens[b], 0);
+  s.t0 = min(max(c0, 0), a.token_bound);
+  const int m_all = min(max(c1, s.t0), a.token_bound) - s.t0;
+  s.m = min(m_all, a.max_q);
+  s.off = n - m_all;
+  s.len = min(n, a.max_len);
+  s.rows = s.m * a.group;
+  s.tiles = (s.rows + kUnitRows * W - 1) / (kUnitRows * W);
+  const int last = a.causal ? min(s.off + s.m, s.len) : s.len;  // keys of the last query
+  s.n_kt = s.m > 0 ? (max(last, 0) + kPfKTile - 1) / kPfKTile : 0;
+  return s;
+}
+
+// One piece of work: sequence, kv head, row tile, range of key tiles and slot
+// of the partials (-1: the whole range, straight to the output).
+struct Piece {
+  int b, head, tile, split, splits, span, first;  // first: the sequence's first piece
+};
+
+struct LocateLds {
+  int64_t cost[16];
+  int sum[16], pieces[16];
+  int found[5];
+};
+__device__ __forceinline__ int ranges_of(int n_kt, int span) {
+  return max(1, (n_kt + span - 1) / span);
+}
+// The piece (MERGE: the 32-row unit of a cut tile) numbered `index`, found by
+// all NT threads, each summing its own sequences.  False: there are fewer.
+template <int W, int NT, bool MERGE>
+__device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds& x, Piece& p) {
+  constexpr int NW = NT / 64;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int per = (a.batch + NT - 1) / NT, b0 = min(t * per, a.batch), b1 = min(b0 + per, a.batch);
+  int span = INT32_MAX;
+  if (a.target > 0) {  // uniform
+    int64_t cost = 0;
+    for (int b = b0; b < b1; ++b) {
+      const SeqWork s = seq_work<W>(a, b);
+      cost += (int64_t)s.tiles * s.n_kt;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) cost += __shfl_xor(cost, o);
+    if (lane == 0) x.cost[wave] = cost;
+    __syncthreads();
+    cost = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) cost += x.cost[w];
+    cost *= a.n_kv_heads;
+    span = (int)min((cost + a.target - 1) / a.target, (int64_t)INT32_MAX);
+    span = max(span, kMinSplitTiles);
+  }
+  int count = 0, before = 0;  // this thread's units, and its pieces
+  for (int b = b0; b < b1; ++b) {
+    const SeqWork s = seq_work<W>(a, b);
+    const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
+    before += n * r;
+    count += MERGE ? (r > 1 ? n * W : 0) : n * r;
+  }
+  int incl = count, pincl = before;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(incl, o), z = __shfl_up(pincl, o);
+    if (lane >= o) {
+      incl += y;
+      pincl += z;
+    }
+  }
+  if (lane == 63) {
+    x.sum[wave] = incl;
+    x.pieces[wave] = pincl;
+  }
+  if (t == 0) x.found[0] = -1;
+  __syncthreads();
+  int excl = incl - count, pexcl = pincl - before;
+  for (int w = 0; w < wave; ++w) {
+    excl += x.sum[w];
+    pexcl += x.pieces[w];
+  }
+  if (index >= excl && index < excl + count) {  // one thread
+    for (int b = b0; b < b1; ++b) {
+      const SeqWork s = seq_work<W>(a, b);
+      const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
+      const int c = MERGE ? (r > 1 ? n * W : 0) : n * r;
+      if (index < excl + c) {
+        x.found[0] = b;
+        x.found[1] = index - excl;
+        x.found[2] = r;
+        x.found[3] = (s.n_kt + r - 1) / r;
+        x.found[4] = pexcl;
+        break;
+      }
+      excl += c;
+      pexcl += n * r;
+    }
+  }
+  __syncthreads();
+  p.b = __builtin_amdgcn_readfirstlane(x.found[0]);
+  if (p.b < 0) return false;
+  const SeqWork s = seq_work<W>(a, p.b);
+  const int k = __builtin_amdgcn_readfirstlane(x.found[1]);
+  p.splits = __builtin_amdgcn_readfirstlane(x.found[2]);
+  p.span = __builtin_amdgcn_readfirstlane(x.found[3]);
+  p.first = __builtin_amdgcn_readfirstlane(x.found[4]);
+  // kv heads slowest, then row tiles from the last (the most keys) to the first
+  const int per_tile = MERGE ? W : p.splits;
+  const int q = k / per_tile;
+  p.split = k - q * per_tile;  // MERGE: the unit
+  p.head = q / s.tiles;
+  p.tile = s.tiles - 1 - (q - p.head * s.tiles);
+  return true;
+}
+
+#define KV4_BARRIER()                                  \
+  do {                                                 \
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); \
+    __builtin_amdgcn_s_barrier();                      \
+    asm volatile("" ::: "memory");                     \
+  } while (0)
+
+// The codes of one block for one lane, as in the decode attention.
+template <int D>
+struct CodeRegs {
+  uint32_t k[D / 32], v[D / 32], ks, vs;
+};
+template <int D>
+__device__ __forceinline__ void load_codes(CodeRegs<D>& c, __amdgpu_buffer_rsrc_t r, int lane) {
+  constexpr int REC = kv4_record_bytes(D), CODES = kv4_code_bytes(D);
+  const int j = lane & 15, g = lane >> 4;
+  if constexpr (D == 64) {
+    const u32x2 k = __builtin_amdgcn_raw_buffer_load_b64(r, 8 * lane, 0, 0);
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, REC + 8 * lane, 0, 0);
+    c.k[0] = k.x; c.k[1] = k.y;
+    c.v[0] = v.x; c.v[1] = v.y;
+  } else {
+    const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, 0, 0);
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, REC + 16 * lane, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c.k[i] = k[i];
+      c.v[i] = v[i];
+    }
+  }
+  c.ks = __builtin_amdgcn_raw_buffer_load_b8(r, CODES + (D == 64 ? g >> 1 : g) * kKv4Tokens + j, 0, 0);
+  c.vs = __builtin_amdgcn_raw_buffer_load_b32(
+      r, REC + CODES + (j * (D / 16) / kKv4Group) * kKv4Tokens + 4 * g, 0, 0);
+}
+
+// Rows of 2 D bytes in LDS, their 16-byte chunks permuted by the row so that the
+// operand reads hit distinct banks (as the prompt attention stores them).
+template <int D>
+__device__ __forceinline__ int k_chunk(int row, int c) {
+  return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int v_chunk(int row, int c) {
+  return D == 128 ? c ^ ((row & 3) << 2) : c ^ (((row >> 1) & 1) << 2);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void put_k(uint8_t* lds, const CodeRegs<D>& c, int u, int lane) {
+  using C = Kv4Elem<DT>;
+  constexpr int NW = D / 32;
+  const int j = lane & 15, g = lane >> 4, row = kKv4Tokens * u + j;
+  const float s = kv4_scale(c.ks);
+#pragma unroll
+  for (int i = 0; i < NW; ++i)
+    *reinterpret_cast<u32x4*>(lds + row * 2 * D + k_chunk<D>(row, NW * g + i) * 16) =
+        u32x4{C::template dq<0>(c.k[i], s), C::template dq<1>(c.k[i], s),
+              C::template dq<2>(c.k[i], s), C::template dq<3>(c.k[i], s)};
+}
+// V's tokens at or past `left` (of the block's 16) and its NaN groups are stored
+// as zeros, as a weight of zero does not undo a NaN; the groups are noted in
+// nan[D/32] (bit: token), which is written when the return value is true.
+template <int DT, int D>
+__device__ __forceinline__ bool put_v(uint8_t* lds, uint16_t* nan, CodeRegs<D>& c, int u, int left,
+                                      int lane) {
+  using C = Kv4Elem<DT>;
+  const int j = lane & 15, g = lane >> 4;
+  uint32_t e[4];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e[i] = (c.vs >> (8 * i)) & 0xffu;
+    if (4 * g + i >= left) {  // scale byte 0, and code bits 0 below
+      e[i] = 0;
+      if constexpr (D == 64) c.v[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+      else c.v[i] = 0;
+    }
+    bad |= e[i] == kKv4ScaleNan;
+  }
+  const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
+  if (any) {  // rare; uniform
+    uint64_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      at[i] = __builtin_amdgcn_ballot_w64(e[i] == kKv4ScaleNan);
+      if (e[i] == kKv4ScaleNan) e[i] = 0;  // finite whatever its codes
+    }
+    if (lane < D / 32) {  // group `lane`: lanes j = lane * 512 / D of each quad
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          m |= (uint32_t)(at[i] >> (16 * q + lane * (512 / D)) & 1) << (4 * q + i);
+      nan[lane] = (uint16_t)m;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = kKv4Tokens * u + 4 * g + i;
+    const float s = kv4_scale(e[i]);
+    if constexpr (D == 64) {
+      const uint32_t w = c.v[i >> 1];
+      const u32x2 x = i & 1 ? u32x2{C::template dq<2>(w, s), C::template dq<3>(w, s)}
+                            : u32x2{C::template dq<0>(w, s), C::template dq<1>(w, s)};
+      *reinterpret_cast<u32x2*>(lds + row * 2 * D + v_chunk<D>(row, j >> 1) * 16 + 8 * (j & 1)) = x;
+    } else {
+      const uint32_t w = c.v[i];
+      *reinterpret_cast<u32x4*>(lds + row * 2 * D + v_chunk<D>(row, j) * 16) =
+          u32x4{C::template dq<0>(w, s), C::template dq<1>(w, s), C::template dq<2>(w, s),
+                C::template dq<3>(w, s)};
+    }
+  }
+  return any;
+}
+
+// A wave's unit of 32 rows.
+template <int DT, int D>
+struct RowUnit : WaveSoftmax<DT, D> {
+  using Base = WaveSoftmax<DT, D>;
+  using Base::DB;
+  using Base::KS;
+  using Base::lsum;
+  using Base::m;
+  using Base::o;
+  using Base::qv;
+  int r0, rows;     // first row; the sequence's rows
+  int limit;        // last key of this lane's row (-1: none)
+  int lim_lo, lim_hi;  // of the unit's first and last row
+
+  __device__ __forceinline__ void init(const VarlenArgs& a, const SeqWork& s, int head, int unit) {
+    const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+    r0 = unit * kUnitRows;
+    rows = s.rows;
+    const int r = min(r0 + col, rows - 1);
+    const int i = a.by_group.div(r), h = head * a.group + r - i * a.group;
+    auto last_of = [&](int row) {
+      const int q = a.by_group.div(min(row, rows - 1));
+      return max(-1, a.causal ? min(s.off + q, s.len - 1) : s.len - 1);
+    };
+    limit = last_of(r);
+    lim_lo = last_of(r0);
+    lim_hi = r0 < rows ? last_of(r0 + kUnitRows - 1) : -1;
+    const uint8_t* qp = a.q + (int64_t)(s.t0 + i) * a.q_tok_b + ((int64_t)h * D + 8 * hh) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qv[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+    m = -INFINITY;
+    lsum = 0.f;
+  }
+  // the softmax's scale is positive: another one's sign goes into the queries
+  // (0: no query, every score 0)
+  __device__ __forceinline__ void sign_queries(int sign) {
+    if (sign > 0) return;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qv[ks][e] = sign < 0 ? qv[ks][e] ^ 0x80008000u : 0u;
+  }
+  __device__ __forceinline__ bool sees(int kt) const { return kt * kPfKTile <= lim_hi; }  // uniform
+
+  __device__ __forceinline__ void qk(const uint8_t* lds, f32x16 (&s)[2]) const {
+    const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+    const uint8_t* kp = lds + col * 2 * D;
+    const int kx = k_chunk<D>(col, hh) * 16;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[sb][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+        s[sb] = PfOps<DT>::mfma(
+            *reinterpret_cast<const u32x4*>(kp + (kx ^ (32 * ks)) + 32 * sb * 2 * D), qv[ks], s[sb]);
+  }
+  // -inf for keys past a row's last one and for unreadable blocks (bit u)
+  __device__ __forceinline__ void mask(f32x16 (&s)[2], int k0, uint32_t unreadable) const {
+    const int hh = (threadIdx.x & 63) >> 5;
+    if (k0 + kPfKTile - 1 > lim_lo) {
+      const int last = limit - k0 - 4 * hh;
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[sb][e] = last >= 32 * sb + 8 * (e >> 2) + (e & 3) ? s[sb][e] : -INFINITY;
+    }
+    if (unreadable) {
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[sb][e] = unreadable >> (2 * sb + (e >> 3)) & 1 ? -INFINITY : s[sb][e];
+    }
+  }
+  __device__ __forceinline__ void pv(const uint8_t* lds, const u32x4 (&pb)[4]) {
+    constexpr int RB = 2 * D;
+    const int lane = threadIdx.x & 63, G = lane >> 4, x = lane & 15;
+    const int key = 4 * (G >> 1) + (x >> 2);
+    const int vx = v_chunk<D>(key, 0) * 16;
+    const uint8_t* vp = lds + key * RB + (2 * (G & 1) + ((x & 3) >> 1)) * 16 + 8 * (x & 1);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint8_t* y = vp + (vx ^ (64 * db)) + 16 * kk * RB;
+        const u32x2 lo = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)y));
+        const u32x2 hi = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(y + 8 * RB)));
+        o[db] = PfOps<DT>::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[kk], o[db]);
+      }
+  }
+  // NaN to the dims of V's NaN groups (nan[block][group], bit: token) for the
+  // rows that see one of their tokens
+  __device__ __forceinline__ void spoil(const uint16_t (*nan)[D / 32], uint32_t blocks, int k0) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      int first = kPfKTile;  // the tile's first such key
+      for (int u = kTileBlocks - 1; u >= 0; --u)
+        if (blocks >> u & 1 && nan[u][db]) first = kKv4Tokens * u + __builtin_ctz(nan[u][db]);
+      const bool seen = first < kPfKTile && k0 + first <= limit;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = seen ? __builtin_nanf("") : o[db][e];
+    }
+  }
+  __device__ __forceinline__ float total() const { return lsum + __shfl_xor(lsum, 32); }
+
+  // normalise and store the rows (x: 32 rows of LDS of the wave's own), as the
+  // prompt attention does; rows without a key get zeros
+  __device__ __forceinline__ void store(const VarlenArgs& a, const SeqWork& s, uint8_t* x,
+                                        int head) const {
+    constexpr int RB = D * 2, CPR = D / 8, RPI = 64 / CPR;
+    const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+    const float lt = total();
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    uint8_t* xw = x + col * RB + 8 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x16& v = o[db];
+        *reinterpret_cast<u32x2*>(xw + ((4 * db + g) ^ (col % CPR)) * 16) =
+            u32x2{PfOps<DT>::pack(v[4 * g] * inv, v[4 * g + 1] * inv),
+                  PfOps<DT>::pack(v[4 * g + 2] * inv, v[4 * g + 3] * inv)};
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes
+    const int row = lane / CPR, pos = lane % CPR;
+#pragma unroll
+    for (int n = 0; n < 32 / RPI; ++n) {
+      const int r = RPI * n + row;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(x + 1024 * n + 16 * lane);
+      if (r0 + r < rows) {
+        const int i = a.by_group.div(r0 + r), h = head * a.group + r0 + r - i * a.group;
+        *reinterpret_cast<u32x4*>(a.out + (int64_t)(s.t0 + i) * a.o_tok_b + (int64_t)h * RB +
+                                  (pos ^ (r % CPR)) * 16) = v;
+      }
+    }
+  }
+  __device__ __forceinline__ void store_partial(const VarlenArgs& a, int64_t slot_row) const {
+    const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
+    const float lt = total();
+    if (r0 + col >= rows) return;
+    float* po = a.part_o + (slot_row + col) * D + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(po + 32 * db + 8 * g) =
+            f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    if (hh == 0) a.part_ml[slot_row + col] = make_float2(m, lt);
+  }
+};
+
+// W = 4: wave w converts block w of each key tile.
+template <int DT, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv4_varlen_kernel(VarlenArgs a) {
+  static_assert(W == kTileBlocks, "a block per wave");
+  constexpr int T_BYTES = kPfKTile * D * 2;
+  static_assert(W * kUnitRows * D * 2 <= 2 * T_BYTES, "the outputs fit the tiles");
+  __shared__ __align__(16) uint8_t lds[2 * T_BYTES];  // K, then V
+  __shared__ uint16_t s_nan[kTileBlocks][D / 32];
+  __shared__ uint32_t s_nan_any[kTileBlocks];
+  __shared__ LocateLds s_loc;
+  Piece p;
+  if (!locate<W, 64 * W, false>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  const SeqWork s = seq_work<W>(a, p.b);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n_blk = (s.len + kKv4Tokens - 1) / kKv4Tokens;
+  // the key tiles of this piece that the tile's last row sees
+  const int last_q = a.by_group.div(min(s.rows, (p.tile + 1) * W * kUnitRows) - 1);
+  const int keys = a.causal ? min(s.off + last_q + 1, s.len) : s.len;
+  const int kt0 = p.split * p.span;
+  const int kt1 = min(kt0 + p.span, (max(keys, 0) + kPfKTile - 1) / kPfKTile);
+
+  RowUnit<DT, D> unit;
+  unit.init(a, s, p.head, p.tile * W + w);
+  unit.sign_queries(a.scale_sign);
+
+  // block ids of 16 key tiles, one per lane, and the next 16
+  const int32_t* table = a.tables + (int64_t)p.b * a.max_blocks;
+  auto ids_from = [&](int blk) -> int { return table[min(blk + lane, n_blk - 1)]; };
+  const int64_t head_off = (int64_t)p.head * 17 * D;
+  int base = kt0 * kTileBlocks, ids = 0, ids_next = 0;
+  uint32_t unreadable = 0, unreadable_next = 0;
+  CodeRegs<D> c;
+  auto load = [&](int kt) {
+    const int blk = kt * kTileBlocks;
+    if (blk - base >= 64) {
+      ids = ids_next;
+      base += 64;
+      ids_next = ids_from(base + 64);
+    }
+    unreadable_next = 0;
+    bool mine = false;
+    int my_id = 0;
+#pragma unroll
+    for (int u = 0; u < kTileBlocks; ++u) {
+      const int id = __builtin_amdgcn_readlane(ids, blk - base + u);
+      const bool ok = blk + u < n_blk && id >= 0 && id < a.n_blocks;
+      if (blk + u < n_blk && !ok) unreadable_next |= 1u << u;
+      if (u == w) {
+        mine = ok;
+        my_id = id;
+      }
+    }
+    load_codes<D>(c, byte_range(a.cache + (int64_t)(mine ? my_id : 0) * a.blk_b + head_off,
+                                mine ? 17 * D : 0u), lane);
+  };
+  if (kt0 < kt1) {
+    ids = ids_from(base);
+    ids_next = ids_from(base + 64);
+    load(kt0);
+  }
+  for (int kt = kt0; kt < kt1; ++kt) {
+    if (kt > kt0) KV4_BARRIER();  // every wave's reads of the tile before
+    put_k<DT, D>(lds, c, w, lane);
+    const int left = s.len - (kt * kTileBlocks + w) * kKv4Tokens;
+    const bool any = put_v<DT, D>(lds + T_BYTES, s_nan[w], c, w, left, lane);
+    if (lane == 0) s_nan_any[w] = any;
+    unreadable = unreadable_next;
+    if (kt + 1 < kt1) load(kt + 1);
+    KV4_BARRIER();
+    if (unit.sees(kt)) {
+      f32x16 sc[2];
+      u32x4 pb[4];
+      unit.qk(lds, sc);
+      unit.mask(sc, kt * kPfKTile, unreadable);
+      unit.softmax(sc, pb, a.scale_log2, kt == kt0);
+      unit.pv(lds + T_BYTES, pb);
+      uint32_t nan = 0;
+#pragma unroll
+      for (int u = 0; u < kTileBlocks; ++u) nan |= s_nan_any[u] << u;
+      if (__builtin_amdgcn_readfirstlane(nan)) unit.spoil(s_nan, nan, kt * kPfKTile);
+    }
+  }
+  if (p.splits > 1) {
+    unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
+    return;
+  }
+  KV4_BARRIER();  // the tiles: every wave is past its last read of them
+  unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
+}
+
+// Merges the pieces of one 32-row unit of a cut tile:
+//   out = sum_s w_s o_s / sum_s w_s l_s,  w_s = 2^(m_s - max m);
+// eight threads per row, D / 8 columns each.
+constexpr int kMerge4Threads = 256;
+template <int DT, int D, int W>
+__global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(VarlenArgs a) {
+  __shared__ LocateLds s_loc;
+  Piece p;
+  if (!locate<W, kMerge4Threads, true>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  const SeqWork s = seq_work<W>(a, p.b);
+  const int row = (int)threadIdx.x >> 3, part = threadIdx.x & 7;
+  const int r = (p.tile * W + p.split) * kUnitRows + row;  // p.split: the unit
+  if (r >= s.rows) return;
+  // the tile's pieces follow each other (locate); those past the grid were not run
+  const int piece0 = p.first + (p.head * s.tiles + s.tiles - 1 - p.tile) * p.splits;
+  const int n = min(p.splits, a.n_pieces - piece0);
+  const int64_t row0 = ((int64_t)piece0 * W + p.split) * kUnitRows + row;
+  constexpr int64_t kStep = (int64_t)W * kUnitRows;  // slot rows from piece to piece
+  float mx = -INFINITY;
+  for (int k = 0; k < n; ++k) mx = fmaxf(mx, a.part_ml[row0 + k * kStep].x);
+  constexpr int NV = D / 32;
+  f32x4 acc[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float lt = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = a.part_ml[row0 + k * kStep];
+    const float* po = a.part_o + (row0 + k * kStep) * D + 4 * part;
+    f32x4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const f32x4*>(po + 32 * i);
+    // a piece without a key of this row: nothing
+    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
+    lt += ml.y * w;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] += v[i] * w;
+  }
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  const int i = a.by_group.div(r), h = p.head * a.group + r - i * a.group;
+  uint8_t* op = a.out + (int64_t)(s.t0 + i) * a.o_tok_b + ((int64_t)h * D + 4 * part) * 2;
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    *reinterpret_cast<u32x2*>(op + 64 * k) =
+        u32x2{PfOps<DT>::pack(acc[k][0] * inv, acc[k][1] * inv),
+              PfOps<DT>::pack(acc[k][2] * inv, acc[k][3] * inv)};
+}
+
+// The launch of a call: how many pieces at most, and whether sequences are cut.
+struct VarlenShape {
+  int64_t pieces;   // bound of the pieces (the main grid)
+  int64_t target;   // pieces wanted (0: uncut)
+  int64_t merge;    // bound of the merge's units
+  int64_t o_bytes, ml_bytes;
+};
+constexpr int kWorkgroupsPerCu4 = 2;
+
+int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
+                 int32_t n_kv_heads, int32_t head_dim, VarlenShape* out) {
+  constexpr int W = kShortWaves4;
+  DeviceState* ds = nullptr;
+  const int rc = current_device_state(&ds);
+  if (rc) return rc;
+  const int64_t group = n_q_heads / n_kv_heads, tile_rows = W * kUnitRows;
+  const int64_t max_tiles = ((int64_t)max_q * group + tile_rows - 1) / tile_rows;
+  // row tiles: those that the tokens fill, and a part-filled one per sequence
+  const int64_t tiles = std::min((int64_t)batch * max_tiles, total_q * group / tile_rows + batch);
+  const int64_t jobs = tiles * n_kv_heads;
+  const int64_t max_kt = ((int64_t)max_len + kPfKTile - 1) / kPfKTile;
+  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * kWorkgroupsPerCu4;
+  VarlenShape s{jobs, 0, 0, 0, 0};
+  if (jobs < 4 * slots && max_kt > kMinSplitTiles) {
+    s.target = 2 * slots;
+    // a sequence of cost x has at most x / span + its tiles
+    s.pieces = std::min(s.target + jobs, jobs * ((max_kt + kMinSplitTiles - 1) / kMinSplitTiles));
+    s.merge = jobs * W;
+    s.ml_bytes = s.pieces * tile_rows * 8;
+    s.o_bytes = s.pieces * tile_rows * head_dim * 4;
+  }
+  if (s.pieces > INT32_MAX / 2 || s.merge > INT32_MAX / 2) return AEGKV_ERR_UNSUPPORTED;
+  *out = s;
+  return AEGKV_OK;
+}
+
+int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
+                 int32_t n_kv_heads, int32_t head_dim, int32_t dtype) {
+  if (batch < 0 || total_q < 0 || max_q < 0 || max_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
+      n_q_heads % n_kv_heads)
+    return AEGKV_ERR_INVALID_ARG;
+  if ((head_dim != 64 && head_dim != 128) ||
+      (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16))
+    return AEGKV_ERR_UNSUPPORTED;
+  // rows of a sequence in 32 bits, a tile further
+  if ((int64_t)max_q * (n_q_heads / n_kv_heads) > INT32_MAX / 2 || max_len > INT32_MAX - kPfKTile)
+    return AEGKV_ERR_UNSUPPORTED;
+  return AEGKV_OK;
+}
+
+template <int DT, int D>
+int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
+  constexpr int W = kShortWaves4;
+  hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, W>), dim3((uint32_t)s.pieces), dim3(64 * W), 0, st, a);
+  AEGKV_HIP_TRY(hipGetLastError());
+  if (s.target > 0) {
+    hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W>), dim3((uint32_t)s.merge),
+                       dim3(kMerge4Threads), 0, st, a);
+    AEGKV_HIP_TRY(hipGetLastError());
+  }
+  return AEGKV_OK;
+}
+
+}  // namespace
+}  // namespace aegkv
+
+using namespace aegkv;
+
+extern "C" {
+
+int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q,
+                                                  int32_t max_seqlen_q, int32_t max_seq_len,
+                                                  int32_t n_q_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim, int32_t dtype) {
+  int rc = varlen_check(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
+                        dtype);
+  if (rc) return rc;
+  if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return 0;
+  VarlenShape s;
+  rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  if (rc) return rc > 0 ? AEGKV_ERR_RUNTIME : rc;
+  return s.o_bytes + s.ml_bytes;
+}
+
+int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* q,
+                               int64_t q_token_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* cu_seqlens_q, const int32_t* seq_lens, int32_t batch,
+                               int64_t total_q, int32_t max_seqlen_q, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                               int32_t causal, int32_t dtype, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream) {
+  int rc = varlen_check(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
+                        dtype);
+  if (rc) return rc;
+  if (max_blocks < 0 || n_blocks < 0 || !std::isfinite(scale)) return AEGKV_ERR_INVALID_ARG;
+  if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return AEGKV_OK;
+  if (!out || !q || !cache || !block_tables || !cu_seqlens_q || !seq_lens || n_blocks == 0)
+    return AEGKV_ERR_INVALID_ARG;
+  if (q_token_stride < (int64_t)n_q_heads * head_dim ||
+      out_token_stride < (int64_t)n_q_heads * head_dim)
+    return AEGKV_ERR_INVALID_ARG;
+  if (!aligned16(out) || !aligned16(q) || !aligned16(cache) || q_token_stride % 8 ||
+      out_token_stride % 8 || cache_block_stride % 16)
+    return AEGKV_ERR_MISALIGNED;
+  if (((int64_t)max_seq_len + kKv4Tokens - 1) / kKv4Tokens > max_blocks) return AEGKV_ERR_INVALID_ARG;
+  VarlenShape s;
+  rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  if (rc) return rc;
+  if (s.target > 0 && (!workspace || workspace_bytes < (uint64_t)(s.o_bytes + s.ml_bytes)))
+    return AEGKV_ERR_WORKSPACE;
+  if (s.target > 0 && !aligned16(workspace)) return AEGKV_ERR_MISALIGNED;
+  VarlenArgs a;
+  a.q = static_cast<const uint8_t*>(q);
+  a.out = static_cast<uint8_t*>(out);
+  a.q_tok_b = q_token_stride * 2;
+  a.o_tok_b = out_token_stride * 2;
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.blk_b = cache_block_stride;
+  a.n_blocks = n_blocks;
+  a.tables = block_tables;
+  a.max_blocks = max_blocks;
+  a.cu = cu_seqlens_q;
+  a.seq_lens = seq_lens;
+  a.batch = batch;
+  a.n_kv_heads = n_kv_heads;
+  a.group = n_q_heads / n_kv_heads;
+  a.max_q = max_seqlen_q;
+  a.max_len = max_seq_len;
+  a.causal = causal ? 1 : 0;
+  a.token_bound = (int32_t)std::min<int64_t>(total_q, INT32_MAX);
+  a.by_group = fast_div(a.group);
+  a.scale_sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
+  a.scale_log2 = scale == 0 ? 1.f : std::fabs(scale) * 1.4426950408889634f;
+  a.target = s.target;
+  a.n_pieces = (int32_t)s.pieces;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.o_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == AEGKV_DTYPE_BF16)
+    return head_dim == 64 ? launch_varlen<AEGKV_DTYPE_BF16, 64>(a, s, st)
+                          : launch_varlen<AEGKV_DTYPE_BF16, 128>(a, s, st);
+  return head_dim == 64 ? launch_varlen<AEGKV_DTYPE_FP16, 64>(a, s, st)
+                        : launch_varlen<AEGKV_DTYPE_FP16, 128>(a, s, st);
+}
+
+}  // extern "C"

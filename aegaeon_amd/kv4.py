@@ -25,7 +25,8 @@ import torch
 
 from . import _lib
 from ._gpu import StreamBuffer, device_guard, raw_stream, stream_buffer
-from .attention import _DTYPES, _OWN_WORKSPACE, DecodePlan, _check_on, _check_rows, _int32_dense
+from .attention import (_DTYPES, _OWN_WORKSPACE, DecodePlan, _check_on, _check_rows, _gpu,
+                        _int32_dense)
 
 BLOCK_SIZE = 16
 
@@ -276,3 +277,85 @@ def _check_workspace(workspace: torch.Tensor, nbytes: int, dev: torch.device) ->
     if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < nbytes:
         raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} bytes, "
                          f"the call needs {nbytes} in one piece")
+
+
+def varlen_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
+                         cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, max_seqlen_q: int,
+                         max_seq_len: int, scale: float, causal: bool = True,
+                         out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of several query tokens per sequence over one layer
+    ``kv_cache [N, Hkv, 2, R]`` of the 4-bit cache: ``q [T, Hq, D]`` (any token
+    stride, dense heads) -> ``out [T, Hq, D]``, both of the type the cache was
+    written from.  Sequence b's queries are ``cu_seqlens_q[b] ..
+    cu_seqlens_q[b + 1]`` (int32 on the GPU), the last of its ``seq_lens[b]``
+    cached tokens (append them first); query i of m attends to keys ``j <=
+    seq_lens[b] - m + i``, all of them when not ``causal``, and gives zeros
+    without any.  ``max_seqlen_q`` and ``max_seq_len`` are host bounds: queries
+    past the first are left alone, keys past the second not attended.  head_dim
+    64 or 128.  ``workspace``: :func:`varlen_attention_workspace` (reusable on
+    one stream, by one thread at a time); by default one per (device, stream)
+    that threads may share."""
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens, Hq, D]")
+    _check_rows(q, "q")
+    if q.dtype not in _DTYPES:
+        raise ValueError("q must be bf16 or fp16")
+    T, Hq, D = q.shape
+    dev = q.device
+    _check_cache(kv_cache, False, D)
+    _check_on(kv_cache, "kv_cache", dev)
+    _check_on(block_tables, "block_tables", dev)
+    _check_on(seq_lens, "seq_lens", dev)
+    B = seq_lens.numel()
+    if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.size(0) != B:
+        raise ValueError("block_tables must be [B, max_blocks] and seq_lens [B]")
+    _check_cu(cu_seqlens_q, "cu_seqlens_q", B, dev)
+    out = _check_out(out, q)
+    if B == 0 or T == 0:
+        return out
+    bt, sl = _int32_dense(block_tables), _int32_dense(seq_lens)
+    lib = _lib.load()
+    sizes = (int(max_seqlen_q), int(max_seq_len), Hq, kv_cache.size(1), D)
+    dtype = _DTYPES[q.dtype]
+    with device_guard(dev):
+        ws_bytes = lib.aegkv_kv4_varlen_attention_workspace_size(B, T, *sizes, dtype)
+        if ws_bytes < 0:
+            _lib.check(int(ws_bytes), "varlen_attention_workspace")
+        stream = raw_stream(dev)
+        shared = None
+        if workspace is not None:
+            _check_workspace(workspace, ws_bytes, dev)
+        elif ws_bytes > 0:
+            shared = _own_workspace(dev, stream)
+        with _OWN_WORKSPACE if shared is None else shared.lock:
+            if shared is not None:
+                workspace = shared.at_least(ws_bytes, dev)
+            elif workspace is None and ws_bytes > 0:
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            rc = lib.aegkv_kv4_varlen_attention(
+                out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), kv_cache.data_ptr(),
+                kv_cache.stride(0), kv_cache.size(0), bt.data_ptr(), bt.size(1),
+                cu_seqlens_q.data_ptr(), sl.data_ptr(), B, T, *sizes, float(scale),
+                int(bool(causal)), dtype, workspace.data_ptr() if ws_bytes > 0 else None, ws_bytes,
+                stream)
+    _lib.check(rc, "varlen_attention_kv4")
+    return out
+
+
+def varlen_attention_workspace(batch: int, total_q: int, max_seqlen_q: int, max_seq_len: int,
+                               n_q_heads: int, n_kv_heads: int, head_dim: int,
+                               dtype: torch.dtype = torch.bfloat16,
+                               device=None) -> Optional[torch.Tensor]:
+    """A workspace for :func:`varlen_attention_kv4` calls of exactly these
+    sizes on ``device`` (None when they need none)."""
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be bfloat16 or float16")
+    dev = _gpu(device)
+    with device_guard(dev):
+        n = _lib.load().aegkv_kv4_varlen_attention_workspace_size(
+            batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
+            _DTYPES[dtype])
+    if n < 0:
+        _lib.check(int(n), "varlen_attention_workspace")
+    return torch.empty(int(n), dtype=torch.uint8, device=dev) if n > 0 else None

@@ -464,6 +464,38 @@ int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, cons
                                        int32_t dtype, int32_t n_workgroups, void* workspace,
                                        uint64_t workspace_bytes, aegkv_stream_t stream);
 
+/* Attention of several query tokens per sequence over a layer of the 4-bit
+ * cache: a prompt's next chunk over what is cached of it (its own rows appended
+ * first), or drafted tokens.  q/out [total_q][n_q_heads][head_dim] (DEVICE,
+ * token strides in elements, the heads of a token contiguous); sequence b's m
+ * queries are tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (DEVICE int32 [batch
+ * + 1], not decreasing: the grid counts on sequences that share no tokens), the
+ * last m of its seq_lens[b] = n cached tokens.  Query i attends to keys
+ * j <= n - m + i (every j < n when causal is 0), softmax(scale * q.k) in fp32
+ * with P rounded to 16 bits before P.V (any finite scale); without such a key
+ * it gives zeros.  Queries past max_seqlen_q of a sequence are left alone; keys
+ * past max_seq_len are not attended; tokens are clamped to [0, total_q).  A
+ * block id outside [0, n_blocks) is never dereferenced: its tokens are masked.
+ * An infinity or NaN that was appended shows in the rows that attend to its
+ * token, and in no others.
+ *   workspace: DEVICE scratch of aegkv_kv4_varlen_attention_workspace_size(...)
+ *     bytes (0: none) for the partials of sequences whose keys several
+ *     workgroups share; used as aegkv_paged_decode_attention's.
+ * head_dim 64 or 128, n_q_heads a multiple of n_kv_heads. */
+int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q,
+                                                  int32_t max_seqlen_q, int32_t max_seq_len,
+                                                  int32_t n_q_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim, int32_t dtype);
+int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* q,
+                               int64_t q_token_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* cu_seqlens_q, const int32_t* seq_lens, int32_t batch,
+                               int64_t total_q, int32_t max_seqlen_q, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                               int32_t causal, int32_t dtype, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream);
+
 /* ---- a8: node-wide block manager (host bookkeeping) ----------------------
  * Replaces the allocation and move bookkeeping of BlockManager
  * (aegaeon/aegaeon/block_manager.py:180-874).  Pure host code, no HIP calls;

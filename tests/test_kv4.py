@@ -219,6 +219,34 @@ def test_decode_host_checks(lib):
     assert planned(bs=8) == MISALIGNED
 
 
+def test_varlen_host_checks(lib):
+    raw, p = _buf(1 << 12)
+
+    def call(out=p, q=p, cache=p, tables=p, cu=p, qs=28 * 128, os_=28 * 128, bs=17 * 512, blocks=8,
+             max_blocks=4, batch=1, total=16, max_q=16, longest=64, hq=28, hkv=4, d=128, scale=0.1,
+             dt=0, ws=p, wsb=1 << 40):
+        return lib.aegkv_kv4_varlen_attention(out, os_, q, qs, cache, bs, blocks, tables, max_blocks,
+                                              cu, p, batch, total, max_q, longest, hq, hkv, d,
+                                              scale, 1, dt, ws, wsb, None)
+
+    assert call(hkv=5) == INVALID                  # Hq not a multiple of Hkv
+    assert call(d=256) == UNSUP and call(d=32) == UNSUP and call(dt=7) == UNSUP
+    assert call(scale=float("nan")) == INVALID and call(scale=float("inf")) == INVALID
+    assert call(batch=-1) == INVALID and call(longest=-1) == INVALID and call(max_q=-1) == INVALID
+    assert call(batch=0, q=None) == OK and call(total=0) == OK and call(max_q=0) == OK
+    assert call(q=None) == INVALID and call(cache=None) == INVALID and call(tables=None) == INVALID
+    assert call(cu=None) == INVALID and call(blocks=0) == INVALID
+    assert call(qs=27 * 128) == INVALID and call(os_=27 * 128) == INVALID
+    assert call(q=p + 2) == MISALIGNED and call(os_=28 * 128 + 4) == MISALIGNED
+    assert call(bs=17 * 512 + 8) == MISALIGNED
+    assert call(longest=65) == INVALID             # five blocks, the table has four
+    assert call(max_q=1 << 30) == UNSUP            # rows past 32 bits
+    size = lib.aegkv_kv4_varlen_attention_workspace_size
+    assert size(0, 0, 0, 64, 28, 4, 128, 0) == 0
+    assert size(1, 16, 16, 64, 28, 5, 128, 0) == INVALID
+    assert size(1, 16, 16, 64, 28, 4, 256, 0) == UNSUP
+
+
 def test_python_entry_points_refuse_host_tensors():
     cache = kv4.kv4_cache(3, 2, 4, 128, device="cpu")
     assert cache.shape == (3, 2, 4, 2, 1088) and not cache.any()
@@ -234,3 +262,7 @@ def test_python_entry_points_refuse_host_tensors():
     with pytest.raises(ValueError):
         kv4.paged_decode_attention_kv4(x[0], cache[:, 0], torch.zeros(5, 1, dtype=torch.int32),
                                        torch.ones(5, dtype=torch.int32), 0.1, 1)
+    with pytest.raises(ValueError):
+        kv4.varlen_attention_kv4(x[0], cache[:, 0], torch.zeros(1, 1, dtype=torch.int32),
+                                 torch.zeros(2, dtype=torch.int32),
+                                 torch.ones(1, dtype=torch.int32), 1, 1, 0.1)
