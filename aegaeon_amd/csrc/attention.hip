@@ -242,6 +242,8 @@ struct AttnArgs {
   int32_t n_ranges;  // n_wg * kWaves / heads
   RangeRule ranges;  // how many of them take part
   float scale_log2;  // softmax scale * log2(e)
+  int32_t scale_sign;        // 4-bit cache: its sign, 1, -1 or 0
+  float abs_scale_log2;      // and magnitude (1 for 0)
   int32_t max_seq_len;  // host bound; longer device lengths are clamped to it
   uint16_t* out;
   int64_t out_bstride;  // elements
@@ -515,19 +517,36 @@ __device__ __forceinline__ void compute_block(KVRegs<D>& r, const u32x4* qv, f32
 }
 
 // ---- the 4-bit cache (kv4_format.h) ----
-// Codes and scale bytes of one block for one lane (j, g): K token j, whose
-// words hold 8 dims each of the chunks g (and, D = 256, 4 + g); V tokens 4g ..
-// 4g + 3, dims D/16 j .. of each.  The contraction over the head dim runs in
-// the codes' order: k-step ks takes the lane's word ks, dims kv4_dim(ks, g) ..
-// + 7, of K and of the query alike.
+// K and V are converted to 16 bits, where code times scale is exact, so nothing
+// past the conversion differs from the 16-bit cache's arithmetic.  Per block of
+// 16 tokens, with lane l = 16 g + j:
+//   S^T[16 tok x 16 heads] = K . Q^T: a word of codes converts to the 16-bit
+//     MFMA's operand, so the contraction runs in the codes' order: k-step ks
+//     takes the lane's word ks, dims kv4_dim(ks, g) .. + 7 of K and of the query
+//     alike.  (The scaled MFMA 16x16x128 would take codes and scale bytes as they
+//     lie in memory, with the query in 8-bit parts, but sums its 128 products
+//     with some 15 bits: errors of 1e-5 of the sum of their magnitudes.)
+//   O^T[D x 16 heads] += V^T . P^T: a byte of codes converts to the two
+//     neighbouring dims of one token in one register; the operand V^T[16 dim
+//     pairs x 32] takes those registers as they are, the contraction running
+//     over (token, dim of the pair), with P^T's entries of the pair's other dim
+//     zero: one product gives the even dims, one with P moved to the other
+//     entries the odd ones.  P is split into a 16-bit high part and the
+//     remainder's, as above.  (Operands of one dim each took two permutes per
+//     conversion and copies of V for both parts of P.)
+
+// Codes and scale bytes of one block for one lane: K token j, dims 32 g .. (D =
+// 64: 16 g ..; D = 256: and 128 + 32 g ..); V tokens 4g .. 4g + 3, dims D/16 j ..
+// of each.
 template <int D>
 struct KV4Regs {
-  static constexpr int KS = D / 32;  // QK k-steps: words of K codes per lane
+  static constexpr int NW = D / 32;  // words of codes
   static constexpr int NS = D >= 256 ? 2 : 1;
-  uint32_t k[KS], v[KS];  // D = 64: a word of V holds two tokens' four codes
-  uint32_t ks[NS];        // scale byte of the K words (each NS-th part of them)
+  uint32_t k[NW], v[NW];  // D = 64: a word of V holds two tokens' four codes
+  uint32_t ks[NS];        // scale byte of each NS-th part of the K words
   uint32_t vs;            // scale bytes of the four V tokens
 };
+
 template <int D>
 __device__ __forceinline__ int kv4_dim(int ks, int g) {
   return 128 * (ks >> 2) + (D == 64 ? 16 : 32) * g + 8 * (ks & 3);
@@ -563,26 +582,60 @@ __device__ __forceinline__ void load_block4(KV4Regs<D>& b, __amdgpu_buffer_rsrc_
       r, REC + CODES + (j * (D / 16) / kKv4Group) * kBlockSize + 4 * g, 0, kNt);
 }
 
-// A step of up to kStep4 consecutive blocks of one sequence, its first token
+// The lane's value and those of the lanes 16 and 32 away, the largest: all
+// four lanes (j, *) get it.
+__device__ __forceinline__ float max_over_g(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t w = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// P's operands for the pair's even (low half) and odd dim, of its high part and
+// of the remainder's.
+template <int DT>
+struct Weights4 {
+  u32x4 even_hi, odd_hi, even_lo, odd_lo;
+  __device__ __forceinline__ void set(int c, float p) {
+    if constexpr (DT == AEGKV_DTYPE_BF16) {  // the top 16 bits: p - hi is exact
+      const uint32_t u = __float_as_uint(p);
+      odd_hi[c] = u & 0xffff0000u;
+      even_hi[c] = u >> 16;
+      const uint32_t r = __float_as_uint(p - __uint_as_float(u & 0xffff0000u));
+      odd_lo[c] = r & 0xffff0000u;
+      even_lo[c] = r >> 16;
+    } else {
+      uint32_t hi, lo;
+      Elem<DT>::split(p, hi, lo);
+      even_hi[c] = hi;
+      odd_hi[c] = hi << 16;
+      even_lo[c] = lo;
+      odd_lo[c] = lo << 16;
+    }
+  }
+};
+
+// A step of up to step4() consecutive blocks of one sequence, its first token
 // tok0: the softmax update and P.V of compute_block, with one maximum and one
-// rescale test for all of them.  K and V are converted to 16 bits, where every
-// code times its scale is exact, so nothing past the conversion differs from
-// the 16-bit cache's arithmetic.  Tokens at or past `limit` are masked, and the
+// rescale test for all of them.  Tokens at or past `limit` are masked, and the
 // blocks whose bit in `skip` is set (unreadable ids, and those past the step).
-constexpr int kStep4 = 4;
+template <int D>
+constexpr int step4() { return D >= 256 ? 2 : 4; }
 template <int DT, int D>
-__device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[kStep4], const u32x4* qv, f32x4* acc,
-                                              float& m, float& lsum, int tok0, int limit,
-                                              uint32_t skip, int g, float scale_log2) {
+__device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const u32x4* qv,
+                                              f32x4* acc, float& m, float& lsum, int tok0,
+                                              int limit, uint32_t skip, int g, float scale_log2) {
   using E = Elem<DT>;
   using C = Kv4Elem<DT>;
-  constexpr int KS = KV4Regs<D>::KS;
+  constexpr int kStep4 = step4<D>();
   f32x4 sc[kStep4];
 #pragma unroll
   for (int u = 0; u < kStep4; ++u) {
     sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
+    for (int ks = 0; ks < KV4Regs<D>::NW; ++ks) {
       const float s = kv4_scale(r[u].ks[ks >> 2]);
       const uint32_t w = r[u].k[ks];
       sc[u] = E::mfma(u32x4{C::template dq<0>(w, s), C::template dq<1>(w, s),
@@ -590,88 +643,83 @@ __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[kStep4], const u32
                       qv[ks], sc[u]);
     }
   }
-  const int last = limit - tok0 - 4 * g;  // this lane's tokens 16 u + i below it
-  float x[kStep4][4];
+  if (skip != 0 || tok0 + 16 * kStep4 > limit) {  // uniform
+    const int last = limit - tok0 - 4 * g;  // this lane's tokens 16 u + i below it
+#pragma unroll
+    for (int u = 0; u < kStep4; ++u) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sc[u][i] = (16 * u + i < last && !(skip >> u & 1)) ? sc[u][i] : -INFINITY;
+      // V's stale bytes, maybe the scale byte of NaN: scale byte and codes zero,
+      // which reads as zero
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool keep = 16 * u + c < last;
+        r[u].vs = keep ? r[u].vs : r[u].vs & ~(0xffu << (8 * c));
+        if constexpr (D == 64) {
+          r[u].v[c >> 1] = keep ? r[u].v[c >> 1]
+                                : r[u].v[c >> 1] & (c & 1 ? 0x0000ffffu : 0xffff0000u);
+        } else {
+#pragma unroll
+          for (int f = 0; f < D / 128; ++f) r[u].v[4 * f + c] = keep ? r[u].v[4 * f + c] : 0u;
+        }
+      }
+    }
+  }
+  float bm = sc[0][0];
 #pragma unroll
   for (int u = 0; u < kStep4; ++u)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[u][i] = (16 * u + i < last && !(skip >> u & 1)) ? sc[u][i] * scale_log2 : -INFINITY;
-  float bm = x[0][0];
-#pragma unroll
-  for (int u = 0; u < kStep4; ++u)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bm = fmaxf(bm, x[u][i]);
-  bm = fmaxf(bm, __shfl_xor(bm, 16));
-  bm = fmaxf(bm, __shfl_xor(bm, 32));
+    for (int i = 0; i < 4; ++i) bm = fmaxf(bm, sc[u][i]);
+  bm = max_over_g(bm) * scale_log2;
   if (__builtin_amdgcn_ballot_w64(bm > m + kRescaleSlack)) {  // lazy rescaling, as in compute_block
     const float mn = fmaxf(m, bm);
-    const float alpha = __builtin_amdgcn_exp2f(m - mn);  // 0 while m = -inf
+    // 0 while m = -inf (beside another head's first finite score too)
+    const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
     lsum *= alpha;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) acc[t] *= alpha;
     m = mn;
   }
-  const float ms = m == -INFINITY ? 0.f : m;  // -inf only while every token is masked
+  const float nms = m == -INFINITY ? 0.f : -m;  // -inf only while every token is masked
 #pragma unroll
   for (int u = 0; u < kStep4; ++u) {
+    Weights4<DT> w;
     float p[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(x[u][i] - ms);
-    lsum += (p[0] + p[1]) + (p[2] + p[3]);
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) E::split(p[i], hi[i], lo[i]);
-    const u32x4 bop = {hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16), lo[0] | (lo[1] << 16),
-                       lo[2] | (lo[3] << 16)};
-    // tokens past the end hold stale bytes, maybe the scale byte of NaN: scale
-    // byte zero and codes zero read as zero
-    uint32_t vs = r[u].vs;
-    uint32_t v[KS];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) v[i] = r[u].v[i];
-    if (tok0 + 16 * (u + 1) > limit) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool keep = 16 * u + c < last;
-        vs = keep ? vs : vs & ~(0xffu << (8 * c));
-        if constexpr (D == 64) {
-          v[c >> 1] = keep ? v[c >> 1] : v[c >> 1] & (c & 1 ? 0x0000ffffu : 0xffff0000u);
-        } else {
-#pragma unroll
-          for (int f = 0; f < D / 128; ++f) v[4 * f + c] = keep ? v[4 * f + c] : 0u;
-        }
-      }
+    for (int i = 0; i < 4; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], scale_log2, nms));
+      w.set(i, p[i]);
     }
-    float s[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s[c] = kv4_scale((vs >> (8 * c)) & 0xffu);
-    // dims t and t + 1 (t even) of the four tokens -> the tokens of each dim
-    auto tile_pair = [&](int t, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
-      const uint32_t e0 = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
-      const uint32_t e1 = __builtin_amdgcn_perm(x3, x2, 0x05040100u);
-      const uint32_t o0 = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
-      const uint32_t o1 = __builtin_amdgcn_perm(x3, x2, 0x07060302u);
-      acc[t] = E::mfma(u32x4{e0, e1, e0, e1}, bop, acc[t]);
-      acc[t + 1] = E::mfma(u32x4{o0, o1, o0, o1}, bop, acc[t + 1]);
+    lsum += (p[0] + p[1]) + (p[2] + p[3]);
+    // the conversions read a scale's exponent bits alone: its byte is shifted
+    // there and its neighbours are left in place
+    const uint32_t vs = r[u].vs;
+    const float s[4] = {__uint_as_float(vs << 23), __uint_as_float(vs << 15),
+                        __uint_as_float(vs << 7), __uint_as_float(vs >> 1)};
+    auto pair = [&](int t, u32x4 x) {  // dims t (even) and t + 1
+      acc[t] = E::mfma(x, w.even_hi, acc[t]);
+      acc[t + 1] = E::mfma(x, w.odd_hi, acc[t + 1]);
+      acc[t] = E::mfma(x, w.even_lo, acc[t]);
+      acc[t + 1] = E::mfma(x, w.odd_lo, acc[t + 1]);
     };
+    const uint32_t* v = r[u].v;
     if constexpr (D == 64) {
-      tile_pair(0, C::template dq<0>(v[0], s[0]), C::template dq<2>(v[0], s[1]),
-                C::template dq<0>(v[1], s[2]), C::template dq<2>(v[1], s[3]));
-      tile_pair(2, C::template dq<1>(v[0], s[0]), C::template dq<3>(v[0], s[1]),
-                C::template dq<1>(v[1], s[2]), C::template dq<3>(v[1], s[3]));
+      pair(0, u32x4{C::template dq<0>(v[0], s[0]), C::template dq<2>(v[0], s[1]),
+                    C::template dq<0>(v[1], s[2]), C::template dq<2>(v[1], s[3])});
+      pair(2, u32x4{C::template dq<1>(v[0], s[0]), C::template dq<3>(v[0], s[1]),
+                    C::template dq<1>(v[1], s[2]), C::template dq<3>(v[1], s[3])});
     } else {
 #pragma unroll
-      for (int f = 0; f < D / 128; ++f) {
-        const uint32_t* w = v + 4 * f;
-        tile_pair(8 * f + 0, C::template dq<0>(w[0], s[0]), C::template dq<0>(w[1], s[1]),
-                  C::template dq<0>(w[2], s[2]), C::template dq<0>(w[3], s[3]));
-        tile_pair(8 * f + 2, C::template dq<1>(w[0], s[0]), C::template dq<1>(w[1], s[1]),
-                  C::template dq<1>(w[2], s[2]), C::template dq<1>(w[3], s[3]));
-        tile_pair(8 * f + 4, C::template dq<2>(w[0], s[0]), C::template dq<2>(w[1], s[1]),
-                  C::template dq<2>(w[2], s[2]), C::template dq<2>(w[3], s[3]));
-        tile_pair(8 * f + 6, C::template dq<3>(w[0], s[0]), C::template dq<3>(w[1], s[1]),
-                  C::template dq<3>(w[2], s[2]), C::template dq<3>(w[3], s[3]));
+      for (int f = 0; f < D / 128; ++f, v += 4) {
+        pair(8 * f + 0, u32x4{C::template dq<0>(v[0], s[0]), C::template dq<0>(v[1], s[1]),
+                              C::template dq<0>(v[2], s[2]), C::template dq<0>(v[3], s[3])});
+        pair(8 * f + 2, u32x4{C::template dq<1>(v[0], s[0]), C::template dq<1>(v[1], s[1]),
+                              C::template dq<1>(v[2], s[2]), C::template dq<1>(v[3], s[3])});
+        pair(8 * f + 4, u32x4{C::template dq<2>(v[0], s[0]), C::template dq<2>(v[1], s[1]),
+                              C::template dq<2>(v[2], s[2]), C::template dq<2>(v[3], s[3])});
+        pair(8 * f + 6, u32x4{C::template dq<3>(v[0], s[0]), C::template dq<3>(v[1], s[1]),
+                              C::template dq<3>(v[2], s[2]), C::template dq<3>(v[3], s[3])});
       }
     }
   }
@@ -1120,7 +1168,7 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
 }
 
 // attend_items over the 4-bit cache: the same items, ids, pieces and records,
-// in steps of up to kStep4 blocks that end where a piece does.  The step that
+// in steps of up to step4() blocks that end where a piece does.  The step that
 // is loaded is NSET - 1 steps ahead of the one computed, across sequences: the
 // load side keeps a sequence position of its own, and hands a step's to the
 // compute side with its registers.  Past the range a step loads nothing (empty
@@ -1130,8 +1178,7 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
                                               const int32_t* s_len, uint8_t* stage, int4* meta,
                                               int range, int grp, int hl, int b0, int i0, int i1,
                                               bool have_first, int id_first) {
-  constexpr int KS = D / 32;
-  constexpr int DPL = D / 16;
+  constexpr int KS = D / 32, DPL = D / 16, kStep4 = step4<D>();
   const int lane = threadIdx.x & 63;
   const int h = grp * a.heads + hl;
   if (h >= a.n_kv_heads) return;  // wave past the last kv head (uniform)
@@ -1159,12 +1206,20 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
     while (uni(s_bcum[b + 1]) == uni(s_bcum[b])) ++b;
     return b;
   };
-  auto load_q = [&](int b, u32x4* qv) {  // lanes past the group load its first head
+  // lanes past the group load its first head; the softmax's scale is positive,
+  // another one's sign goes into the query (0: no query, every score 0)
+  auto load_q = [&](int b, u32x4* qv) {
     const uint16_t* qp =
         a.q + (int64_t)b * a.q_bstride + (int64_t)(head_ok ? hq : h * a.group) * D;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       qv[ks] = *reinterpret_cast<const u32x4*>(qp + kv4_dim<D>(ks, g));
+    if (a.scale_sign <= 0) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qv[ks][i] = a.scale_sign < 0 ? qv[ks][i] ^ 0x80008000u : 0u;
+    }
   };
 
   // the load side: sequence bl, whose items in range end at lend; next item il
@@ -1206,7 +1261,6 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   int bc = b0, first = uni(s_bcum[b0]), cend = lend, len = uni(s_len[b0]), ic = i0;
   bool complete = first >= i0 && cend == uni(s_bcum[b0 + 1]);
   u32x4 qv[KS];
-  load_q(bc, qv);
   f32x4 acc[DPL];
 #pragma unroll
   for (int t = 0; t < DPL; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1231,7 +1285,7 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   };
   auto compute = [&](KV4Regs<D> (&r)[kStep4], const Step& s) {
     compute_step4<DT, D>(r, qv, acc, m, lsum, (ic - first) * kBlockSize,
-                         min(len, (cend - first) * kBlockSize), s.skip, g, a.scale_log2);
+                         min(len, (cend - first) * kBlockSize), s.skip, g, a.abs_scale_log2);
     ic += s.n;
     if (ic == cend) {  // the piece of sequence bc in this range ends (uniform)
       float lt = lsum + __shfl_xor(lsum, 16);
@@ -1264,6 +1318,7 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
     load_step(buf[decltype(kc)::value], st[decltype(kc)::value]);
     return false;
   });
+  load_q(bc, qv);  // behind the first steps' loads
   bool more = true;
   while (more) {
     unrolled_steps<NSET>([&](auto kc) {
@@ -2062,6 +2117,8 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
   a.n_ranges = n_ranges;
   a.ranges = range_rule(n_wg, n_kv_heads, heads);
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_sign = scale < 0.f ? -1 : scale == 0.f ? 0 : 1;
+  a.abs_scale_log2 = scale == 0.f ? 1.f : std::fabs(a.scale_log2);
   a.max_seq_len = max_seq_len;
   a.q_bstride = q_batch_stride;
   a.out_bstride = out_batch_stride;
