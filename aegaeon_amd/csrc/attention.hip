@@ -593,26 +593,77 @@ __device__ __forceinline__ float max_over_g(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// P's operands for the pair's even (low half) and odd dim, of its high part and
-// of the remainder's.
-template <int DT>
+// The 16 columns of P^T's operand.  A product for the even dims and one for the
+// odd, of P's high part and of the remainder's, are four per operand of V; with
+// 8 query heads per kv head or fewer half the columns would be copies, so
+// PACK = 2 gives the columns 8 + head to the remainder's part and needs two
+// products, and PACK = 4 (4 heads or fewer) the columns 4 + head to the odd dims
+// as well and needs one.  Column j then belongs to head j % (16 / PACK), whose
+// query its lane loads, and unpack_columns adds and moves the parts to where
+// PACK = 1 has them.  (MFMA time per step of four blocks at D = 128: 1280, 768
+// and 512 clocks.)
+inline int pack_for(int32_t group) { return group <= 4 ? 4 : group <= 8 ? 2 : 1; }
+template <int D, int PACK>
+constexpr int acc_tiles() { return PACK == 4 ? D / 32 : D / 16; }
+
+template <int CTRL>
+__device__ __forceinline__ float row_dpp(float x) {  // within 16 lanes
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+      0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, false));
+}
+// Packed accumulators to those of head j in lane (j, g), dims as store_piece
+// takes them; lanes past the heads hold no one's.
+template <int D, int PACK>
+__device__ __forceinline__ void unpack_columns(const f32x4* packed, f32x4* acc) {
+#pragma unroll
+  for (int t = 0; t < acc_tiles<D, PACK>(); ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = packed[t][i];
+      if constexpr (PACK == 1) {
+        acc[t][i] = x;
+      } else {
+        const float y = x + row_dpp<0x128>(x);  // + the lane 8 away (row_ror 8)
+        if constexpr (PACK == 2) {
+          acc[t][i] = y;
+        } else {
+          acc[2 * t][i] = y;
+          acc[2 * t + 1][i] = row_dpp<0x104>(y);  // the lane 4 up (row_shl 4)
+        }
+      }
+    }
+}
+
+// P's operands of one block.  16-bit parts in a register's low half belong to
+// the even dims of V's pairs, in the high half to the odd ones.  low_part, odd:
+// this lane's column (PACK 2, 4).
+template <int DT, int PACK>
 struct Weights4 {
-  u32x4 even_hi, odd_hi, even_lo, odd_lo;
-  __device__ __forceinline__ void set(int c, float p) {
+  static constexpr int N = 4 / PACK;  // operands: (even, odd) of the high part, of the other
+  u32x4 w[N];
+  __device__ __forceinline__ void set(int c, float p, bool low_part, bool odd) {
+    uint32_t hi, lo;  // the parts' bits, in the high half
     if constexpr (DT == AEGKV_DTYPE_BF16) {  // the top 16 bits: p - hi is exact
-      const uint32_t u = __float_as_uint(p);
-      odd_hi[c] = u & 0xffff0000u;
-      even_hi[c] = u >> 16;
-      const uint32_t r = __float_as_uint(p - __uint_as_float(u & 0xffff0000u));
-      odd_lo[c] = r & 0xffff0000u;
-      even_lo[c] = r >> 16;
+      hi = __float_as_uint(p) & 0xffff0000u;
+      lo = __float_as_uint(p - __uint_as_float(hi));
     } else {
-      uint32_t hi, lo;
       Elem<DT>::split(p, hi, lo);
-      even_hi[c] = hi;
-      odd_hi[c] = hi << 16;
-      even_lo[c] = lo;
-      odd_lo[c] = lo << 16;
+      hi <<= 16;
+      lo <<= 16;
+    }
+    if constexpr (PACK == 1) {
+      w[0][c] = hi >> 16;
+      w[1][c] = hi;
+      w[2][c] = lo >> 16;
+      w[3][c] = lo & 0xffff0000u;
+    } else {
+      const uint32_t x = low_part ? lo : hi;
+      if constexpr (PACK == 2) {
+        w[0][c] = x >> 16;
+        w[1][c] = x & 0xffff0000u;
+      } else {
+        w[0][c] = odd ? x & 0xffff0000u : x >> 16;
+      }
     }
   }
 };
@@ -623,7 +674,7 @@ struct Weights4 {
 // blocks whose bit in `skip` is set (unreadable ids, and those past the step).
 template <int D>
 constexpr int step4() { return D >= 256 ? 2 : 4; }
-template <int DT, int D>
+template <int DT, int D, int PACK>
 __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const u32x4* qv,
                                               f32x4* acc, float& m, float& lsum, int tok0,
                                               int limit, uint32_t skip, int g, float scale_log2) {
@@ -678,18 +729,19 @@ __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const
     const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
     lsum *= alpha;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) acc[t] *= alpha;
+    for (int t = 0; t < acc_tiles<D, PACK>(); ++t) acc[t] *= alpha;
     m = mn;
   }
+  const bool low_part = (threadIdx.x & 8) != 0, odd = (threadIdx.x & 4) != 0;
   const float nms = m == -INFINITY ? 0.f : -m;  // -inf only while every token is masked
 #pragma unroll
   for (int u = 0; u < kStep4; ++u) {
-    Weights4<DT> w;
+    Weights4<DT, PACK> w;
     float p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], scale_log2, nms));
-      w.set(i, p[i]);
+      w.set(i, p[i], low_part, odd);
     }
     lsum += (p[0] + p[1]) + (p[2] + p[3]);
     // the conversions read a scale's exponent bits alone: its byte is shifted
@@ -698,10 +750,13 @@ __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const
     const float s[4] = {__uint_as_float(vs << 23), __uint_as_float(vs << 15),
                         __uint_as_float(vs << 7), __uint_as_float(vs >> 1)};
     auto pair = [&](int t, u32x4 x) {  // dims t (even) and t + 1
-      acc[t] = E::mfma(x, w.even_hi, acc[t]);
-      acc[t + 1] = E::mfma(x, w.odd_hi, acc[t + 1]);
-      acc[t] = E::mfma(x, w.even_lo, acc[t]);
-      acc[t + 1] = E::mfma(x, w.odd_lo, acc[t + 1]);
+      if constexpr (PACK == 4) {
+        acc[t / 2] = E::mfma(x, w.w[0], acc[t / 2]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < 4 / PACK; ++n)
+          acc[t + (n & 1)] = E::mfma(x, w.w[n], acc[t + (n & 1)]);
+      }
     };
     const uint32_t* v = r[u].v;
     if constexpr (D == 64) {
@@ -1173,7 +1228,7 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
 // load side keeps a sequence position of its own, and hands a step's to the
 // compute side with its registers.  Past the range a step loads nothing (empty
 // buffer ranges) and is not computed.
-template <int DT, int D, int NSET, bool PLANNED>
+template <int DT, int D, int NSET, int PACK, bool PLANNED>
 __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* s_bcum,
                                               const int32_t* s_len, uint8_t* stage, int4* meta,
                                               int range, int grp, int hl, int b0, int i0, int i1,
@@ -1208,9 +1263,10 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   };
   // lanes past the group load its first head; the softmax's scale is positive,
   // another one's sign goes into the query (0: no query, every score 0)
+  const int jq = j % (16 / PACK);
   auto load_q = [&](int b, u32x4* qv) {
-    const uint16_t* qp =
-        a.q + (int64_t)b * a.q_bstride + (int64_t)(head_ok ? hq : h * a.group) * D;
+    const uint16_t* qp = a.q + (int64_t)b * a.q_bstride +
+                         (int64_t)(h * a.group + (jq < a.group ? jq : 0)) * D;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       qv[ks] = *reinterpret_cast<const u32x4*>(qp + kv4_dim<D>(ks, g));
@@ -1261,9 +1317,10 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   int bc = b0, first = uni(s_bcum[b0]), cend = lend, len = uni(s_len[b0]), ic = i0;
   bool complete = first >= i0 && cend == uni(s_bcum[b0 + 1]);
   u32x4 qv[KS];
-  f32x4 acc[DPL];
+  constexpr int NT = acc_tiles<D, PACK>();
+  f32x4 acc[NT];
 #pragma unroll
-  for (int t = 0; t < DPL; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, lsum = 0.f;
 
   const int rec_bytes = stage_record_bytes<D>();
@@ -1284,20 +1341,23 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
     nstaged = 0;
   };
   auto compute = [&](KV4Regs<D> (&r)[kStep4], const Step& s) {
-    compute_step4<DT, D>(r, qv, acc, m, lsum, (ic - first) * kBlockSize,
-                         min(len, (cend - first) * kBlockSize), s.skip, g, a.abs_scale_log2);
+    compute_step4<DT, D, PACK>(r, qv, acc, m, lsum, (ic - first) * kBlockSize,
+                               min(len, (cend - first) * kBlockSize), s.skip, g,
+                               a.abs_scale_log2);
     ic += s.n;
     if (ic == cend) {  // the piece of sequence bc in this range ends (uniform)
       float lt = lsum + __shfl_xor(lsum, 16);
       lt += __shfl_xor(lt, 32);
       const int pslot = range + grp * a.batch + bc;
+      f32x4 o[DPL];
+      unpack_columns<D, PACK>(acc, o);
       if (stages_pieces<D>() && a.stage_slots > 0) {
         if (nstaged == a.stage_slots) flush();
-        if (head_ok) put_record<D>(my_rec + nstaged * slot_bytes, acc, m, lt);
+        if (head_ok) put_record<D>(my_rec + nstaged * slot_bytes, o, m, lt);
         if (lane == 0) meta[nstaged] = make_int4(bc, complete ? 1 : 0, pslot, 0);
         ++nstaged;
       } else if (head_ok) {
-        store_piece<DT, D>(a, acc, m, lt, bc, hq, complete, pslot, hl0);
+        store_piece<DT, D>(a, o, m, lt, bc, hq, complete, pslot, hl0);
       }
       if (ic < i1) {
         bc = next_seq(bc);
@@ -1307,7 +1367,7 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
         complete = cend == uni(s_bcum[bc + 1]);  // it starts in range
         load_q(bc, qv);
 #pragma unroll
-        for (int t = 0; t < DPL; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY;
         lsum = 0.f;
       }
@@ -1441,7 +1501,8 @@ __device__ __forceinline__ int items_before(const int32_t* cum, const int32_t* b
   return bcum[b] + min(max(p - cum[b] - kSegmentCost, 0), bcum[b + 1] - bcum[b]);
 }
 
-template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, bool Q4>
+// PACK: 0, the 16-bit caches; 1, 2 or 4, the 4-bit cache (pack_for).
+template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, int PACK>
 __global__ __launch_bounds__(64 * kWaves, D >= 256 ? 1 : 2) void
 paged_decode_attention_kernel(AttnArgs a) {
   // cum[batch + 1] (positions), len[batch], bcum[batch + 1] (blocks)
@@ -1492,8 +1553,8 @@ paged_decode_attention_kernel(AttnArgs a) {
       const int b0 = first_pass ? uni(rec[3]) : uni(rec[5]);
       const int i1 = grp == uni(rec[1]) ? uni(rec[4]) : items;
       if (i1 <= i0) continue;
-      if constexpr (Q4)
-        attend_items4<DT, D, NBUF, true>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
+      if constexpr (PACK > 0)
+        attend_items4<DT, D, NBUF, PACK, true>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
                                          i0, i1, first_pass, id_first);
       else
         attend_items<DT, D, NBUF, true, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
@@ -1534,9 +1595,9 @@ paged_decode_attention_kernel(AttnArgs a) {
       if (hl == 0 && lane == 0) a.desc[range] = continued_desc(b0, grp, w0, w1, range);
       first_pass = false;
     }
-    if constexpr (Q4) {
+    if constexpr (PACK > 0) {
       if (i1 > i0)
-        attend_items4<DT, D, NBUF, false>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
+        attend_items4<DT, D, NBUF, PACK, false>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
                                           i0, i1, false, 0);
     } else if (i1 > i0)
       attend_items<DT, D, NBUF, false, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
@@ -2008,18 +2069,26 @@ int launch_combine(const AttnArgs& a, hipStream_t stream) {
   return AEGKV_OK;
 }
 
-template <int DT, int D, bool PLANNED, bool FUSED, bool Q4 = false>
+template <int DT, int D, bool PLANNED, bool FUSED, int PACK = 0>
 void launch_main(const AttnArgs& a, size_t lds, hipStream_t stream) {
-  constexpr int NBUF = Q4 ? kv4_pipeline_depth<D>() : pipeline_depth<D>();
-  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, Q4>),
+  constexpr int NBUF = PACK > 0 ? kv4_pipeline_depth<D>() : pipeline_depth<D>();
+  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, PACK>),
                      dim3(a.n_wg), dim3(64 * kWaves), lds, stream, a);
+}
+template <int DT, int D, bool PLANNED>
+void launch_main4(const AttnArgs& a, size_t lds, hipStream_t stream) {
+  switch (pack_for(a.group)) {
+    case 4: return launch_main<DT, D, PLANNED, false, 4>(a, lds, stream);
+    case 2: return launch_main<DT, D, PLANNED, false, 2>(a, lds, stream);
+    default: return launch_main<DT, D, PLANNED, false, 1>(a, lds, stream);
+  }
 }
 
 template <int DT, int D>
 int launch_attention(const AttnArgs& a, bool kv4, size_t lds, hipStream_t stream) {
   if (kv4) {
-    if (a.plan_wg) launch_main<DT, D, true, false, true>(a, lds, stream);
-    else launch_main<DT, D, false, false, true>(a, lds, stream);
+    if (a.plan_wg) launch_main4<DT, D, true>(a, lds, stream);
+    else launch_main4<DT, D, false>(a, lds, stream);
   } else if (a.plan_wg) {
     if (a.knew) launch_main<DT, D, true, true>(a, lds, stream);
     else launch_main<DT, D, true, false>(a, lds, stream);
