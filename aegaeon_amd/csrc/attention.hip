@@ -1242,81 +1242,66 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   const int hq = h * a.group + j;
   const int hl0 = hl * a.group;
 
-  // ids of items [cbase, cbase + 64) and of the next 64, one lane per item
-  auto item_id = [&](int i, int bh) -> int {
-    i = min(i, i1 - 1);
-    if constexpr (PLANNED) {
-      return a.plan_ids[i];
-    } else {
-      int b = bh;
-      if (s_bcum[b + 1] <= i) b = s_bcum[b + 2] > i ? b + 1 : seq_at(s_bcum, a.batch, i);
-      return a.block_tables[(int64_t)b * a.max_blocks + (i - s_bcum[b])];
-    }
-  };
-  int id_cur = PLANNED && have_first ? id_first : item_id(i0 + lane, b0);
-  int id_nxt = item_id(i0 + 64 + lane, b0);
-  int cbase = i0;
   auto next_seq = [&](int b) -> int {  // the next non-empty sequence (one exists)
     ++b;
     while (uni(s_bcum[b + 1]) == uni(s_bcum[b])) ++b;
     return b;
   };
-  // lanes past the group load its first head; the softmax's scale is positive,
-  // another one's sign goes into the query (0: no query, every score 0)
-  const int jq = j % (16 / PACK);
-  auto load_q = [&](int b, u32x4* qv) {
-    const uint16_t* qp = a.q + (int64_t)b * a.q_bstride +
-                         (int64_t)(h * a.group + (jq < a.group ? jq : 0)) * D;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qv[ks] = *reinterpret_cast<const u32x4*>(qp + kv4_dim<D>(ks, g));
-    if (a.scale_sign <= 0) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qv[ks][i] = a.scale_sign < 0 ? qv[ks][i] ^ 0x80008000u : 0u;
-    }
-  };
 
-  // the load side: sequence bl, whose items in range end at lend; next item il
-  int bl = b0, il = i0, lend = min(uni(s_bcum[b0 + 1]), i1);
+  // The load side: sequence bl, whose blocks start at item lfirst and end in
+  // range at lend; next item il, whose step's block ids are in lanes 0 .. 3 of
+  // `ids`.  A step brings its query along (lanes past the group its first head),
+  // and the ids of the step after it, loaded ahead of its own blocks, so that no
+  // load stands under a condition: the waits of a sequence's start, and of ids,
+  // would be for every load in flight.
+  int bl = b0, il = i0, lfirst = uni(s_bcum[b0]), lend = min(uni(s_bcum[b0 + 1]), i1);
+  auto load_ids = [&]() -> int {
+    const int i = min(il + (lane & 3), lend - 1);  // (past the range: its last item)
+    if constexpr (PLANNED) return a.plan_ids[i];
+    else return a.block_tables[(int64_t)bl * a.max_blocks + (i - lfirst)];
+  };
+  int ids = PLANNED && have_first ? id_first : load_ids();
+  const int jq = j % (16 / PACK);
+  const uint16_t* q_lane =
+      a.q + (int64_t)(h * a.group + (jq < a.group ? jq : 0)) * D + kv4_dim<D>(0, g);
   struct Step {
     int n;          // blocks (0: past the range)
     uint32_t skip;  // blocks not to attend: unreadable, or past n
+    u32x4 q[KS];    // the sequence's query, this lane's head
+    KV4Regs<D> kv[kStep4];
   };
-  KV4Regs<D> buf[NSET][kStep4];
   Step st[NSET];
-  auto load_step = [&](KV4Regs<D> (&r)[kStep4], Step& s) {
+  auto load_step = [&](Step& s) {
     s.n = min(kStep4, lend - il);
     s.skip = 0;
-    if (il - cbase >= 64) {
-      id_cur = id_nxt;
-      cbase += 64;
-      id_nxt = item_id(cbase + 64 + lane, bl);
-    }
+    int id[kStep4];
 #pragma unroll
-    for (int u = 0; u < kStep4; ++u) {
-      // item il + u of the 128 at hand
-      const int k = il + u - cbase;
-      const int id = k < 64 ? __builtin_amdgcn_readlane(id_cur, k & 63)
-                            : __builtin_amdgcn_readlane(id_nxt, k & 63);
-      const bool ok = u < s.n && id >= 0 && id < a.n_blocks;
-      if (!ok) s.skip |= 1u << u;
-      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id : 0) * a.blk_stride) +
-                         (int64_t)h * 17 * D;
-      load_block4<D>(r[u], byte_range(p, ok ? 17 * D : 0u), lane);
-    }
+    for (int u = 0; u < kStep4; ++u) id[u] = __builtin_amdgcn_readlane(ids, u);
+    const uint16_t* qp = q_lane + (int64_t)bl * a.q_bstride;
     il += s.n;
     if (il == lend && il < i1) {
       bl = next_seq(bl);
+      lfirst = uni(s_bcum[bl]);
       lend = min(uni(s_bcum[bl + 1]), i1);
+    }
+    ids = load_ids();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      s.q[ks] = *reinterpret_cast<const u32x4*>(qp + (kv4_dim<D>(ks, 0) - kv4_dim<D>(0, 0)));
+#pragma unroll
+    for (int u = 0; u < kStep4; ++u) {
+      const bool ok = u < s.n && id[u] >= 0 && id[u] < a.n_blocks;
+      if (!ok) s.skip |= 1u << u;
+      const uint8_t* p =
+          reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id[u] : 0) * a.blk_stride) +
+          (int64_t)h * 17 * D;
+      load_block4<D>(s.kv[u], byte_range(p, ok ? 17 * D : 0u), lane);
     }
   };
 
   // the compute side
   int bc = b0, first = uni(s_bcum[b0]), cend = lend, len = uni(s_len[b0]), ic = i0;
   bool complete = first >= i0 && cend == uni(s_bcum[b0 + 1]);
-  u32x4 qv[KS];
   constexpr int NT = acc_tiles<D, PACK>();
   f32x4 acc[NT];
 #pragma unroll
@@ -1340,8 +1325,14 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
     }
     nstaged = 0;
   };
-  auto compute = [&](KV4Regs<D> (&r)[kStep4], const Step& s) {
-    compute_step4<DT, D, PACK>(r, qv, acc, m, lsum, (ic - first) * kBlockSize,
+  auto compute = [&](Step& s) {
+    if (a.scale_sign <= 0) {  // the softmax's is positive: its sign to the query (0: none)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.q[ks][i] = a.scale_sign < 0 ? s.q[ks][i] ^ 0x80008000u : 0u;
+    }
+    compute_step4<DT, D, PACK>(s.kv, s.q, acc, m, lsum, (ic - first) * kBlockSize,
                                min(len, (cend - first) * kBlockSize), s.skip, g,
                                a.abs_scale_log2);
     ic += s.n;
@@ -1365,7 +1356,6 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
         cend = min(uni(s_bcum[bc + 1]), i1);
         len = uni(s_len[bc]);
         complete = cend == uni(s_bcum[bc + 1]);  // it starts in range
-        load_q(bc, qv);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY;
@@ -1375,23 +1365,20 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   };
 
   unrolled_steps<NSET>([&](auto kc) {
-    load_step(buf[decltype(kc)::value], st[decltype(kc)::value]);
+    load_step(st[decltype(kc)::value]);
     return false;
   });
-  load_q(bc, qv);  // behind the first steps' loads
-  bool more = true;
-  while (more) {
+  // One exit, at the loop's end: an exit after each step had the compiler count
+  // a path on which the newest loads are those of the step computed next, so
+  // that it waited for every load in flight.
+  do {
     unrolled_steps<NSET>([&](auto kc) {
       constexpr int k = decltype(kc)::value;
-      compute(buf[k], st[k]);
-      if (ic == i1) {  // every item is computed (uniform)
-        more = false;
-        return true;
-      }
-      load_step(buf[k], st[k]);
+      if (st[k].n > 0) compute(st[k]);  // uniform
+      load_step(st[k]);
       return false;
     });
-  }
+  } while (ic < i1);
   flush();
 }
 
