@@ -38,7 +38,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr int kUnitRows = 32;   // rows of a wave
 constexpr int kTileBlocks = kPfKTile / kKv4Tokens;
 constexpr int kShortWaves4 = 4;
-constexpr int kMinSplitTiles = 4;  // least key tiles of a piece
 
 struct VarlenArgs {
   const uint8_t* q;
@@ -57,6 +56,7 @@ struct VarlenArgs {
   float scale_log2;          // |softmax scale| * log2(e), > 0 (1 for 0)
   int32_t scale_sign;        // of the scale: 1, -1 or 0
   int64_t target;            // pieces wanted (0: no sequence is cut)
+  int32_t least;             // least key tiles of a piece
   int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
   float* part_o;             // [n_pieces][32 W][D]
   float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
@@ -86,16 +86,16 @@ __device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
   return s;
 }
 
-// One piece of work: sequence, kv head, row tile, range of key tiles and slot
-// of the partials (-1: the whole range, straight to the output).
+// One piece of work: the sequence, its kv head, row tile and range of key tiles.
 struct Piece {
+  SeqWork s;
   int b, head, tile, split, splits, span, first;  // first: the sequence's first piece
 };
 
 struct LocateLds {
   int64_t cost[16];
   int sum[16], pieces[16];
-  int found[5];
+  int found[11];
 };
 __device__ __forceinline__ int ranges_of(int n_kt, int span) {
   return max(1, (n_kt + span - 1) / span);
@@ -107,11 +107,14 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   constexpr int NW = NT / 64;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.batch + NT - 1) / NT, b0 = min(t * per, a.batch), b1 = min(b0 + per, a.batch);
+  // the thread's first sequence, its only one in batches of up to NT
+  const SeqWork mine = seq_work<W>(a, min(b0, a.batch - 1));
+  auto work = [&](int b) { return b == b0 ? mine : seq_work<W>(a, b); };
   int span = INT32_MAX;
   if (a.target > 0) {  // uniform
     int64_t cost = 0;
     for (int b = b0; b < b1; ++b) {
-      const SeqWork s = seq_work<W>(a, b);
+      const SeqWork s = work(b);
       cost += (int64_t)s.tiles * s.n_kt;
     }
 #pragma unroll
@@ -123,15 +126,16 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
     for (int w = 0; w < NW; ++w) cost += x.cost[w];
     cost *= a.n_kv_heads;
     span = (int)min((cost + a.target - 1) / a.target, (int64_t)INT32_MAX);
-    span = max(span, kMinSplitTiles);
+    span = max(span, a.least);
   }
   int count = 0, before = 0;  // this thread's units, and its pieces
-  for (int b = b0; b < b1; ++b) {
-    const SeqWork s = seq_work<W>(a, b);
+  auto add = [&](const SeqWork& s, int& units, int& pieces) {
     const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
-    before += n * r;
-    count += MERGE ? (r > 1 ? n * W : 0) : n * r;
-  }
+    pieces += n * r;
+    units += MERGE ? (r > 1 ? n * W : 0) : n * r;
+    return r;
+  };
+  for (int b = b0; b < b1; ++b) add(work(b), count, before);
   int incl = count, pincl = before;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -154,35 +158,41 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   }
   if (index >= excl && index < excl + count) {  // one thread
     for (int b = b0; b < b1; ++b) {
-      const SeqWork s = seq_work<W>(a, b);
-      const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
-      const int c = MERGE ? (r > 1 ? n * W : 0) : n * r;
-      if (index < excl + c) {
-        x.found[0] = b;
-        x.found[1] = index - excl;
-        x.found[2] = r;
-        x.found[3] = (s.n_kt + r - 1) / r;
-        x.found[4] = pexcl;
+      const SeqWork s = work(b);
+      int units = 0, pieces = 0;
+      const int r = add(s, units, pieces);
+      if (index < excl + units) {
+        const int f[11] = {b,   index - excl, r,      (s.n_kt + r - 1) / r, pexcl, s.t0,
+                           s.m, s.off,        s.len, s.rows,               s.tiles};
+#pragma unroll
+        for (int i = 0; i < 11; ++i) x.found[i] = f[i];
         break;
       }
-      excl += c;
-      pexcl += n * r;
+      excl += units;
+      pexcl += pieces;
     }
   }
   __syncthreads();
-  p.b = __builtin_amdgcn_readfirstlane(x.found[0]);
+  int f[11];
+#pragma unroll
+  for (int i = 0; i < 11; ++i) f[i] = __builtin_amdgcn_readfirstlane(x.found[i]);
+  p.b = f[0];
   if (p.b < 0) return false;
-  const SeqWork s = seq_work<W>(a, p.b);
-  const int k = __builtin_amdgcn_readfirstlane(x.found[1]);
-  p.splits = __builtin_amdgcn_readfirstlane(x.found[2]);
-  p.span = __builtin_amdgcn_readfirstlane(x.found[3]);
-  p.first = __builtin_amdgcn_readfirstlane(x.found[4]);
+  p.splits = f[2];
+  p.span = f[3];
+  p.first = f[4];
+  p.s.t0 = f[5];
+  p.s.m = f[6];
+  p.s.off = f[7];
+  p.s.len = f[8];
+  p.s.rows = f[9];
+  p.s.tiles = f[10];
   // kv heads slowest, then row tiles from the last (the most keys) to the first
   const int per_tile = MERGE ? W : p.splits;
-  const int q = k / per_tile;
-  p.split = k - q * per_tile;  // MERGE: the unit
-  p.head = q / s.tiles;
-  p.tile = s.tiles - 1 - (q - p.head * s.tiles);
+  const int q = f[1] / per_tile;
+  p.split = f[1] - q * per_tile;  // MERGE: the unit
+  p.head = q / p.s.tiles;
+  p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
   return true;
 }
 
@@ -193,32 +203,38 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
     asm volatile("" ::: "memory");                     \
   } while (0)
 
-// The codes of one block for one lane, as in the decode attention.
+// The K or V codes of one block for one lane, as in the decode attention:
+// words and scale byte(s).
 template <int D>
 struct CodeRegs {
-  uint32_t k[D / 32], v[D / 32], ks, vs;
+  uint32_t w[D / 32], s;
 };
 template <int D>
-__device__ __forceinline__ void load_codes(CodeRegs<D>& c, __amdgpu_buffer_rsrc_t r, int lane) {
-  constexpr int REC = kv4_record_bytes(D), CODES = kv4_code_bytes(D);
-  const int j = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void load_words4(CodeRegs<D>& c, __amdgpu_buffer_rsrc_t r, int at,
+                                            int lane) {
   if constexpr (D == 64) {
-    const u32x2 k = __builtin_amdgcn_raw_buffer_load_b64(r, 8 * lane, 0, 0);
-    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, REC + 8 * lane, 0, 0);
-    c.k[0] = k.x; c.k[1] = k.y;
-    c.v[0] = v.x; c.v[1] = v.y;
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, at + 8 * lane, 0, 0);
+    c.w[0] = x.x; c.w[1] = x.y;
   } else {
-    const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(r, 16 * lane, 0, 0);
-    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, REC + 16 * lane, 0, 0);
+    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * lane, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c.k[i] = k[i];
-      c.v[i] = v[i];
-    }
+    for (int i = 0; i < 4; ++i) c.w[i] = x[i];
   }
-  c.ks = __builtin_amdgcn_raw_buffer_load_b8(r, CODES + (D == 64 ? g >> 1 : g) * kKv4Tokens + j, 0, 0);
-  c.vs = __builtin_amdgcn_raw_buffer_load_b32(
-      r, REC + CODES + (j * (D / 16) / kKv4Group) * kKv4Tokens + 4 * g, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ void load_k(CodeRegs<D>& c, __amdgpu_buffer_rsrc_t r, int lane) {
+  const int j = lane & 15, g = lane >> 4;
+  load_words4<D>(c, r, 0, lane);
+  c.s = __builtin_amdgcn_raw_buffer_load_b8(
+      r, kv4_code_bytes(D) + (D == 64 ? g >> 1 : g) * kKv4Tokens + j, 0, 0);
+}
+template <int D>
+__device__ __forceinline__ void load_v(CodeRegs<D>& c, __amdgpu_buffer_rsrc_t r, int lane) {
+  constexpr int REC = kv4_record_bytes(D);
+  const int j = lane & 15, g = lane >> 4;
+  load_words4<D>(c, r, REC, lane);
+  c.s = __builtin_amdgcn_raw_buffer_load_b32(
+      r, REC + kv4_code_bytes(D) + (j * (D / 16) / kKv4Group) * kKv4Tokens + 4 * g, 0, 0);
 }
 
 // Rows of 2 D bytes in LDS, their 16-byte chunks permuted by the row so that the
@@ -237,68 +253,48 @@ __device__ __forceinline__ void put_k(uint8_t* lds, const CodeRegs<D>& c, int u,
   using C = Kv4Elem<DT>;
   constexpr int NW = D / 32;
   const int j = lane & 15, g = lane >> 4, row = kKv4Tokens * u + j;
-  const float s = kv4_scale(c.ks);
+  const float s = kv4_scale(c.s);
 #pragma unroll
   for (int i = 0; i < NW; ++i)
     *reinterpret_cast<u32x4*>(lds + row * 2 * D + k_chunk<D>(row, NW * g + i) * 16) =
-        u32x4{C::template dq<0>(c.k[i], s), C::template dq<1>(c.k[i], s),
-              C::template dq<2>(c.k[i], s), C::template dq<3>(c.k[i], s)};
+        u32x4{C::template dq<0>(c.w[i], s), C::template dq<1>(c.w[i], s),
+              C::template dq<2>(c.w[i], s), C::template dq<3>(c.w[i], s)};
 }
 // V's tokens at or past `left` (of the block's 16) and its NaN groups are stored
-// as zeros, as a weight of zero does not undo a NaN; the groups are noted in
-// nan[D/32] (bit: token), which is written when the return value is true.
+// as zeros, as a weight of zero does not undo a NaN.  True when there was such a
+// group (uniform): its rows are found at the end (RowUnit::find_nan).
 template <int DT, int D>
-__device__ __forceinline__ bool put_v(uint8_t* lds, uint16_t* nan, CodeRegs<D>& c, int u, int left,
-                                      int lane) {
+__device__ __forceinline__ bool put_v(uint8_t* lds, CodeRegs<D>& c, int u, int left, int lane) {
   using C = Kv4Elem<DT>;
   const int j = lane & 15, g = lane >> 4;
   uint32_t e[4];
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    e[i] = (c.vs >> (8 * i)) & 0xffu;
-    if (4 * g + i >= left) {  // scale byte 0, and code bits 0 below
-      e[i] = 0;
-      if constexpr (D == 64) c.v[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
-      else c.v[i] = 0;
-    }
-    bad |= e[i] == kKv4ScaleNan;
-  }
-  const bool any = __builtin_amdgcn_ballot_w64(bad) != 0;
-  if (any) {  // rare; uniform
-    uint64_t at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      at[i] = __builtin_amdgcn_ballot_w64(e[i] == kKv4ScaleNan);
-      if (e[i] == kKv4ScaleNan) e[i] = 0;  // finite whatever its codes
-    }
-    if (lane < D / 32) {  // group `lane`: lanes j = lane * 512 / D of each quad
-      uint32_t m = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          m |= (uint32_t)(at[i] >> (16 * q + lane * (512 / D)) & 1) << (4 * q + i);
-      nan[lane] = (uint16_t)m;
-    }
+    e[i] = (c.s >> (8 * i)) & 0xffu;
+    const bool past = 4 * g + i >= left, nan = e[i] == kKv4ScaleNan;
+    bad |= nan && !past;
+    e[i] = past || nan ? 0u : e[i];  // scale byte 0: finite whatever the codes
+    if constexpr (D == 64) c.w[i >> 1] = past ? c.w[i >> 1] & (i & 1 ? 0x0000ffffu : 0xffff0000u) : c.w[i >> 1];
+    else c.w[i] = past ? 0u : c.w[i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = kKv4Tokens * u + 4 * g + i;
     const float s = kv4_scale(e[i]);
     if constexpr (D == 64) {
-      const uint32_t w = c.v[i >> 1];
+      const uint32_t w = c.w[i >> 1];
       const u32x2 x = i & 1 ? u32x2{C::template dq<2>(w, s), C::template dq<3>(w, s)}
                             : u32x2{C::template dq<0>(w, s), C::template dq<1>(w, s)};
       *reinterpret_cast<u32x2*>(lds + row * 2 * D + v_chunk<D>(row, j >> 1) * 16 + 8 * (j & 1)) = x;
     } else {
-      const uint32_t w = c.v[i];
+      const uint32_t w = c.w[i];
       *reinterpret_cast<u32x4*>(lds + row * 2 * D + v_chunk<D>(row, j) * 16) =
           u32x4{C::template dq<0>(w, s), C::template dq<1>(w, s), C::template dq<2>(w, s),
                 C::template dq<3>(w, s)};
     }
   }
-  return any;
+  return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
 
 // A wave's unit of 32 rows.
@@ -314,6 +310,7 @@ struct RowUnit : WaveSoftmax<DT, D> {
   int r0, rows;     // first row; the sequence's rows
   int limit;        // last key of this lane's row (-1: none)
   int lim_lo, lim_hi;  // of the unit's first and last row
+  uint32_t spoiled;    // bit: dims 32 db .. of this lane's row are NaN
 
   __device__ __forceinline__ void init(const VarlenArgs& a, const SeqWork& s, int head, int unit) {
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
@@ -337,6 +334,7 @@ struct RowUnit : WaveSoftmax<DT, D> {
       for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
     m = -INFINITY;
     lsum = 0.f;
+    spoiled = 0;
   }
   // the softmax's scale is positive: another one's sign goes into the queries
   // (0: no query, every score 0)
@@ -349,6 +347,9 @@ struct RowUnit : WaveSoftmax<DT, D> {
   }
   __device__ __forceinline__ bool sees(int kt) const { return kt * kPfKTile <= lim_hi; }  // uniform
 
+  // ORDERED: LDS reads stay two MFMAs ahead of their use (pv: four), as the long
+  // prompts' kernel orders them
+  template <bool ORDERED>
   __device__ __forceinline__ void qk(const uint8_t* lds, f32x16 (&s)[2]) const {
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const uint8_t* kp = lds + col * 2 * D;
@@ -363,26 +364,32 @@ struct RowUnit : WaveSoftmax<DT, D> {
       for (int sb = 0; sb < 2; ++sb)
         s[sb] = PfOps<DT>::mfma(
             *reinterpret_cast<const u32x4*>(kp + (kx ^ (32 * ks)) + 32 * sb * 2 * D), qv[ks], s[sb]);
+    if (ORDERED) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+#pragma unroll
+      for (int i = 0; i < 2 * KS - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // the next read
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    }
   }
   // -inf for keys past a row's last one and for unreadable blocks (bit u)
   __device__ __forceinline__ void mask(f32x16 (&s)[2], int k0, uint32_t unreadable) const {
-    const int hh = (threadIdx.x & 63) >> 5;
-    if (k0 + kPfKTile - 1 > lim_lo) {
-      const int last = limit - k0 - 4 * hh;
+    if (k0 + kPfKTile - 1 > lim_lo || unreadable) {
+      const int hh = (threadIdx.x & 63) >> 5, last = limit - k0 - 4 * hh;
 #pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
+      for (int u = 0; u < kTileBlocks; ++u) {
+        const int l = unreadable >> u & 1 ? -1 : last;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          s[sb][e] = last >= 32 * sb + 8 * (e >> 2) + (e & 3) ? s[sb][e] : -INFINITY;
-    }
-    if (unreadable) {
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          s[sb][e] = unreadable >> (2 * sb + (e >> 3)) & 1 ? -INFINITY : s[sb][e];
+        for (int e = 0; e < 8; ++e) {
+          const int i = 8 * (u & 1) + e;
+          s[u >> 1][i] = l >= 16 * u + 8 * (e >> 2) + (e & 3) ? s[u >> 1][i] : -INFINITY;
+        }
+      }
     }
   }
+  template <bool ORDERED>
   __device__ __forceinline__ void pv(const uint8_t* lds, const u32x4 (&pb)[4]) {
     constexpr int RB = 2 * D;
     const int lane = threadIdx.x & 63, G = lane >> 4, x = lane & 15;
@@ -400,19 +407,41 @@ struct RowUnit : WaveSoftmax<DT, D> {
             u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(y + 8 * RB)));
         o[db] = PfOps<DT>::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[kk], o[db]);
       }
-  }
-  // NaN to the dims of V's NaN groups (nan[block][group], bit: token) for the
-  // rows that see one of their tokens
-  __device__ __forceinline__ void spoil(const uint16_t (*nan)[D / 32], uint32_t blocks, int k0) {
+    if (ORDERED) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int db = 0; db < DB; ++db) {
-      int first = kPfKTile;  // the tile's first such key
-      for (int u = kTileBlocks - 1; u >= 0; --u)
-        if (blocks >> u & 1 && nan[u][db]) first = kKv4Tokens * u + __builtin_ctz(nan[u][db]);
-      const bool seen = first < kPfKTile && k0 + first <= limit;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[db][e] = seen ? __builtin_nanf("") : o[db][e];
+      for (int i = 0; i < 4 * DB - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
     }
+  }
+  // Key tiles [kt0, kt1) hold V groups of NaN (rare): the rows that see one's
+  // token get NaN in its dims when they are stored.  Visible keys are a prefix, so
+  // each group's first such key decides.
+  __device__ void find_nan(const VarlenArgs& a, const int32_t* table, int64_t head_off, int len,
+                           int kt0, int kt1) {
+    const int lane = threadIdx.x & 63;
+    const int n_blk = min(kt1 * kTileBlocks, (len + kKv4Tokens - 1) / kKv4Tokens);
+    uint32_t found = 0;  // groups whose first key is known
+    for (int blk = kt0 * kTileBlocks; blk < n_blk; ++blk) {
+      const int id = __builtin_amdgcn_readfirstlane(table[blk]);
+      if (id < 0 || id >= a.n_blocks) continue;
+      uint32_t e = 0;  // lane: group lane / 16, token lane % 16
+      if (lane < D / 2 && blk * kKv4Tokens + (lane & 15) < len)
+        e = a.cache[(int64_t)id * a.blk_b + head_off + kv4_record_bytes(D) + kv4_code_bytes(D) + lane];
+      const uint64_t at = __builtin_amdgcn_ballot_w64(e == kKv4ScaleNan);
+      for (int db = 0; db < DB; ++db) {
+        const uint32_t t = (uint32_t)(at >> (16 * db)) & 0xffffu;
+        if (!t || (found >> db & 1)) continue;
+        found |= 1u << db;
+        if (blk * kKv4Tokens + __builtin_ctz(t) <= limit) spoiled |= 1u << db;
+      }
+    }
+  }
+  __device__ __forceinline__ float finite_or_nan(int db) const {
+    return spoiled >> db & 1 ? __builtin_nanf("") : 1.f;
   }
   __device__ __forceinline__ float total() const { return lsum + __shfl_xor(lsum, 32); }
 
@@ -423,13 +452,13 @@ struct RowUnit : WaveSoftmax<DT, D> {
     constexpr int RB = D * 2, CPR = D / 8, RPI = 64 / CPR;
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const float lt = total();
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
     uint8_t* xw = x + col * RB + 8 * hh;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x16& v = o[db];
+        const float inv = (lt == 0.f ? 0.f : 1.f / lt) * finite_or_nan(db);
         *reinterpret_cast<u32x2*>(xw + ((4 * db + g) ^ (col % CPR)) * 16) =
             u32x2{PfOps<DT>::pack(v[4 * g] * inv, v[4 * g + 1] * inv),
                   PfOps<DT>::pack(v[4 * g + 2] * inv, v[4 * g + 3] * inv)};
@@ -457,7 +486,8 @@ struct RowUnit : WaveSoftmax<DT, D> {
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4*>(po + 32 * db + 8 * g) =
-            f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+            f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]} *
+            finite_or_nan(db);
     if (hh == 0) a.part_ml[slot_row + col] = make_float2(m, lt);
   }
 };
@@ -469,12 +499,11 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_varlen_kernel(VarlenArgs a) {
   constexpr int T_BYTES = kPfKTile * D * 2;
   static_assert(W * kUnitRows * D * 2 <= 2 * T_BYTES, "the outputs fit the tiles");
   __shared__ __align__(16) uint8_t lds[2 * T_BYTES];  // K, then V
-  __shared__ uint16_t s_nan[kTileBlocks][D / 32];
-  __shared__ uint32_t s_nan_any[kTileBlocks];
+  __shared__ uint32_t s_nan[W];
   __shared__ LocateLds s_loc;
   Piece p;
   if (!locate<W, 64 * W, false>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
-  const SeqWork s = seq_work<W>(a, p.b);
+  const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_blk = (s.len + kKv4Tokens - 1) / kKv4Tokens;
   // the key tiles of this piece that the tile's last row sees
@@ -493,7 +522,7 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_varlen_kernel(VarlenArgs a) {
   const int64_t head_off = (int64_t)p.head * 17 * D;
   int base = kt0 * kTileBlocks, ids = 0, ids_next = 0;
   uint32_t unreadable = 0, unreadable_next = 0;
-  CodeRegs<D> c;
+  CodeRegs<D> ck, cv;
   auto load = [&](int kt) {
     const int blk = kt * kTileBlocks;
     if (blk - base >= 64) {
@@ -514,42 +543,184 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_varlen_kernel(VarlenArgs a) {
         my_id = id;
       }
     }
-    load_codes<D>(c, byte_range(a.cache + (int64_t)(mine ? my_id : 0) * a.blk_b + head_off,
-                                mine ? 17 * D : 0u), lane);
+    const auto r = byte_range(a.cache + (int64_t)(mine ? my_id : 0) * a.blk_b + head_off,
+                              mine ? 17 * D : 0u);
+    load_k<D>(ck, r, lane);
+    load_v<D>(cv, r, lane);
   };
   if (kt0 < kt1) {
     ids = ids_from(base);
     ids_next = ids_from(base + 64);
     load(kt0);
   }
+  bool nan = false;
   for (int kt = kt0; kt < kt1; ++kt) {
     if (kt > kt0) KV4_BARRIER();  // every wave's reads of the tile before
-    put_k<DT, D>(lds, c, w, lane);
+    put_k<DT, D>(lds, ck, w, lane);
     const int left = s.len - (kt * kTileBlocks + w) * kKv4Tokens;
-    const bool any = put_v<DT, D>(lds + T_BYTES, s_nan[w], c, w, left, lane);
-    if (lane == 0) s_nan_any[w] = any;
+    nan |= put_v<DT, D>(lds + T_BYTES, cv, w, left, lane);
     unreadable = unreadable_next;
     if (kt + 1 < kt1) load(kt + 1);
     KV4_BARRIER();
     if (unit.sees(kt)) {
       f32x16 sc[2];
       u32x4 pb[4];
-      unit.qk(lds, sc);
+      unit.template qk<false>(lds, sc);
       unit.mask(sc, kt * kPfKTile, unreadable);
       unit.softmax(sc, pb, a.scale_log2, kt == kt0);
-      unit.pv(lds + T_BYTES, pb);
-      uint32_t nan = 0;
-#pragma unroll
-      for (int u = 0; u < kTileBlocks; ++u) nan |= s_nan_any[u] << u;
-      if (__builtin_amdgcn_readfirstlane(nan)) unit.spoil(s_nan, nan, kt * kPfKTile);
+      __builtin_amdgcn_sched_barrier(0);  // V's reads stay behind the softmax: registers
+      unit.template pv<false>(lds + T_BYTES, pb);
     }
   }
+  if (lane == 0) s_nan[w] = nan;
+  KV4_BARRIER();  // and the tiles: every wave is past its last read of them
+  nan = false;
+#pragma unroll
+  for (int i = 0; i < W; ++i) nan |= s_nan[i] != 0;
+  if (__builtin_amdgcn_readfirstlane(nan)) unit.find_nan(a, table, head_off, s.len, kt0, kt1);
   if (p.splits > 1) {
     unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
     return;
   }
-  KV4_BARRIER();  // the tiles: every wave is past its last read of them
   unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
+}
+
+// Long rows: eight units in ping-pong, as the long prompts' kernel runs them.
+// Waves w and w + 4 share a SIMD and run opposite phases between workgroup
+// barriers: in a matrix phase a wave takes S_j and O += V_{j-1}^T.P_{j-1}, in the
+// next its softmax, waves 4-7 one phase later than waves 0-3.  The conversions
+// go with the softmax: in slot 2j + 1 waves 0-3 convert a block of K_{j+1} each,
+// in slot 2j waves 4-7 one of V_j.  K_{j+1}'s stage was last read (as K_{j-1})
+// in slot 2j - 1 and is read from slot 2j + 2 on, V_j's as well.
+constexpr int kLongWaves4 = 8;
+template <int DT, int D>
+__global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(VarlenArgs a) {
+  constexpr int W = kLongWaves4;
+  constexpr int T_BYTES = kPfKTile * D * 2;
+  static_assert(W / 2 * kUnitRows * D * 2 <= 2 * T_BYTES, "a half's outputs fit its stages");
+  __shared__ __align__(16) uint8_t lds[4 * T_BYTES];  // two K stages, two V stages
+  __shared__ uint32_t s_nan[W / 2];
+  __shared__ LocateLds s_loc;
+  Piece p;
+  if (!locate<W, 64 * W, false>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  const SeqWork& s = p.s;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = w >> 2, u = w & 3;  // and the block of each tile that the wave converts
+  const int n_blk = (s.len + kKv4Tokens - 1) / kKv4Tokens;
+  const int last_q = a.by_group.div(min(s.rows, (p.tile + 1) * W * kUnitRows) - 1);
+  const int keys = a.causal ? min(s.off + last_q + 1, s.len) : s.len;
+  const int kt0 = p.split * p.span;
+  const int n_kt = max(min(p.span, (max(keys, 0) + kPfKTile - 1) / kPfKTile - kt0), 0);
+
+  RowUnit<DT, D> unit;
+  unit.init(a, s, p.head, p.tile * W + w);
+  unit.sign_queries(a.scale_sign);
+  // tiles j of the piece that the wave's rows see
+  const int jw = min(n_kt, unit.lim_hi < 0 ? 0 : max(unit.lim_hi / kPfKTile + 1 - kt0, 0));
+
+  const int32_t* table = a.tables + (int64_t)p.b * a.max_blocks;
+  auto ids_from = [&](int blk) -> int { return table[min(blk + lane, n_blk - 1)]; };
+  const int64_t head_off = (int64_t)p.head * 17 * D;
+  // ids of 16 key tiles from tile `base` of the piece, and of the next 16
+  int base = 0, ids = 0, ids_next = 0;
+  auto id_of = [&](int j, int x) -> int {  // -1: unreadable
+    const int id = __builtin_amdgcn_readlane(ids, (j - base) * kTileBlocks + x);
+    return id >= 0 && id < a.n_blocks ? id : -1;
+  };
+  // the blocks of tile j that are unreadable (a tile at or before the one loaded)
+  auto bad_of = [&](int j) -> uint32_t {
+    uint32_t m = 0;
+    for (int x = 0; x < kTileBlocks; ++x)
+      if ((kt0 + j) * kTileBlocks + x < n_blk && id_of(j, x) < 0) m |= 1u << x;
+    return m;
+  };
+  CodeRegs<D> c;
+  uint32_t bad_now = 0, bad_next = 0;  // of the tile computed, of the one loaded
+  // this wave's codes of tile j (none past the piece): K of block u, or V
+  auto load = [&](int j) {
+    if (j - base == 16) {
+      ids = ids_next;
+      base += 16;
+      ids_next = ids_from((kt0 + base + 16) * kTileBlocks);
+    }
+    const int id = j < n_kt && (kt0 + j) * kTileBlocks + u < n_blk ? id_of(j, u) : -1;
+    bad_next = j < n_kt ? bad_of(j) : 0;
+    const auto r = byte_range(a.cache + (int64_t)max(id, 0) * a.blk_b + head_off,
+                              id >= 0 ? 17 * D : 0u);
+    if (half == 0) load_k<D>(c, r, lane);
+    else load_v<D>(c, r, lane);
+  };
+  bool nan = false;
+  auto put = [&](int j) {  // and the loads of the tile after it
+    if (half == 0) {
+      put_k<DT, D>(lds + (j & 1) * T_BYTES, c, u, lane);
+    } else {
+      const int left = s.len - ((kt0 + j) * kTileBlocks + u) * kKv4Tokens;
+      nan |= put_v<DT, D>(lds + (2 + (j & 1)) * T_BYTES, c, u, left, lane);
+    }
+    load(j + 1);
+  };
+  auto qk = [&](int j, f32x16 (&sc)[2]) { unit.template qk<true>(lds + (j & 1) * T_BYTES, sc); };
+  auto softmax = [&](int j, f32x16 (&sc)[2], u32x4 (&pb)[4], uint32_t bad) {
+    unit.mask(sc, (kt0 + j) * kPfKTile, bad);
+    unit.softmax(sc, pb, a.scale_log2, j == 0);
+  };
+  auto pv = [&](int j, const u32x4 (&pb)[4]) {
+    unit.template pv<true>(lds + (2 + (j & 1)) * T_BYTES, pb);
+  };
+
+  u32x4 pb[4];
+  if (n_kt > 0) {  // uniform: every wave passes 2 n_kt + 3 barriers
+    ids = ids_from(kt0 * kTileBlocks);
+    ids_next = ids_from((kt0 + 16) * kTileBlocks);
+    load(0);
+    if (half == 0) {
+      bad_now = bad_next;
+      put(0);  // K_0; loads K_1
+      KV4_BARRIER();
+      for (int j = 0; j < n_kt; ++j) {
+        f32x16 sc[2];  // slot 2j
+        if (j < jw) qk(j, sc);
+        if (j >= 1 && j - 1 < jw) pv(j - 1, pb);
+        KV4_BARRIER();
+        const uint32_t bad = bad_now;  // slot 2j + 1
+        bad_now = bad_next;
+        if (j + 1 < n_kt) put(j + 1);
+        if (j < jw) softmax(j, sc, pb, bad);
+        KV4_BARRIER();
+      }
+      if (n_kt - 1 < jw) pv(n_kt - 1, pb);  // slot 2 n_kt
+      KV4_BARRIER();
+      KV4_BARRIER();
+    } else {
+      KV4_BARRIER();
+      bad_now = bad_next;
+      put(0);  // slot 0: V_0; loads V_1
+      KV4_BARRIER();
+      for (int j = 0; j < n_kt; ++j) {
+        f32x16 sc[2];  // slot 2j + 1
+        if (j < jw) qk(j, sc);
+        if (j >= 1 && j - 1 < jw) pv(j - 1, pb);
+        KV4_BARRIER();
+        const uint32_t bad = bad_now;  // slot 2j + 2
+        bad_now = bad_next;
+        if (j + 1 < n_kt) put(j + 1);
+        if (j < jw) softmax(j, sc, pb, bad);
+        KV4_BARRIER();
+      }
+      if (n_kt - 1 < jw) pv(n_kt - 1, pb);  // slot 2 n_kt + 1
+      KV4_BARRIER();
+    }
+  }
+  if (half == 1 && lane == 0) s_nan[u] = nan;
+  KV4_BARRIER();  // and the stages: every wave is past its last read of them
+  nan = false;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) nan |= s_nan[i] != 0;
+  if (__builtin_amdgcn_readfirstlane(nan))
+    unit.find_nan(a, table, head_off, s.len, kt0, kt0 + n_kt);
+  if (p.splits > 1) unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
+  else unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
 }
 
 // Merges the pieces of one 32-row unit of a cut tile:
@@ -561,7 +732,7 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
   __shared__ LocateLds s_loc;
   Piece p;
   if (!locate<W, kMerge4Threads, true>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
-  const SeqWork s = seq_work<W>(a, p.b);
+  const SeqWork& s = p.s;
   const int row = (int)threadIdx.x >> 3, part = threadIdx.x & 7;
   const int r = (p.tile * W + p.split) * kUnitRows + row;  // p.split: the unit
   if (r >= s.rows) return;
@@ -600,34 +771,48 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
               PfOps<DT>::pack(acc[k][2] * inv, acc[k][3] * inv)};
 }
 
-// The launch of a call: how many pieces at most, and whether sequences are cut.
+// The launch of a call: which kernel, how many pieces at most, and whether
+// sequences are cut.
 struct VarlenShape {
+  int waves;        // of a workgroup: units of a row tile
   int64_t pieces;   // bound of the pieces (the main grid)
   int64_t target;   // pieces wanted (0: uncut)
+  int32_t least;    // key tiles of a piece at least
   int64_t merge;    // bound of the merge's units
   int64_t o_bytes, ml_bytes;
 };
-constexpr int kWorkgroupsPerCu4 = 2;
+#ifndef LONG_ROWS
+#define LONG_ROWS 512
+#define TGT_LONG 1
+#define TGT_SHORT 1
+#define LEAST_LONG 16
+#define LEAST_SHORT 4
+#endif
+constexpr int kLongRows = LONG_ROWS;
 
 int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
                  int32_t n_kv_heads, int32_t head_dim, VarlenShape* out) {
-  constexpr int W = kShortWaves4;
   DeviceState* ds = nullptr;
   const int rc = current_device_state(&ds);
   if (rc) return rc;
-  const int64_t group = n_q_heads / n_kv_heads, tile_rows = W * kUnitRows;
+  const int64_t group = n_q_heads / n_kv_heads;
+  const bool long_rows = (int64_t)max_q * group > kLongRows;
+  VarlenShape s{};
+  s.waves = long_rows ? kLongWaves4 : kShortWaves4;
+  const int64_t tile_rows = s.waves * kUnitRows;
   const int64_t max_tiles = ((int64_t)max_q * group + tile_rows - 1) / tile_rows;
   // row tiles: those that the tokens fill, and a part-filled one per sequence
   const int64_t tiles = std::min((int64_t)batch * max_tiles, total_q * group / tile_rows + batch);
   const int64_t jobs = tiles * n_kv_heads;
   const int64_t max_kt = ((int64_t)max_len + kPfKTile - 1) / kPfKTile;
-  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * kWorkgroupsPerCu4;
-  VarlenShape s{jobs, 0, 0, 0, 0};
-  if (jobs < 4 * slots && max_kt > kMinSplitTiles) {
-    s.target = 2 * slots;
+  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (long_rows ? 1 : 2);
+  s.pieces = jobs;
+  s.least = long_rows ? LEAST_LONG : LEAST_SHORT;
+  if (jobs < 4 * slots && max_kt > s.least) {
+    s.target = slots * (long_rows ? TGT_LONG : TGT_SHORT);
     // a sequence of cost x has at most x / span + its tiles
-    s.pieces = std::min(s.target + jobs, jobs * ((max_kt + kMinSplitTiles - 1) / kMinSplitTiles));
-    s.merge = jobs * W;
+    s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
+    s.merge = jobs * s.waves;
     s.ml_bytes = s.pieces * tile_rows * 8;
     s.o_bytes = s.pieces * tile_rows * head_dim * 4;
   }
@@ -652,12 +837,21 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
 
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
-  constexpr int W = kShortWaves4;
-  hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, W>), dim3((uint32_t)s.pieces), dim3(64 * W), 0, st, a);
+  const dim3 grid((uint32_t)s.pieces), merge((uint32_t)s.merge);
+  const bool long_rows = s.waves == kLongWaves4;
+  if (long_rows)
+    hipLaunchKernelGGL((kv4_varlen_long_kernel<DT, D>), grid, dim3(64 * kLongWaves4), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, kShortWaves4>), grid, dim3(64 * kShortWaves4), 0,
+                       st, a);
   AEGKV_HIP_TRY(hipGetLastError());
   if (s.target > 0) {
-    hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W>), dim3((uint32_t)s.merge),
-                       dim3(kMerge4Threads), 0, st, a);
+    if (long_rows)
+      hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, kLongWaves4>), merge, dim3(kMerge4Threads),
+                         0, st, a);
+    else
+      hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, kShortWaves4>), merge,
+                         dim3(kMerge4Threads), 0, st, a);
     AEGKV_HIP_TRY(hipGetLastError());
   }
   return AEGKV_OK;
@@ -736,6 +930,7 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
   a.scale_sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
   a.scale_log2 = scale == 0 ? 1.f : std::fabs(scale) * 1.4426950408889634f;
   a.target = s.target;
+  a.least = s.least;
   a.n_pieces = (int32_t)s.pieces;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.o_bytes);
