@@ -23,6 +23,7 @@
 // pieces wanted.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "aegkv_internal.h"
 #include "kv4_format.h"
@@ -62,15 +63,15 @@ struct VarlenArgs {
   float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
 };
 
-// What a sequence asks for, in tiles of W units.
+// What a sequence asks for, in row tiles of W units and steps of KS key tiles.
 struct SeqWork {
   int t0, m;        // first query token, queries (at most max_q)
   int off;          // key position of query 0
   int len;          // keys
   int rows, tiles;  // rows of one kv head, row tiles
-  int n_kt;         // key tiles that its last row sees
+  int n_kt;         // key steps that its last row sees
 };
-template <int W>
+template <int W, int KS>
 __device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
   SeqWork s;
   const int c0 = a.cu[b], c1 = a.cu[b + 1], n = max(a.seq_lens[b], 0);
@@ -82,11 +83,12 @@ __device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
   s.rows = s.m * a.group;
   s.tiles = (s.rows + kUnitRows * W - 1) / (kUnitRows * W);
   const int last = a.causal ? min(s.off + s.m, s.len) : s.len;  // keys of the last query
-  s.n_kt = s.m > 0 ? (max(last, 0) + kPfKTile - 1) / kPfKTile : 0;
+  s.n_kt = s.m > 0 ? (max(last, 0) + KS * kPfKTile - 1) / (KS * kPfKTile) : 0;
   return s;
 }
 
-// One piece of work: the sequence, its kv head, row tile and range of key tiles.
+// One piece of work: the sequence, its kv head, row tile and range of key steps;
+// to the merge, the R rows from tile * R.
 struct Piece {
   SeqWork s;
   int b, head, tile, split, splits, span, first;  // first: the sequence's first piece
@@ -100,16 +102,17 @@ struct LocateLds {
 __device__ __forceinline__ int ranges_of(int n_kt, int span) {
   return max(1, (n_kt + span - 1) / span);
 }
-// The piece (MERGE: the 32-row unit of a cut tile) numbered `index`, found by
-// all NT threads, each summing its own sequences.  False: there are fewer.
-template <int W, int NT, bool MERGE>
+// The piece (R > 0: the R rows of a cut sequence's kv head) numbered `index`,
+// found by all NT threads, each summing its own sequences.  False: there are
+// fewer.
+template <int W, int KS, int NT, int R = 0>
 __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds& x, Piece& p) {
   constexpr int NW = NT / 64;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.batch + NT - 1) / NT, b0 = min(t * per, a.batch), b1 = min(b0 + per, a.batch);
   // the thread's first sequence, its only one in batches of up to NT
-  const SeqWork mine = seq_work<W>(a, min(b0, a.batch - 1));
-  auto work = [&](int b) { return b == b0 ? mine : seq_work<W>(a, b); };
+  const SeqWork mine = seq_work<W, KS>(a, min(b0, a.batch - 1));
+  auto work = [&](int b) { return b == b0 ? mine : seq_work<W, KS>(a, b); };
   int span = INT32_MAX;
   if (a.target > 0) {  // uniform
     int64_t cost = 0;
@@ -132,7 +135,7 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   auto add = [&](const SeqWork& s, int& units, int& pieces) {
     const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
     pieces += n * r;
-    units += MERGE ? (r > 1 ? n * W : 0) : n * r;
+    units += R == 0 ? n * r : r > 1 ? (s.rows + R - 1) / max(R, 1) * a.n_kv_heads : 0;
     return r;
   };
   for (int b = b0; b < b1; ++b) add(work(b), count, before);
@@ -188,19 +191,29 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   p.s.rows = f[9];
   p.s.tiles = f[10];
   // kv heads slowest, then row tiles from the last (the most keys) to the first
-  const int per_tile = MERGE ? W : p.splits;
-  const int q = f[1] / per_tile;
-  p.split = f[1] - q * per_tile;  // MERGE: the unit
-  p.head = q / p.s.tiles;
-  p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
+  if constexpr (R > 0) {
+    const int per_head = (p.s.rows + R - 1) / R;
+    p.head = f[1] / per_head;
+    p.tile = f[1] - p.head * per_head;
+    p.split = 0;
+  } else {
+    const int q = f[1] / p.splits;
+    p.split = f[1] - q * p.splits;
+    p.head = q / p.s.tiles;
+    p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
+  }
   return true;
 }
 
+// Nothing is scheduled across: the softmax would otherwise sink into the next
+// matrix phase.
 #define KV4_BARRIER()                                  \
   do {                                                 \
+    __builtin_amdgcn_sched_barrier(0);                 \
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); \
     __builtin_amdgcn_s_barrier();                      \
     asm volatile("" ::: "memory");                     \
+    __builtin_amdgcn_sched_barrier(0);                 \
   } while (0)
 
 // The K or V codes of one block for one lane, as in the decode attention:
@@ -297,6 +310,42 @@ __device__ __forceinline__ bool put_v(uint8_t* lds, CodeRegs<D>& c, int u, int l
   return __builtin_amdgcn_ballot_w64(bad) != 0;
 }
 
+// The block ids of a piece's key tiles, 16 tiles at a time, one id per lane, with
+// the next 16 tiles' loaded ahead.  Tiles are asked for in order.
+struct TileIds {
+  const int32_t* table;  // the sequence's, n_blk > 0 entries
+  int n_blk, n_blocks;   // (pools are below 2^31 blocks, as ids are int32)
+  int base, cur, next;   // first tile at hand
+  __device__ __forceinline__ int from(int tile) const {
+    return table[min(tile * kTileBlocks + (int)(threadIdx.x & 63), n_blk - 1)];
+  }
+  __device__ __forceinline__ void start(int tile) {
+    base = tile;
+    cur = from(tile);
+    next = from(tile + 16);
+  }
+  __device__ __forceinline__ void reach(int tile) {
+    if (tile - base == 16) {
+      cur = next;
+      base += 16;
+      next = from(base + 16);
+    }
+  }
+  // the id of block u of the tile, -1 when it is none of the sequence's or unreadable
+  __device__ __forceinline__ int id(int tile, int u) const {
+    const int x = __builtin_amdgcn_readlane(cur, ((tile - base) * kTileBlocks + u) & 63);
+    return tile * kTileBlocks + u < n_blk && x >= 0 && x < n_blocks ? x : -1;
+  }
+  // the tile's blocks that are the sequence's and unreadable
+  __device__ __forceinline__ uint32_t unreadable(int tile) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int u = 0; u < kTileBlocks; ++u)
+      if (tile * kTileBlocks + u < n_blk && id(tile, u) < 0) m |= 1u << u;
+    return m;
+  }
+};
+
 // A wave's unit of 32 rows.
 template <int DT, int D>
 struct RowUnit : WaveSoftmax<DT, D> {
@@ -309,7 +358,7 @@ struct RowUnit : WaveSoftmax<DT, D> {
   using Base::qv;
   int r0, rows;     // first row; the sequence's rows
   int limit;        // last key of this lane's row (-1: none)
-  int lim_lo, lim_hi;  // of the unit's first and last row
+  int lim_lo;       // of the unit's first row
   uint32_t spoiled;    // bit: dims 32 db .. of this lane's row are NaN
 
   __device__ __forceinline__ void init(const VarlenArgs& a, const SeqWork& s, int head, int unit) {
@@ -324,7 +373,6 @@ struct RowUnit : WaveSoftmax<DT, D> {
     };
     limit = last_of(r);
     lim_lo = last_of(r0);
-    lim_hi = r0 < rows ? last_of(r0 + kUnitRows - 1) : -1;
     const uint8_t* qp = a.q + (int64_t)(s.t0 + i) * a.q_tok_b + ((int64_t)h * D + 8 * hh) * 2;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qv[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
@@ -345,7 +393,6 @@ struct RowUnit : WaveSoftmax<DT, D> {
 #pragma unroll
       for (int e = 0; e < 4; ++e) qv[ks][e] = sign < 0 ? qv[ks][e] ^ 0x80008000u : 0u;
   }
-  __device__ __forceinline__ bool sees(int kt) const { return kt * kPfKTile <= lim_hi; }  // uniform
 
   // ORDERED: LDS reads stay two MFMAs ahead of their use (pv: four), as the long
   // prompts' kernel orders them
@@ -377,6 +424,7 @@ struct RowUnit : WaveSoftmax<DT, D> {
   // -inf for keys past a row's last one and for unreadable blocks (bit u)
   __device__ __forceinline__ void mask(f32x16 (&s)[2], int k0, uint32_t unreadable) const {
     if (k0 + kPfKTile - 1 > lim_lo || unreadable) {
+      asm volatile("");  // a branch, not selects on every tile
       const int hh = (threadIdx.x & 63) >> 5, last = limit - k0 - 4 * hh;
 #pragma unroll
       for (int u = 0; u < kTileBlocks; ++u) {
@@ -443,6 +491,27 @@ struct RowUnit : WaveSoftmax<DT, D> {
   __device__ __forceinline__ float finite_or_nan(int db) const {
     return spoiled >> db & 1 ? __builtin_nanf("") : 1.f;
   }
+  // The sums to and from LDS, one float per lane and register (no key: -inf, 0, 0).
+  __device__ __forceinline__ void put_sums(uint8_t* x) const {
+    float* f = reinterpret_cast<float*>(x) + (threadIdx.x & 63);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[64 * (16 * db + e)] = o[db][e];
+    f[64 * 16 * DB] = m;
+    f[64 * (16 * DB + 1)] = lsum;
+  }
+  __device__ __forceinline__ void add_sums(const uint8_t* x) {
+    const float* f = reinterpret_cast<const float*>(x) + (threadIdx.x & 63);
+    const float m2 = f[64 * 16 * DB], mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+    const float w1 = __builtin_amdgcn_exp2f(m - ref), w2 = __builtin_amdgcn_exp2f(m2 - ref);
+    lsum = lsum * w1 + f[64 * (16 * DB + 1)] * w2;
+    m = mn;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = o[db][e] * w1 + f[64 * (16 * db + e)] * w2;
+  }
   __device__ __forceinline__ float total() const { return lsum + __shfl_xor(lsum, 32); }
 
   // normalise and store the rows (x: 32 rows of LDS of the wave's own), as the
@@ -492,97 +561,111 @@ struct RowUnit : WaveSoftmax<DT, D> {
   }
 };
 
-// W = 4: wave w converts block w of each key tile.
-template <int DT, int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void kv4_varlen_kernel(VarlenArgs a) {
-  static_assert(W == kTileBlocks, "a block per wave");
+// Four waves.  KS = 1: four units, and wave w converts block w of each key tile.
+// KS = 2, for row tiles of up to two units: waves 2 and 3 take the units of waves 0
+// and 1 over the second of two key tiles per step, and the pairs are joined at the
+// end.  (Two waves converting only: 48 x 5 drafted tokens over 1000 each of 32/4
+// heads 49.7 us, so 31.1.)
+template <int DT, int D, int KS>
+__global__ __launch_bounds__(64 * kShortWaves4, 2) void kv4_varlen_kernel(VarlenArgs a) {
+  constexpr int NW = kShortWaves4, W = NW / KS;  // waves, units of a row tile
   constexpr int T_BYTES = kPfKTile * D * 2;
+  static_assert(NW == kTileBlocks, "a block of each key tile per wave");
   static_assert(W * kUnitRows * D * 2 <= 2 * T_BYTES, "the outputs fit the tiles");
-  __shared__ __align__(16) uint8_t lds[2 * T_BYTES];  // K, then V
-  __shared__ uint32_t s_nan[W];
+  static_assert(KS == 1 || W * 64 * (D / 2 + 3) * 4 <= KS * 2 * T_BYTES, "the joined halves fit");
+  __shared__ __align__(16) uint8_t lds[KS * 2 * T_BYTES];  // K and V of each key tile
+  __shared__ uint32_t s_nan[NW];
   __shared__ LocateLds s_loc;
   Piece p;
-  if (!locate<W, 64 * W, false>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  if (!locate<W, KS, 64 * NW>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
   const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = w / W;  // the key tile of a step that the wave attends to
   const int n_blk = (s.len + kKv4Tokens - 1) / kKv4Tokens;
-  // the key tiles of this piece that the tile's last row sees
+  // the key steps of this piece that the tile's last row sees
   const int last_q = a.by_group.div(min(s.rows, (p.tile + 1) * W * kUnitRows) - 1);
   const int keys = a.causal ? min(s.off + last_q + 1, s.len) : s.len;
   const int kt0 = p.split * p.span;
-  const int kt1 = min(kt0 + p.span, (max(keys, 0) + kPfKTile - 1) / kPfKTile);
+  const int kt1 =
+      min(kt0 + p.span, (max(keys, 0) + KS * kPfKTile - 1) / (KS * kPfKTile));
 
   RowUnit<DT, D> unit;
-  unit.init(a, s, p.head, p.tile * W + w);
+  unit.init(a, s, p.head, p.tile * W + w % W);
   unit.sign_queries(a.scale_sign);
 
-  // block ids of 16 key tiles, one per lane, and the next 16
   const int32_t* table = a.tables + (int64_t)p.b * a.max_blocks;
-  auto ids_from = [&](int blk) -> int { return table[min(blk + lane, n_blk - 1)]; };
   const int64_t head_off = (int64_t)p.head * 17 * D;
-  int base = kt0 * kTileBlocks, ids = 0, ids_next = 0;
-  uint32_t unreadable = 0, unreadable_next = 0;
-  CodeRegs<D> ck, cv;
-  auto load = [&](int kt) {
-    const int blk = kt * kTileBlocks;
-    if (blk - base >= 64) {
-      ids = ids_next;
-      base += 64;
-      ids_next = ids_from(base + 64);
-    }
-    unreadable_next = 0;
-    bool mine = false;
-    int my_id = 0;
-#pragma unroll
-    for (int u = 0; u < kTileBlocks; ++u) {
-      const int id = __builtin_amdgcn_readlane(ids, blk - base + u);
-      const bool ok = blk + u < n_blk && id >= 0 && id < a.n_blocks;
-      if (blk + u < n_blk && !ok) unreadable_next |= 1u << u;
-      if (u == w) {
-        mine = ok;
-        my_id = id;
-      }
-    }
-    const auto r = byte_range(a.cache + (int64_t)(mine ? my_id : 0) * a.blk_b + head_off,
-                              mine ? 17 * D : 0u);
-    load_k<D>(ck, r, lane);
-    load_v<D>(cv, r, lane);
-  };
-  if (kt0 < kt1) {
-    ids = ids_from(base);
-    ids_next = ids_from(base + 64);
-    load(kt0);
-  }
   bool nan = false;
-  for (int kt = kt0; kt < kt1; ++kt) {
-    if (kt > kt0) KV4_BARRIER();  // every wave's reads of the tile before
-    put_k<DT, D>(lds, ck, w, lane);
-    const int left = s.len - (kt * kTileBlocks + w) * kKv4Tokens;
-    nan |= put_v<DT, D>(lds + T_BYTES, cv, w, left, lane);
-    unreadable = unreadable_next;
-    if (kt + 1 < kt1) load(kt + 1);
-    KV4_BARRIER();
-    if (unit.sees(kt)) {
-      f32x16 sc[2];
-      u32x4 pb[4];
-      unit.template qk<false>(lds, sc);
-      unit.mask(sc, kt * kPfKTile, unreadable);
-      unit.softmax(sc, pb, a.scale_log2, kt == kt0);
-      __builtin_amdgcn_sched_barrier(0);  // V's reads stay behind the softmax: registers
-      unit.template pv<false>(lds + T_BYTES, pb);
+  if (kt0 < kt1) {  // uniform
+    TileIds ids{table, n_blk, (int)min(a.n_blocks, (int64_t)INT32_MAX)};
+    ids.start(kt0 * KS);
+    // this wave's codes of the next step (tiles past the piece: nothing)
+    struct {
+      CodeRegs<D> k, v;
+    } next[KS];
+    uint32_t unreadable_next = 0;  // of the wave's key tile
+    auto load = [&](int kt) {
+      ids.reach(kt * KS);
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const int id = kt < kt1 ? ids.id(kt * KS + t, w) : -1;
+        const auto r = byte_range(a.cache + (int64_t)max(id, 0) * a.blk_b + head_off,
+                                  id >= 0 ? 17 * D : 0u);
+        load_k<D>(next[t].k, r, lane);
+        load_v<D>(next[t].v, r, lane);
+      }
+      unreadable_next = kt < kt1 ? ids.unreadable(kt * KS + part) : 0u;
+    };
+    uint8_t* mine = lds + part * 2 * T_BYTES;
+    // No step is skipped for rows that do not see it: branches around the products
+    // had their accumulators copied.  A wave without rows only converts.
+    auto step = [&](auto with_rows, int kt) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        uint8_t* tile = lds + t * 2 * T_BYTES;
+        put_k<DT, D>(tile, next[t].k, w, lane);
+        nan |= put_v<DT, D>(tile + T_BYTES, next[t].v, w,
+                            s.len - ((kt * KS + t) * kTileBlocks + w) * kKv4Tokens, lane);
+      }
+      const uint32_t unreadable = unreadable_next;
+      load(kt + 1);
+      KV4_BARRIER();
+      if constexpr (decltype(with_rows)::value) {
+        f32x16 sc[2];
+        u32x4 pb[4];
+        unit.template qk<false>(mine, sc);
+        unit.mask(sc, (kt * KS + part) * kPfKTile, unreadable);
+        unit.softmax(sc, pb, a.scale_log2, kt == kt0);
+        __builtin_amdgcn_sched_barrier(0);  // V's reads stay behind the softmax: registers
+        unit.template pv<false>(mine + T_BYTES, pb);
+      }
+      KV4_BARRIER();  // every wave's reads of the tiles
+    };
+    load(kt0);
+    if (unit.r0 < s.rows) {
+      for (int kt = kt0; kt < kt1; ++kt) step(std::true_type{}, kt);
+    } else {
+      for (int kt = kt0; kt < kt1; ++kt) step(std::false_type{}, kt);
     }
   }
-  if (lane == 0) s_nan[w] = nan;
-  KV4_BARRIER();  // and the tiles: every wave is past its last read of them
+  if constexpr (KS > 1) {  // the second key tiles' sums to the waves of the first
+    uint8_t* x = lds + w % W * (64 * (D / 2 + 3) * 4);
+    if (part > 0) unit.put_sums(x);
+    if (lane == 0) s_nan[w] = nan;
+    KV4_BARRIER();
+    if (part == 0) unit.add_sums(x);
+  } else {
+    if (lane == 0) s_nan[w] = nan;
+  }
+  KV4_BARRIER();
   nan = false;
 #pragma unroll
-  for (int i = 0; i < W; ++i) nan |= s_nan[i] != 0;
-  if (__builtin_amdgcn_readfirstlane(nan)) unit.find_nan(a, table, head_off, s.len, kt0, kt1);
-  if (p.splits > 1) {
-    unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
-    return;
-  }
-  unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
+  for (int i = 0; i < NW; ++i) nan |= s_nan[i] != 0;
+  if (part > 0) return;
+  if (__builtin_amdgcn_readfirstlane(nan))
+    unit.find_nan(a, table, head_off, s.len, kt0 * KS, kt1 * KS);
+  if (p.splits > 1) unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
+  else unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
 }
 
 // Long rows: eight units in ping-pong, as the long prompts' kernel runs them.
@@ -602,7 +685,7 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   __shared__ uint32_t s_nan[W / 2];
   __shared__ LocateLds s_loc;
   Piece p;
-  if (!locate<W, 64 * W, false>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  if (!locate<W, 1, 64 * W>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
   const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = w >> 2, u = w & 3;  // and the block of each tile that the wave converts
@@ -615,50 +698,34 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   RowUnit<DT, D> unit;
   unit.init(a, s, p.head, p.tile * W + w);
   unit.sign_queries(a.scale_sign);
-  // tiles j of the piece that the wave's rows see
-  const int jw = min(n_kt, unit.lim_hi < 0 ? 0 : max(unit.lim_hi / kPfKTile + 1 - kt0, 0));
 
   const int32_t* table = a.tables + (int64_t)p.b * a.max_blocks;
-  auto ids_from = [&](int blk) -> int { return table[min(blk + lane, n_blk - 1)]; };
   const int64_t head_off = (int64_t)p.head * 17 * D;
-  // ids of 16 key tiles from tile `base` of the piece, and of the next 16
-  int base = 0, ids = 0, ids_next = 0;
-  auto id_of = [&](int j, int x) -> int {  // -1: unreadable
-    const int id = __builtin_amdgcn_readlane(ids, (j - base) * kTileBlocks + x);
-    return id >= 0 && id < a.n_blocks ? id : -1;
-  };
-  // the blocks of tile j that are unreadable (a tile at or before the one loaded)
-  auto bad_of = [&](int j) -> uint32_t {
-    uint32_t m = 0;
-    for (int x = 0; x < kTileBlocks; ++x)
-      if ((kt0 + j) * kTileBlocks + x < n_blk && id_of(j, x) < 0) m |= 1u << x;
-    return m;
-  };
-  CodeRegs<D> c;
-  uint32_t bad_now = 0, bad_next = 0;  // of the tile computed, of the one loaded
-  // this wave's codes of tile j (none past the piece): K of block u, or V
-  auto load = [&](int j) {
-    if (j - base == 16) {
-      ids = ids_next;
-      base += 16;
-      ids_next = ids_from((kt0 + base + 16) * kTileBlocks);
-    }
-    const int id = j < n_kt && (kt0 + j) * kTileBlocks + u < n_blk ? id_of(j, u) : -1;
-    bad_next = j < n_kt ? bad_of(j) : 0;
-    const auto r = byte_range(a.cache + (int64_t)max(id, 0) * a.blk_b + head_off,
-                              id >= 0 ? 17 * D : 0u);
-    if (half == 0) load_k<D>(c, r, lane);
-    else load_v<D>(c, r, lane);
+  TileIds ids{table, n_blk, (int)min(a.n_blocks, (int64_t)INT32_MAX)};
+  // this wave's codes of two key tiles (K of block u, or V), loaded two tiles
+  // ahead of their conversion (tiles past the piece: nothing), and the unreadable
+  // blocks of three tiles: of the one computed and the two loaded
+  CodeRegs<D> c[2];
+  uint32_t bad[3] = {};
+  auto load = [&](CodeRegs<D>& r, int j) {
+    ids.reach(kt0 + j);
+    const int id = j < n_kt ? ids.id(kt0 + j, u) : -1;
+    bad[2] = j < n_kt ? ids.unreadable(kt0 + j) : ~0u;
+    const auto range = byte_range(a.cache + (int64_t)max(id, 0) * a.blk_b + head_off,
+                                  id >= 0 ? 17 * D : 0u);
+    if (half == 0) load_k<D>(r, range, lane);
+    else load_v<D>(r, range, lane);
   };
   bool nan = false;
-  auto put = [&](int j) {  // and the loads of the tile after it
-    if (half == 0) {
-      put_k<DT, D>(lds + (j & 1) * T_BYTES, c, u, lane);
-    } else {
-      const int left = s.len - ((kt0 + j) * kTileBlocks + u) * kKv4Tokens;
-      nan |= put_v<DT, D>(lds + (2 + (j & 1)) * T_BYTES, c, u, left, lane);
-    }
-    load(j + 1);
+  auto put = [&](CodeRegs<D>& r, int j) {  // and the loads of the tile two further on
+    if (half == 0)
+      put_k<DT, D>(lds + (j & 1) * T_BYTES, r, u, lane);
+    else
+      nan |= put_v<DT, D>(lds + (2 + (j & 1)) * T_BYTES, r, u,
+                          s.len - ((kt0 + j) * kTileBlocks + u) * kKv4Tokens, lane);
+    bad[0] = bad[1];
+    bad[1] = bad[2];
+    load(r, j + 2);
   };
   auto qk = [&](int j, f32x16 (&sc)[2]) { unit.template qk<true>(lds + (j & 1) * T_BYTES, sc); };
   auto softmax = [&](int j, f32x16 (&sc)[2], u32x4 (&pb)[4], uint32_t bad) {
@@ -670,47 +737,41 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   };
 
   u32x4 pb[4];
-  if (n_kt > 0) {  // uniform: every wave passes 2 n_kt + 3 barriers
-    ids = ids_from(kt0 * kTileBlocks);
-    ids_next = ids_from((kt0 + 16) * kTileBlocks);
-    load(0);
-    if (half == 0) {
-      bad_now = bad_next;
-      put(0);  // K_0; loads K_1
-      KV4_BARRIER();
-      for (int j = 0; j < n_kt; ++j) {
-        f32x16 sc[2];  // slot 2j
-        if (j < jw) qk(j, sc);
-        if (j >= 1 && j - 1 < jw) pv(j - 1, pb);
-        KV4_BARRIER();
-        const uint32_t bad = bad_now;  // slot 2j + 1
-        bad_now = bad_next;
-        if (j + 1 < n_kt) put(j + 1);
-        if (j < jw) softmax(j, sc, pb, bad);
-        KV4_BARRIER();
-      }
-      if (n_kt - 1 < jw) pv(n_kt - 1, pb);  // slot 2 n_kt
-      KV4_BARRIER();
-      KV4_BARRIER();
-    } else {
-      KV4_BARRIER();
-      bad_now = bad_next;
-      put(0);  // slot 0: V_0; loads V_1
-      KV4_BARRIER();
-      for (int j = 0; j < n_kt; ++j) {
-        f32x16 sc[2];  // slot 2j + 1
-        if (j < jw) qk(j, sc);
-        if (j >= 1 && j - 1 < jw) pv(j - 1, pb);
-        KV4_BARRIER();
-        const uint32_t bad = bad_now;  // slot 2j + 2
-        bad_now = bad_next;
-        if (j + 1 < n_kt) put(j + 1);
-        if (j < jw) softmax(j, sc, pb, bad);
-        KV4_BARRIER();
-      }
-      if (n_kt - 1 < jw) pv(n_kt - 1, pb);  // slot 2 n_kt + 1
+  // Tile j: the matrix phase, then the softmax with the conversion of tile j + 1.
+  // Tiles come in pairs behind the first, as the codes ahead have two sets of
+  // registers; a tile past the piece is masked like an unreadable one, and none is
+  // skipped for rows that do not see it (branches around the products had their
+  // accumulators copied).
+  auto tile = [&](auto first, int j, CodeRegs<D>& next) {
+    f32x16 sc[2];
+    qk(j, sc);
+    if constexpr (!decltype(first)::value) pv(j - 1, pb);
+    KV4_BARRIER();
+    const uint32_t unreadable = bad[0];
+    put(next, j + 1);
+    softmax(j, sc, pb, unreadable);
+    KV4_BARRIER();
+  };
+  if (n_kt > 0) {  // uniform: every wave passes 2 (n_kt rounded up to odd) + 3 barriers
+    ids.start(kt0);
+    load(c[0], 0);
+    bad[1] = bad[2];
+    load(c[1], 1);
+    if (half == 0) put(c[0], 0);  // K_0
+    KV4_BARRIER();
+    if (half == 1) {
+      put(c[0], 0);  // slot 0: V_0
       KV4_BARRIER();
     }
+    tile(std::true_type{}, 0, c[1]);
+    int j = 1;
+    for (; j < n_kt; j += 2) {
+      tile(std::false_type{}, j, c[0]);
+      tile(std::false_type{}, j + 1, c[1]);
+    }
+    pv(j - 1, pb);  // slot 2 j, or 2 j + 1
+    KV4_BARRIER();
+    if (half == 0) KV4_BARRIER();
   }
   if (half == 1 && lane == 0) s_nan[u] = nan;
   KV4_BARRIER();  // and the stages: every wave is past its last read of them
@@ -723,44 +784,65 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   else unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
 }
 
-// Merges the pieces of one 32-row unit of a cut tile:
-//   out = sum_s w_s o_s / sum_s w_s l_s,  w_s = 2^(m_s - max m);
-// eight threads per row, D / 8 columns each.
+// Merges the pieces of R rows of a cut sequence's kv head:
+//   out = sum_s w_s o_s / sum_s w_s l_s,  w_s = 2^(m_s - max m).
+// Eight threads take a row's columns, and 32 / R slices of them the pieces in
+// turn, which meet in LDS: with few rows each slice has few pieces and the loads
+// of all are one round trip.  (One slice: a query over 60000 tokens in 235 pieces
+// 62 us.)
 constexpr int kMerge4Threads = 256;
-template <int DT, int D, int W>
+template <int DT, int D, int W, int KS, int R>
 __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(VarlenArgs a) {
+  constexpr int SL = 32 / R, NV = D / 32;
   __shared__ LocateLds s_loc;
+  __shared__ f32x4 s_o[SL > 1 ? SL : 1][SL > 1 ? R : 1][SL > 1 ? D / 4 : 1];
+  __shared__ float2 s_ml[SL][R];
   Piece p;
-  if (!locate<W, kMerge4Threads, true>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  if (!locate<W, KS, kMerge4Threads, R>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
   const SeqWork& s = p.s;
-  const int row = (int)threadIdx.x >> 3, part = threadIdx.x & 7;
-  const int r = (p.tile * W + p.split) * kUnitRows + row;  // p.split: the unit
-  if (r >= s.rows) return;
+  const int part = threadIdx.x & 7, row = ((int)threadIdx.x >> 3) % R, sl = ((int)threadIdx.x >> 3) / R;
+  const int r = p.tile * R + row, tile = r / (W * kUnitRows);
   // the tile's pieces follow each other (locate); those past the grid were not run
-  const int piece0 = p.first + (p.head * s.tiles + s.tiles - 1 - p.tile) * p.splits;
-  const int n = min(p.splits, a.n_pieces - piece0);
-  const int64_t row0 = ((int64_t)piece0 * W + p.split) * kUnitRows + row;
+  const int piece0 = p.first + (p.head * s.tiles + s.tiles - 1 - tile) * p.splits;
+  const int n = r < s.rows ? min(p.splits, a.n_pieces - piece0) : 0;
   constexpr int64_t kStep = (int64_t)W * kUnitRows;  // slot rows from piece to piece
-  float mx = -INFINITY;
-  for (int k = 0; k < n; ++k) mx = fmaxf(mx, a.part_ml[row0 + k * kStep].x);
-  constexpr int NV = D / 32;
+  const int64_t row0 = (int64_t)piece0 * kStep + (r - tile * kStep);
+  float mx = -INFINITY, lt = 0.f;
   f32x4 acc[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float lt = 0.f;
-#pragma unroll 2
-  for (int k = 0; k < n; ++k) {
+  auto add = [&](float m2, float l2, const f32x4 (&v)[NV]) {
+    const float mn = fmaxf(mx, m2), ref = mn == -INFINITY ? 0.f : mn;
+    const float w1 = __builtin_amdgcn_exp2f(mx - ref), w2 = __builtin_amdgcn_exp2f(m2 - ref);
+    lt = lt * w1 + l2 * w2;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = acc[i] * w1 + v[i] * w2;
+    mx = mn;
+  };
+#pragma unroll 4
+  for (int k = sl; k < n; k += SL) {
     const float2 ml = a.part_ml[row0 + k * kStep];
     const float* po = a.part_o + (row0 + k * kStep) * D + 4 * part;
     f32x4 v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const f32x4*>(po + 32 * i);
-    // a piece without a key of this row: nothing
-    const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mx);
-    lt += ml.y * w;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] += v[i] * w;
+    add(ml.x, ml.y, v);
   }
+  if constexpr (SL > 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s_o[sl][row][8 * i + part] = acc[i];
+    if (part == 0) s_ml[sl][row] = make_float2(mx, lt);
+    __syncthreads();
+    if (sl > 0) return;
+#pragma unroll
+    for (int k = 1; k < SL; ++k) {
+      f32x4 v[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = s_o[k][row][8 * i + part];
+      add(s_ml[k][row].x, s_ml[k][row].y, v);
+    }
+  }
+  if (r >= s.rows) return;
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   const int i = a.by_group.div(r), h = p.head * a.group + r - i * a.group;
   uint8_t* op = a.out + (int64_t)(s.t0 + i) * a.o_tok_b + ((int64_t)h * D + 4 * part) * 2;
@@ -774,17 +856,19 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
 // The launch of a call: which kernel, how many pieces at most, and whether
 // sequences are cut.
 struct VarlenShape {
-  int waves;        // of a workgroup: units of a row tile
+  bool long_rows;
+  int key_tiles;    // of a step
   int64_t pieces;   // bound of the pieces (the main grid)
   int64_t target;   // pieces wanted (0: uncut)
-  int32_t least;    // key tiles of a piece at least
-  int64_t merge;    // bound of the merge's units
+  int32_t least;    // key steps of a piece at least
+  int merge_rows;   // rows of a merge workgroup
+  int64_t merge;    // bound of the merge's workgroups
   int64_t o_bytes, ml_bytes;
 };
 #ifndef LONG_ROWS
 #define LONG_ROWS 512
-#define TGT_LONG 1
-#define TGT_SHORT 1
+#define TGT_LONG 256
+#define TGT_SHORT 512
 #define LEAST_LONG 16
 #define LEAST_SHORT 4
 #endif
@@ -795,24 +879,30 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   DeviceState* ds = nullptr;
   const int rc = current_device_state(&ds);
   if (rc) return rc;
-  const int64_t group = n_q_heads / n_kv_heads;
-  const bool long_rows = (int64_t)max_q * group > kLongRows;
+  const int64_t group = n_q_heads / n_kv_heads, max_rows = (int64_t)max_q * group;
   VarlenShape s{};
-  s.waves = long_rows ? kLongWaves4 : kShortWaves4;
-  const int64_t tile_rows = s.waves * kUnitRows;
-  const int64_t max_tiles = ((int64_t)max_q * group + tile_rows - 1) / tile_rows;
+  s.long_rows = max_rows > kLongRows;
+  s.key_tiles = max_rows <= kShortWaves4 / 2 * kUnitRows ? 2 : 1;
+  const int64_t tile_rows =
+      (s.long_rows ? kLongWaves4 : kShortWaves4 / s.key_tiles) * kUnitRows;
   // row tiles: those that the tokens fill, and a part-filled one per sequence
-  const int64_t tiles = std::min((int64_t)batch * max_tiles, total_q * group / tile_rows + batch);
+  const int64_t tiles = std::min(batch * ((max_rows + tile_rows - 1) / tile_rows),
+                                 total_q * group / tile_rows + batch);
   const int64_t jobs = tiles * n_kv_heads;
-  const int64_t max_kt = ((int64_t)max_len + kPfKTile - 1) / kPfKTile;
-  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (long_rows ? 1 : 2);
+  const int64_t step = (int64_t)s.key_tiles * kPfKTile;
+  const int64_t max_kt = (max_len + step - 1) / step;
   s.pieces = jobs;
-  s.least = long_rows ? LEAST_LONG : LEAST_SHORT;
+  s.least = s.long_rows ? LEAST_LONG : LEAST_SHORT;
+  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (s.long_rows ? 1 : 2);
   if (jobs < 4 * slots && max_kt > s.least) {
-    s.target = slots * (long_rows ? TGT_LONG : TGT_SHORT);
+    s.target = slots * (s.long_rows ? TGT_LONG : TGT_SHORT) / 256;
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
-    s.merge = jobs * s.waves;
+    auto merges = [&](int64_t r) {
+      return n_kv_heads * std::min(batch * ((max_rows + r - 1) / r), total_q * group / r + batch);
+    };
+    s.merge_rows = merges(4) <= 4096 ? 4 : 32;
+    s.merge = merges(s.merge_rows);
     s.ml_bytes = s.pieces * tile_rows * 8;
     s.o_bytes = s.pieces * tile_rows * head_dim * 4;
   }
@@ -835,23 +925,23 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   return AEGKV_OK;
 }
 
+template <int DT, int D, int W, int KS>
+void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
+  const dim3 g((uint32_t)s.merge), t(kMerge4Threads);
+  if (s.merge_rows == 4) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, KS, 4>), g, t, 0, st, a);
+  else hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, KS, 32>), g, t, 0, st, a);
+}
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
-  const dim3 grid((uint32_t)s.pieces), merge((uint32_t)s.merge);
-  const bool long_rows = s.waves == kLongWaves4;
-  if (long_rows)
-    hipLaunchKernelGGL((kv4_varlen_long_kernel<DT, D>), grid, dim3(64 * kLongWaves4), 0, st, a);
-  else
-    hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, kShortWaves4>), grid, dim3(64 * kShortWaves4), 0,
-                       st, a);
+  const dim3 g((uint32_t)s.pieces), four(64 * kShortWaves4), eight(64 * kLongWaves4);
+  if (s.long_rows) hipLaunchKernelGGL((kv4_varlen_long_kernel<DT, D>), g, eight, 0, st, a);
+  else if (s.key_tiles == 2) hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 2>), g, four, 0, st, a);
+  else hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 1>), g, four, 0, st, a);
   AEGKV_HIP_TRY(hipGetLastError());
   if (s.target > 0) {
-    if (long_rows)
-      hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, kLongWaves4>), merge, dim3(kMerge4Threads),
-                         0, st, a);
-    else
-      hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, kShortWaves4>), merge,
-                         dim3(kMerge4Threads), 0, st, a);
+    if (s.long_rows) launch_merge<DT, D, kLongWaves4, 1>(a, s, st);
+    else if (s.key_tiles == 2) launch_merge<DT, D, kShortWaves4 / 2, 2>(a, s, st);
+    else launch_merge<DT, D, kShortWaves4, 1>(a, s, st);
     AEGKV_HIP_TRY(hipGetLastError());
   }
   return AEGKV_OK;
