@@ -61,6 +61,7 @@ struct VarlenArgs {
   int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
   float* part_o;             // [n_pieces][32 W][D]
   float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
+  uint32_t* any_cut;         // written by the main kernel (target > 0)
 };
 
 // What a sequence asks for, in row tiles of W units and steps of KS key tiles.
@@ -96,7 +97,7 @@ struct Piece {
 
 struct LocateLds {
   int64_t cost[16];
-  int sum[16], pieces[16];
+  int sum[16], pieces[16], cut[16];
   int found[11];
 };
 __device__ __forceinline__ int ranges_of(int n_kt, int span) {
@@ -132,9 +133,11 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
     span = max(span, a.least);
   }
   int count = 0, before = 0;  // this thread's units, and its pieces
+  bool cut = false;
   auto add = [&](const SeqWork& s, int& units, int& pieces) {
     const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
     pieces += n * r;
+    cut |= r > 1;
     units += R == 0 ? n * r : r > 1 ? (s.rows + R - 1) / max(R, 1) * a.n_kv_heads : 0;
     return r;
   };
@@ -152,8 +155,15 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
     x.sum[wave] = incl;
     x.pieces[wave] = pincl;
   }
+  const uint64_t cuts = __builtin_amdgcn_ballot_w64(cut);
+  if (lane == 0) x.cut[wave] = cuts != 0;
   if (t == 0) x.found[0] = -1;
   __syncthreads();
+  if (R == 0 && index == 0 && t == 0 && a.target > 0) {
+    int any = 0;
+    for (int w = 0; w < NW; ++w) any |= x.cut[w];
+    *a.any_cut = any;
+  }
   int excl = incl - count, pexcl = pincl - before;
   for (int w = 0; w < wave; ++w) {
     excl += x.sum[w];
@@ -797,6 +807,7 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
   __shared__ LocateLds s_loc;
   __shared__ f32x4 s_o[SL > 1 ? SL : 1][SL > 1 ? R : 1][SL > 1 ? D / 4 : 1];
   __shared__ float2 s_ml[SL][R];
+  if (*a.any_cut == 0) return;  // uniform
   Piece p;
   if (!locate<W, KS, kMerge4Threads, R>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
   const SeqWork& s = p.s;
@@ -865,14 +876,13 @@ struct VarlenShape {
   int64_t merge;    // bound of the merge's workgroups
   int64_t o_bytes, ml_bytes;
 };
-#ifndef LONG_ROWS
-#define LONG_ROWS 512
-#define TGT_LONG 256
-#define TGT_SHORT 512
-#define LEAST_LONG 16
-#define LEAST_SHORT 4
-#endif
-constexpr int kLongRows = LONG_ROWS;
+// More rows of a kv head than this take the ping-pong kernel (28/4 heads, 8 x 64
+// queries over 4000 tokens each, 448 rows: 77 us by four-wave workgroups, 73 by
+// eight; 8/8 heads, 4 x 256 over 2000, 256 rows: 37 and 58).
+constexpr int kLongRows = 256;
+// A piece's key steps at least: its partials cost about what half of these do
+// (48 x 5 drafted tokens over 1000 each: 31 us, with 8 steps 35, with 2 still 31).
+constexpr int kLeastLong = 16, kLeastShort = 4;
 
 int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
                  int32_t n_kv_heads, int32_t head_dim, VarlenShape* out) {
@@ -892,10 +902,17 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   const int64_t step = (int64_t)s.key_tiles * kPfKTile;
   const int64_t max_kt = (max_len + step - 1) / step;
   s.pieces = jobs;
-  s.least = s.long_rows ? LEAST_LONG : LEAST_SHORT;
+  s.least = s.long_rows ? kLeastLong : kLeastShort;
+  // Workgroups that run at once.  With half as many row tiles or fewer, their keys
+  // are cut into at most as many pieces (8 x 64 queries over 4000, 64 tiles: 74 us,
+  // whole 169, and in one piece per place and one per tile, which need a second
+  // round, 100); with more only sequences of twice the average work of a place, as
+  // partials cost more than an uneven last round (2048 queries over 16001 tokens,
+  // 224 tiles: whole 460 us, cut in two 498; 4 x 512 over 3800 each: 140 and 155).
+  // Four times as many tiles even out by themselves.
   const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (s.long_rows ? 1 : 2);
   if (jobs < 4 * slots && max_kt > s.least) {
-    s.target = slots * (s.long_rows ? TGT_LONG : TGT_SHORT) / 256;
+    s.target = jobs <= slots / 2 ? slots - jobs : slots / 2;
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     auto merges = [&](int64_t r) {
@@ -903,7 +920,7 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
     };
     s.merge_rows = merges(4) <= 4096 ? 4 : 32;
     s.merge = merges(s.merge_rows);
-    s.ml_bytes = s.pieces * tile_rows * 8;
+    s.ml_bytes = s.pieces * tile_rows * 8 + 256;  // and whether a sequence is cut
     s.o_bytes = s.pieces * tile_rows * head_dim * 4;
   }
   if (s.pieces > INT32_MAX / 2 || s.merge > INT32_MAX / 2) return AEGKV_ERR_UNSUPPORTED;
@@ -1024,6 +1041,8 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
   a.n_pieces = (int32_t)s.pieces;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.o_bytes);
+  a.any_cut = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + s.o_bytes +
+                                          s.ml_bytes - 256);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == AEGKV_DTYPE_BF16)
     return head_dim == 64 ? launch_varlen<AEGKV_DTYPE_BF16, 64>(a, s, st)
