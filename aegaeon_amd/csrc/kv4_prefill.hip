@@ -40,6 +40,12 @@ constexpr int kUnitRows = 32;   // rows of a wave
 constexpr int kTileBlocks = kPfKTile / kKv4Tokens;
 constexpr int kShortWaves4 = 4;
 
+// A row tile whose keys are cut: its rows [row0, row1) of kv head `head`, the first
+// of its pieces, which follow each other.
+struct CutTile {
+  int32_t t0, head, row0, row1, piece0, pieces;
+};
+
 struct VarlenArgs {
   const uint8_t* q;
   uint8_t* out;
@@ -61,7 +67,10 @@ struct VarlenArgs {
   int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
   float* part_o;             // [n_pieces][32 W][D]
   float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
-  uint32_t* any_cut;         // written by the main kernel (target > 0)
+  int32_t* n_cut;            // row tiles that are cut, and one CutTile each: written
+  CutTile* cut;              // by the main kernel (target > 0) for the merge
+  int32_t max_cut;           // bound of them
+  int32_t merge_per_tile;    // workgroups of the merge on a row tile
 };
 
 // What a sequence asks for, in row tiles of W units and steps of KS key tiles.
@@ -89,26 +98,26 @@ __device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
 }
 
 // One piece of work: the sequence, its kv head, row tile and range of key steps;
-// to the merge, the R rows from tile * R.
+// a cut row tile's number among those.
 struct Piece {
   SeqWork s;
-  int b, head, tile, split, splits, span, first;  // first: the sequence's first piece
+  int b, head, tile, split, splits, span, cut;
 };
 
 struct LocateLds {
   int64_t cost[16];
-  int sum[16], pieces[16], cut[16];
+  int sum[16], cut[16];
   int found[11];
 };
 __device__ __forceinline__ int ranges_of(int n_kt, int span) {
   return max(1, (n_kt + span - 1) / span);
 }
-// The piece (R > 0: the R rows of a cut sequence's kv head) numbered `index`,
-// found by all NT threads, each summing its own sequences.  False: there are
-// fewer.
-template <int W, int KS, int NT, int R = 0>
-__device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds& x, Piece& p) {
+// The piece numbered blockIdx.x, found by all NT threads, each summing its own
+// sequences.  False: there are fewer.  The first workgroup writes n_cut.
+template <int W, int KS, int NT>
+__device__ __forceinline__ bool locate(const VarlenArgs& a, LocateLds& x, Piece& p) {
   constexpr int NW = NT / 64;
+  const int index = (int)blockIdx.x;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.batch + NT - 1) / NT, b0 = min(t * per, a.batch), b1 = min(b0 + per, a.batch);
   // the thread's first sequence, its only one in batches of up to NT
@@ -121,9 +130,11 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
       const SeqWork s = work(b);
       cost += (int64_t)s.tiles * s.n_kt;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) cost += __shfl_xor(cost, o);
-    if (lane == 0) x.cost[wave] = cost;
+    // (the wave's sum in 25-bit digits, as 64 of them stay in 31 bits)
+    constexpr int kDigit = (1 << 25) - 1;
+    const int d0 = wave_prefix((int)cost & kDigit), d1 = wave_prefix((int)(cost >> 25) & kDigit),
+              d2 = wave_prefix((int)(cost >> 50));
+    if (lane == 63) x.cost[wave] = ((int64_t)d2 << 50) + ((int64_t)d1 << 25) + d0;
     __syncthreads();
     cost = 0;
 #pragma unroll
@@ -132,57 +143,43 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
     span = (int)min((cost + a.target - 1) / a.target, (int64_t)INT32_MAX);
     span = max(span, a.least);
   }
-  int count = 0, before = 0;  // this thread's units, and its pieces
-  bool cut = false;
-  auto add = [&](const SeqWork& s, int& units, int& pieces) {
+  int count = 0, cuts = 0;  // this thread's pieces and cut row tiles
+  auto add = [&](const SeqWork& s, int& pieces, int& cut) {
     const int n = s.tiles * a.n_kv_heads, r = ranges_of(s.n_kt, span);
     pieces += n * r;
-    cut |= r > 1;
-    units += R == 0 ? n * r : r > 1 ? (s.rows + R - 1) / max(R, 1) * a.n_kv_heads : 0;
+    cut += r > 1 ? n : 0;
     return r;
   };
-  for (int b = b0; b < b1; ++b) add(work(b), count, before);
-  int incl = count, pincl = before;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o), z = __shfl_up(pincl, o);
-    if (lane >= o) {
-      incl += y;
-      pincl += z;
-    }
-  }
+  for (int b = b0; b < b1; ++b) add(work(b), count, cuts);
+  const int incl = wave_prefix(count), cincl = wave_prefix(cuts);
   if (lane == 63) {
     x.sum[wave] = incl;
-    x.pieces[wave] = pincl;
+    x.cut[wave] = cincl;
   }
-  const uint64_t cuts = __builtin_amdgcn_ballot_w64(cut);
-  if (lane == 0) x.cut[wave] = cuts != 0;
   if (t == 0) x.found[0] = -1;
   __syncthreads();
-  if (R == 0 && index == 0 && t == 0 && a.target > 0) {
-    int any = 0;
-    for (int w = 0; w < NW; ++w) any |= x.cut[w];
-    *a.any_cut = any;
-  }
-  int excl = incl - count, pexcl = pincl - before;
+  int excl = incl - count, cexcl = cincl - cuts;
   for (int w = 0; w < wave; ++w) {
     excl += x.sum[w];
-    pexcl += x.pieces[w];
+    cexcl += x.cut[w];
   }
+  // (none if there are pieces past the grid: of overlapping sequences)
+  if (a.target > 0 && index == 0 && t == NT - 1)
+    *a.n_cut = excl + count <= a.n_pieces ? min(cexcl + cuts, a.max_cut) : 0;
   if (index >= excl && index < excl + count) {  // one thread
     for (int b = b0; b < b1; ++b) {
       const SeqWork s = work(b);
-      int units = 0, pieces = 0;
-      const int r = add(s, units, pieces);
-      if (index < excl + units) {
-        const int f[11] = {b,   index - excl, r,      (s.n_kt + r - 1) / r, pexcl, s.t0,
+      int pieces = 0, cut = 0;
+      const int r = add(s, pieces, cut);
+      if (index < excl + pieces) {
+        const int f[11] = {b,   index - excl, r,      (s.n_kt + r - 1) / r, cexcl, s.t0,
                            s.m, s.off,        s.len, s.rows,               s.tiles};
 #pragma unroll
         for (int i = 0; i < 11; ++i) x.found[i] = f[i];
         break;
       }
-      excl += units;
-      pexcl += pieces;
+      excl += pieces;
+      cexcl += cut;
     }
   }
   __syncthreads();
@@ -193,7 +190,6 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   if (p.b < 0) return false;
   p.splits = f[2];
   p.span = f[3];
-  p.first = f[4];
   p.s.t0 = f[5];
   p.s.m = f[6];
   p.s.off = f[7];
@@ -201,18 +197,20 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, int index, LocateLds
   p.s.rows = f[9];
   p.s.tiles = f[10];
   // kv heads slowest, then row tiles from the last (the most keys) to the first
-  if constexpr (R > 0) {
-    const int per_head = (p.s.rows + R - 1) / R;
-    p.head = f[1] / per_head;
-    p.tile = f[1] - p.head * per_head;
-    p.split = 0;
-  } else {
-    const int q = f[1] / p.splits;
-    p.split = f[1] - q * p.splits;
-    p.head = q / p.s.tiles;
-    p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
-  }
+  const int q = f[1] / p.splits;
+  p.split = f[1] - q * p.splits;
+  p.cut = f[4] + q;
+  p.head = q / p.s.tiles;
+  p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
   return true;
+}
+// A cut row tile's entry for the merge, by one thread of its first piece.
+template <int W>
+__device__ __forceinline__ void put_cut(const VarlenArgs& a, const Piece& p) {
+  if (p.splits == 1 || p.split || threadIdx.x || p.cut >= a.max_cut) return;
+  const int row0 = p.tile * W * kUnitRows;
+  a.cut[p.cut] = {p.s.t0, p.head, row0, min(row0 + W * kUnitRows, p.s.rows), (int)blockIdx.x,
+                  p.splits};
 }
 
 // Nothing is scheduled across: the softmax would otherwise sink into the next
@@ -587,7 +585,8 @@ __global__ __launch_bounds__(64 * kShortWaves4, 2) void kv4_varlen_kernel(Varlen
   __shared__ uint32_t s_nan[NW];
   __shared__ LocateLds s_loc;
   Piece p;
-  if (!locate<W, KS, 64 * NW>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  if (!locate<W, KS, 64 * NW>(a, s_loc, p)) return;  // uniform
+  put_cut<W>(a, p);
   const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = w / W;  // the key tile of a step that the wave attends to
@@ -695,7 +694,7 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   __shared__ uint32_t s_nan[W / 2];
   __shared__ LocateLds s_loc;
   Piece p;
-  if (!locate<W, 1, 64 * W>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
+  if (!locate<W, 1, 64 * W>(a, s_loc, p)) return;  // uniform
   const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = w >> 2, u = w & 3;  // and the block of each tile that the wave converts
@@ -790,6 +789,7 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
   for (int i = 0; i < W / 2; ++i) nan |= s_nan[i] != 0;
   if (__builtin_amdgcn_readfirstlane(nan))
     unit.find_nan(a, table, head_off, s.len, kt0, kt0 + n_kt);
+  put_cut<W>(a, p);
   if (p.splits > 1) unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
   else unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
 }
@@ -801,23 +801,19 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
 // of all are one round trip.  (One slice: a query over 60000 tokens in 235 pieces
 // 62 us.)
 constexpr int kMerge4Threads = 256;
-template <int DT, int D, int W, int KS, int R>
+template <int DT, int D, int W, int R>
 __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(VarlenArgs a) {
   constexpr int SL = 32 / R, NV = D / 32;
-  __shared__ LocateLds s_loc;
   __shared__ f32x4 s_o[SL > 1 ? SL : 1][SL > 1 ? R : 1][SL > 1 ? D / 4 : 1];
   __shared__ float2 s_ml[SL][R];
-  if (*a.any_cut == 0) return;  // uniform
-  Piece p;
-  if (!locate<W, KS, kMerge4Threads, R>(a, (int)blockIdx.x, s_loc, p)) return;  // uniform
-  const SeqWork& s = p.s;
+  const int index = (int)blockIdx.x / a.merge_per_tile;
+  const CutTile c = a.cut[index];
+  if (index >= *a.n_cut) return;  // uniform; before c is looked at
   const int part = threadIdx.x & 7, row = ((int)threadIdx.x >> 3) % R, sl = ((int)threadIdx.x >> 3) / R;
-  const int r = p.tile * R + row, tile = r / (W * kUnitRows);
-  // the tile's pieces follow each other (locate); those past the grid were not run
-  const int piece0 = p.first + (p.head * s.tiles + s.tiles - 1 - tile) * p.splits;
-  const int n = r < s.rows ? min(p.splits, a.n_pieces - piece0) : 0;
+  const int r = c.row0 + ((int)blockIdx.x - index * a.merge_per_tile) * R + row;
+  const int n = r < c.row1 ? c.pieces : 0;
   constexpr int64_t kStep = (int64_t)W * kUnitRows;  // slot rows from piece to piece
-  const int64_t row0 = (int64_t)piece0 * kStep + (r - tile * kStep);
+  const int64_t row0 = (int64_t)c.piece0 * kStep + (r - c.row0);
   float mx = -INFINITY, lt = 0.f;
   f32x4 acc[NV];
 #pragma unroll
@@ -853,10 +849,10 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
       add(s_ml[k][row].x, s_ml[k][row].y, v);
     }
   }
-  if (r >= s.rows) return;
+  if (r >= c.row1) return;
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  const int i = a.by_group.div(r), h = p.head * a.group + r - i * a.group;
-  uint8_t* op = a.out + (int64_t)(s.t0 + i) * a.o_tok_b + ((int64_t)h * D + 4 * part) * 2;
+  const int i = a.by_group.div(r), h = c.head * a.group + r - i * a.group;
+  uint8_t* op = a.out + (int64_t)(c.t0 + i) * a.o_tok_b + ((int64_t)h * D + 4 * part) * 2;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
     *reinterpret_cast<u32x2*>(op + 64 * k) =
@@ -872,9 +868,11 @@ struct VarlenShape {
   int64_t pieces;   // bound of the pieces (the main grid)
   int64_t target;   // pieces wanted (0: uncut)
   int32_t least;    // key steps of a piece at least
+  int64_t cut;      // bound of the row tiles that are cut
   int merge_rows;   // rows of a merge workgroup
-  int64_t merge;    // bound of the merge's workgroups
-  int64_t o_bytes, ml_bytes;
+  int64_t merge_per_tile;  // merge workgroups of a row tile
+  int64_t o_bytes, ml_bytes, cut_bytes;
+  int64_t workspace() const { return o_bytes + ml_bytes + cut_bytes; }
 };
 // More rows of a kv head than this take the ping-pong kernel (28/4 heads, 8 x 64
 // queries over 4000 tokens each, 448 rows: 77 us by four-wave workgroups, 73 by
@@ -915,15 +913,15 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
     s.target = jobs <= slots / 2 ? slots - jobs : slots / 2;
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
-    auto merges = [&](int64_t r) {
-      return n_kv_heads * std::min(batch * ((max_rows + r - 1) / r), total_q * group / r + batch);
-    };
-    s.merge_rows = merges(4) <= 4096 ? 4 : 32;
-    s.merge = merges(s.merge_rows);
-    s.ml_bytes = s.pieces * tile_rows * 8 + 256;  // and whether a sequence is cut
+    s.cut = jobs;
+    auto per_tile = [&](int64_t r) { return (std::min(max_rows, tile_rows) + r - 1) / r; };
+    s.merge_rows = jobs * per_tile(4) <= 4096 ? 4 : 32;
+    s.merge_per_tile = per_tile(s.merge_rows);
+    s.ml_bytes = s.pieces * tile_rows * 8;
+    s.cut_bytes = 256 + s.cut * (int64_t)sizeof(CutTile);
     s.o_bytes = s.pieces * tile_rows * head_dim * 4;
   }
-  if (s.pieces > INT32_MAX / 2 || s.merge > INT32_MAX / 2) return AEGKV_ERR_UNSUPPORTED;
+  if (s.pieces > INT32_MAX / 2 || s.cut * s.merge_per_tile > INT32_MAX / 2) return AEGKV_ERR_UNSUPPORTED;
   *out = s;
   return AEGKV_OK;
 }
@@ -942,11 +940,11 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   return AEGKV_OK;
 }
 
-template <int DT, int D, int W, int KS>
+template <int DT, int D, int W>
 void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
-  const dim3 g((uint32_t)s.merge), t(kMerge4Threads);
-  if (s.merge_rows == 4) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, KS, 4>), g, t, 0, st, a);
-  else hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, KS, 32>), g, t, 0, st, a);
+  const dim3 g((uint32_t)(s.cut * s.merge_per_tile)), t(kMerge4Threads);
+  if (s.merge_rows == 4) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 4>), g, t, 0, st, a);
+  else hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 32>), g, t, 0, st, a);
 }
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
@@ -956,9 +954,9 @@ int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   else hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 1>), g, four, 0, st, a);
   AEGKV_HIP_TRY(hipGetLastError());
   if (s.target > 0) {
-    if (s.long_rows) launch_merge<DT, D, kLongWaves4, 1>(a, s, st);
-    else if (s.key_tiles == 2) launch_merge<DT, D, kShortWaves4 / 2, 2>(a, s, st);
-    else launch_merge<DT, D, kShortWaves4, 1>(a, s, st);
+    if (s.long_rows) launch_merge<DT, D, kLongWaves4>(a, s, st);
+    else if (s.key_tiles == 2) launch_merge<DT, D, kShortWaves4 / 2>(a, s, st);
+    else launch_merge<DT, D, kShortWaves4>(a, s, st);
     AEGKV_HIP_TRY(hipGetLastError());
   }
   return AEGKV_OK;
@@ -982,7 +980,7 @@ int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q
   VarlenShape s;
   rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
   if (rc) return rc > 0 ? AEGKV_ERR_RUNTIME : rc;
-  return s.o_bytes + s.ml_bytes;
+  return s.workspace();
 }
 
 int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* q,
@@ -1011,7 +1009,7 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
   VarlenShape s;
   rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
   if (rc) return rc;
-  if (s.target > 0 && (!workspace || workspace_bytes < (uint64_t)(s.o_bytes + s.ml_bytes)))
+  if (s.target > 0 && (!workspace || workspace_bytes < (uint64_t)s.workspace()))
     return AEGKV_ERR_WORKSPACE;
   if (s.target > 0 && !aligned16(workspace)) return AEGKV_ERR_MISALIGNED;
   VarlenArgs a;
@@ -1039,10 +1037,13 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
   a.target = s.target;
   a.least = s.least;
   a.n_pieces = (int32_t)s.pieces;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.o_bytes);
-  a.any_cut = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + s.o_bytes +
-                                          s.ml_bytes - 256);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + s.o_bytes);
+  a.n_cut = reinterpret_cast<int32_t*>(ws + s.o_bytes + s.ml_bytes);
+  a.cut = reinterpret_cast<CutTile*>(ws + s.o_bytes + s.ml_bytes + 256);
+  a.max_cut = (int32_t)s.cut;
+  a.merge_per_tile = (int32_t)s.merge_per_tile;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == AEGKV_DTYPE_BF16)
     return head_dim == 64 ? launch_varlen<AEGKV_DTYPE_BF16, 64>(a, s, st)
