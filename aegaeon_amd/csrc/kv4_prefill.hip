@@ -402,9 +402,8 @@ struct RowUnit : WaveSoftmax<DT, D> {
       for (int e = 0; e < 4; ++e) qv[ks][e] = sign < 0 ? qv[ks][e] ^ 0x80008000u : 0u;
   }
 
-  // ORDERED: LDS reads stay two MFMAs ahead of their use (pv: four), as the long
-  // prompts' kernel orders them
-  template <bool ORDERED>
+  // LDS reads stay two MFMAs ahead of their use (pv: four), as the long prompts'
+  // kernel orders them
   __device__ __forceinline__ void qk(const uint8_t* lds, f32x16 (&s)[2]) const {
     const int lane = threadIdx.x & 63, col = lane & 31, hh = lane >> 5;
     const uint8_t* kp = lds + col * 2 * D;
@@ -419,15 +418,13 @@ struct RowUnit : WaveSoftmax<DT, D> {
       for (int sb = 0; sb < 2; ++sb)
         s[sb] = PfOps<DT>::mfma(
             *reinterpret_cast<const u32x4*>(kp + (kx ^ (32 * ks)) + 32 * sb * 2 * D), qv[ks], s[sb]);
-    if (ORDERED) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
 #pragma unroll
-      for (int i = 0; i < 2 * KS - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // the next read
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    for (int i = 0; i < 2 * KS - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // the next read
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
   }
   // -inf for keys past a row's last one and for unreadable blocks (bit u)
   __device__ __forceinline__ void mask(f32x16 (&s)[2], int k0, uint32_t unreadable) const {
@@ -445,7 +442,6 @@ struct RowUnit : WaveSoftmax<DT, D> {
       }
     }
   }
-  template <bool ORDERED>
   __device__ __forceinline__ void pv(const uint8_t* lds, const u32x4 (&pb)[4]) {
     constexpr int RB = 2 * D;
     const int lane = threadIdx.x & 63, G = lane >> 4, x = lane & 15;
@@ -463,15 +459,13 @@ struct RowUnit : WaveSoftmax<DT, D> {
             u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(y + 8 * RB)));
         o[db] = PfOps<DT>::mfma(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[kk], o[db]);
       }
-    if (ORDERED) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-      for (int i = 0; i < 4 * DB - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    for (int i = 0; i < 4 * DB - 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
   }
   // Key tiles [kt0, kt1) hold V groups of NaN (rare): the rows that see one's
   // token get NaN in its dims when they are stored.  Visible keys are a prefix, so
@@ -642,11 +636,11 @@ __global__ __launch_bounds__(64 * kShortWaves4, 2) void kv4_varlen_kernel(Varlen
       if constexpr (decltype(with_rows)::value) {
         f32x16 sc[2];
         u32x4 pb[4];
-        unit.template qk<false>(mine, sc);
+        unit.qk(mine, sc);
         unit.mask(sc, (kt * KS + part) * kPfKTile, unreadable);
         unit.softmax(sc, pb, a.scale_log2, kt == kt0);
         __builtin_amdgcn_sched_barrier(0);  // V's reads stay behind the softmax: registers
-        unit.template pv<false>(mine + T_BYTES, pb);
+        unit.pv(mine + T_BYTES, pb);
       }
       KV4_BARRIER();  // every wave's reads of the tiles
     };
@@ -736,13 +730,13 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
     bad[1] = bad[2];
     load(r, j + 2);
   };
-  auto qk = [&](int j, f32x16 (&sc)[2]) { unit.template qk<true>(lds + (j & 1) * T_BYTES, sc); };
+  auto qk = [&](int j, f32x16 (&sc)[2]) { unit.qk(lds + (j & 1) * T_BYTES, sc); };
   auto softmax = [&](int j, f32x16 (&sc)[2], u32x4 (&pb)[4], uint32_t bad) {
     unit.mask(sc, (kt0 + j) * kPfKTile, bad);
     unit.softmax(sc, pb, a.scale_log2, j == 0);
   };
   auto pv = [&](int j, const u32x4 (&pb)[4]) {
-    unit.template pv<true>(lds + (2 + (j & 1)) * T_BYTES, pb);
+    unit.pv(lds + (2 + (j & 1)) * T_BYTES, pb);
   };
 
   u32x4 pb[4];
