@@ -9,6 +9,7 @@
 
 #include "aegkv_internal.h"
 #include "kv4_format.h"
+#include "wave_scan.h"
 
 namespace aegkv {
 namespace {
@@ -82,10 +83,9 @@ __global__ __launch_bounds__(kAppend4Threads) void kv4_append_kernel(Append4Args
   if ((c & 3) == 0) rec[kv4_code_bytes(D) + (c >> 2) * kKv4Tokens + r] = (uint8_t)e;
 }
 
-// De-page: a tile is one pass of one block of one sequence and layer, 1024
-// chunks of 8 dims of the block's [K/V][head][token] rows.  Each workgroup
-// scans the batch's block counts into LDS and walks the flattened tiles
-// round-robin; the next tile's block id and output row are fetched while the
+// De-page: a tile is one pass of one block of one sequence, 1024 chunks of 8
+// dims of the block's [K/V][head][token] rows.  Each workgroup scans the batch's
+// block counts into LDS and walks its layer's tiles round-robin; the next tile's block id and output row are fetched while the
 // current one's loads are in flight.
 constexpr int kGather4Threads = 256;
 constexpr int kGather4MaxBatch = 1024;    // sequences per launch (LDS scan)
@@ -106,7 +106,6 @@ struct Gather4Args {
   int64_t out_layer_b;
   int32_t max_seq_len;
   int32_t batch;        // <= kGather4MaxBatch
-  int32_t n_layers;
   int32_t n_heads;
   int32_t passes;       // of a block
 };
@@ -129,12 +128,7 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
     cnt[k] = (len + kKv4Tokens - 1) / kKv4Tokens;
     run += cnt[k];
   }
-  int incl = run;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(incl, off);
-    if ((t & 63) >= off) incl += y;
-  }
+  const int incl = wave_prefix(run);
   if ((t & 63) == 63) wsum[t >> 6] = incl;
   __syncthreads();
   int excl = incl - run;
@@ -147,16 +141,13 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
   }
   if (t == kGather4Threads - 1) pre[B] = excl;  // total (B may equal the capacity)
   __syncthreads();
-  const int64_t per_layer = (int64_t)pre[B] * a.passes;
-  const int64_t total = per_layer * a.n_layers;
-  int64_t g = blockIdx.x;
+  const uint32_t total = (uint32_t)pre[B] * a.passes;
+  uint32_t g = blockIdx.x;
   if (g >= total) return;  // uniform
 
-  auto locate = [&](int64_t gg, int& layer, int& b, int& j, int& ps) {
-    layer = (int)(gg / per_layer);
-    int r = (int)(gg - layer * per_layer);
-    ps = r % a.passes;
-    r /= a.passes;
+  auto locate = [&](uint32_t gg, int& b, int& j, int& ps) {
+    const int r = (int)(gg / (uint32_t)a.passes);
+    ps = (int)(gg - (uint32_t)r * a.passes);
     int lo = 0, hi = B - 1;  // the last sequence whose first block is <= r
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -167,10 +158,10 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
     j = r - pre[lo];
   };
   constexpr int CPR = D / 8;                    // chunks per head's row
-  const int chunks = 2 * a.n_heads * kKv4Tokens * CPR;
   const int64_t row_b = (int64_t)a.n_heads * D * 2;
-  int layer, b, j, ps;
-  locate(g, layer, b, j, ps);
+  const int layer = (int)blockIdx.y;
+  int b, j, ps;
+  locate(g, b, j, ps);
   int32_t id = a.block_tables[(int64_t)b * a.max_blocks + j];
   int64_t row0 = a.cu_seqlens[b];
   while (true) {
@@ -179,16 +170,20 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
     if (row < 0 || row >= a.out_tokens || id < 0 || id >= a.n_blocks) n_tok = 0;
     else n_tok = (int)min((int64_t)n_tok, a.out_tokens - row);
     const uint8_t* blk = a.cache + (int64_t)max(id, 0) * a.blk_b + layer * a.layer_b;
+    // 2^32 / n_tok rounded up: rows below 2^28 divide exactly
+    const uint32_t magic = n_tok > 1 ? 0xffffffffu / (uint32_t)n_tok + 1 : 0;
+    const uint32_t n_rows = 2u * a.n_heads * n_tok;
     uint32_t codes[kGather4PerThread], sb[kGather4PerThread];
     uint8_t* dst[kGather4PerThread];
 #pragma unroll
     for (int k = 0; k < kGather4PerThread; ++k) {
       const int ch = (ps * kGather4PerThread + k) * kGather4Threads + t;
-      const int c = ch % CPR, r = ch / CPR % kKv4Tokens, side = ch / (CPR * kKv4Tokens);
-      const int kv = side / a.n_heads, head = side - kv * a.n_heads;
+      const uint32_t c = ch % CPR, row_at = ch / CPR;
+      const int side = n_tok > 1 ? __umulhi(row_at, magic) : row_at, r = row_at - side * n_tok;
+      const int kv = side >= a.n_heads, head = side - kv * a.n_heads;
       dst[k] = nullptr;
       codes[k] = sb[k] = 0;
-      if (ch < chunks && r < n_tok) {
+      if (row_at < n_rows) {
         const uint8_t* rec = blk + (int64_t)(head * 2 + kv) * kv4_record_bytes(D);
         if (kv && D == 64) {
           const uint8_t* p = rec + kv4_v_byte<D>(r, c);
@@ -203,10 +198,10 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
                  ((int64_t)head * D + 8 * c) * 2;
       }
     }
-    const int64_t gn = g + gridDim.x;
+    const uint32_t gn = g + gridDim.x;
     const bool more = gn < total;
-    int nlayer, nb, nj, nps;
-    locate(more ? gn : g, nlayer, nb, nj, nps);
+    int nb, nj, nps;
+    locate(more ? gn : g, nb, nj, nps);
     const int32_t nid = a.block_tables[(int64_t)nb * a.max_blocks + nj];
     const int64_t nrow0 = a.cu_seqlens[nb];
 #pragma unroll
@@ -218,7 +213,6 @@ __global__ __launch_bounds__(kGather4Threads) void kv4_gather_kernel(Gather4Args
     }
     if (!more) break;
     g = gn;
-    layer = nlayer;
     b = nb;
     j = nj;
     ps = nps;
@@ -238,8 +232,8 @@ void launch_append(const Append4Args& a, int32_t head_dim, uint32_t grid, hipStr
   else hipLaunchKernelGGL((kv4_append_kernel<DT, 256>), g, t, 0, st, a);
 }
 template <int DT>
-void launch_gather(const Gather4Args& a, int32_t head_dim, uint32_t grid, hipStream_t st) {
-  const dim3 g(grid), t(kGather4Threads);
+void launch_gather(const Gather4Args& a, int32_t head_dim, dim3 g, hipStream_t st) {
+  const dim3 t(kGather4Threads);
   if (head_dim == 64) hipLaunchKernelGGL((kv4_gather_kernel<DT, 64>), g, t, 0, st, a);
   else if (head_dim == 128) hipLaunchKernelGGL((kv4_gather_kernel<DT, 128>), g, t, 0, st, a);
   else hipLaunchKernelGGL((kv4_gather_kernel<DT, 256>), g, t, 0, st, a);
@@ -322,7 +316,7 @@ int aegkv_kv4_gather_tokens(const void* cache, int64_t cache_block_stride,
   const int64_t chunks = 2 * (int64_t)n_kv_heads * kKv4Tokens * (head_dim / 8);
   const int64_t per_tile = kGather4Threads * kGather4PerThread;
   const int64_t passes = (chunks + per_tile - 1) / per_tile;
-  if (chunks > INT32_MAX - per_tile || blocks_needed * kGather4MaxBatch * passes > INT32_MAX)
+  if (n_layers > 65535 || chunks > INT32_MAX - per_tile || blocks_needed * kGather4MaxBatch * passes > INT32_MAX)
     return AEGKV_ERR_UNSUPPORTED;
   DeviceState* ds = nullptr;
   int rc = current_device_state(&ds);
@@ -338,18 +332,18 @@ int aegkv_kv4_gather_tokens(const void* cache, int64_t cache_block_stride,
   a.out_tokens = out_tokens;
   a.out_layer_b = out_layer_stride * 2;
   a.max_seq_len = max_seq_len;
-  a.n_layers = n_layers;
   a.n_heads = n_kv_heads;
   a.passes = (int32_t)passes;
-  const int64_t max_grid = (int64_t)std::max(ds->num_cu, 1) * kGather4WorkgroupsPerCu;
+  const int64_t max_grid = std::max<int64_t>(
+      1, ((int64_t)std::max(ds->num_cu, 1) * kGather4WorkgroupsPerCu + n_layers - 1) / n_layers);
   for (int32_t b0 = 0; b0 < batch; b0 += kGather4MaxBatch) {
     const int32_t nb = std::min(kGather4MaxBatch, batch - b0);
     a.batch = nb;
     a.block_tables = block_tables + (int64_t)b0 * max_blocks;
     a.seq_lens = seq_lens + b0;
     a.cu_seqlens = cu_seqlens + b0;
-    const int64_t tiles_max = blocks_needed * nb * n_layers * passes;  // bound of the tiles
-    const uint32_t grid = (uint32_t)std::max<int64_t>(1, std::min(tiles_max, max_grid));
+    const int64_t tiles_max = blocks_needed * nb * passes;  // bound of a layer's tiles
+    const dim3 grid((uint32_t)std::min(tiles_max, max_grid), (uint32_t)n_layers);
     if (dtype == AEGKV_DTYPE_BF16) launch_gather<AEGKV_DTYPE_BF16>(a, head_dim, grid, (hipStream_t)stream);
     else launch_gather<AEGKV_DTYPE_FP16>(a, head_dim, grid, (hipStream_t)stream);
     AEGKV_HIP_TRY(hipGetLastError());

@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "../../include/aegkv.h"
+#include "wave_scan.h"
 
 namespace aegkv {
 namespace {
@@ -19,17 +20,6 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-// Sum over the wave's lanes up to and with this one.
-__device__ __forceinline__ int wave_prefix(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);  // row_shr 2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);  // row_shr 4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);  // row_shr 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true);  // row_bcast 15, rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true);  // row_bcast 31, rows 2 and 3
-  return x;
-}
 
 constexpr int kPfKTile = 64;                 // keys per step
 constexpr float kPfRescaleSlack = 8.f;
