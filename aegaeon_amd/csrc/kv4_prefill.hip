@@ -196,12 +196,13 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, LocateLds& x, Piece&
   p.s.len = f[8];
   p.s.rows = f[9];
   p.s.tiles = f[10];
-  // kv heads slowest, then row tiles from the last (the most keys) to the first
+  // row tiles from the last (the most keys) to the first, kv heads within
   const int q = f[1] / p.splits;
   p.split = f[1] - q * p.splits;
   p.cut = f[4] + q;
-  p.head = q / p.s.tiles;
-  p.tile = p.s.tiles - 1 - (q - p.head * p.s.tiles);
+  p.tile = q / a.n_kv_heads;
+  p.head = q - p.tile * a.n_kv_heads;
+  p.tile = p.s.tiles - 1 - p.tile;
   return true;
 }
 // A cut row tile's entry for the merge, by one thread of its first piece.
