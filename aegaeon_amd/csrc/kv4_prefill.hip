@@ -990,7 +990,8 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
   int rc = varlen_check(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
                         dtype);
   if (rc) return rc;
-  if (max_blocks < 0 || n_blocks < 0 || !std::isfinite(scale)) return AEGKV_ERR_INVALID_ARG;
+  if (max_blocks < 0 || n_blocks < 0 || !std::isfinite(scale * 1.4426950408889634f))
+    return AEGKV_ERR_INVALID_ARG;
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return AEGKV_OK;
   if (!out || !q || !cache || !block_tables || !cu_seqlens_q || !seq_lens || n_blocks == 0)
     return AEGKV_ERR_INVALID_ARG;

@@ -472,10 +472,11 @@ int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, cons
  * + 1], not decreasing: the grid counts on sequences that share no tokens), the
  * last m of its seq_lens[b] = n cached tokens.  Query i attends to keys
  * j <= n - m + i (every j < n when causal is 0), softmax(scale * q.k) in fp32
- * with P rounded to 16 bits before P.V (any finite scale); without such a key
- * it gives zeros.  Queries past max_seqlen_q of a sequence are left alone; keys
- * past max_seq_len are not attended; tokens are clamped to [0, total_q).  A
- * block id outside [0, n_blocks) is never dereferenced: its tokens are masked.
+ * with P rounded to 16 bits before P.V (any scale that stays finite times
+ * log2 e); without such a key it gives zeros.  Queries past max_seqlen_q of a
+ * sequence are left alone; keys past max_seq_len are not attended; tokens are
+ * clamped to [0, total_q).  A block id outside [0, n_blocks) is never
+ * dereferenced: its tokens are masked.
  * An infinity or NaN that was appended shows in the rows that attend to its
  * token, and in no others.
  *   workspace: DEVICE scratch of aegkv_kv4_varlen_attention_workspace_size(...)

@@ -7,6 +7,7 @@ are test_gpu_prefill.py's: the relative L2 error of the float64 result rounded t
 the output type plus 1e-3 (bf16) / 1.5e-4 (fp16) for P's rounding, and per
 element 2^-7 / 2^-9 of the output's largest magnitude."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -104,6 +105,42 @@ def test_lengths(device, new, lens, Hq, Hkv, D):
     caches (cut over workgroups), long ones."""
     b = Batch(device, new, lens, Hq, Hkv, D, "bf16", len(new) + sum(lens))
     b.check(b.run(0.1), 0.1)
+
+
+@pytest.mark.parametrize("new,lens,Hq,Hkv,D", [
+    ([1200], [2500], 14, 2, 128),                      # eight-wave workgroups
+    ([200] * 9, [1000] * 9, 8, 8, 64),                 # four waves, one key tile per step
+    ([64] * 40, [5000] + [100] * 39, 8, 8, 64)])       # two, one sequence cut of many
+def test_cut_sequences_of_many_rows(device, new, lens, Hq, Hkv, D):
+    b = Batch(device, new, lens, Hq, Hkv, D, "bf16", sum(lens))
+    b.check(b.run(0.1), 0.1)
+
+
+@pytest.mark.parametrize("first", [1, 100, 300])
+def test_more_sequences_than_threads(device, first):
+    new = [first] + [1, 0, 2] * 400
+    b = Batch(device, new, [2000] + [3, 40, 17] * 400, 2, 1, 64, "bf16", first)
+    b.check(b.run(0.1), 0.1)
+
+
+def test_threads_share_a_stream(device):
+    sets = [Batch(device, [5, 40], [3000, 700], 28, 4, 128, "bf16", 11),
+            Batch(device, [300], [2500], 14, 2, 128, "bf16", 12)]
+    want = [b.run(0.1) for b in sets]
+    got = [[], []]
+
+    def calls(i):
+        for _ in range(20):
+            got[i].append(sets[i].run(0.1))
+
+    threads = [threading.Thread(target=calls, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, w in zip(got, want):
+        assert len(outs) == 20
+        assert all(torch.equal(o.view(torch.int16), w.view(torch.int16)) for o in outs)
 
 
 def test_one_query_is_the_decode_attention(device):

@@ -232,6 +232,7 @@ def test_varlen_host_checks(lib):
     assert call(hkv=5) == INVALID                  # Hq not a multiple of Hkv
     assert call(d=256) == UNSUP and call(d=32) == UNSUP and call(dt=7) == UNSUP
     assert call(scale=float("nan")) == INVALID and call(scale=float("inf")) == INVALID
+    assert call(scale=3e38) == INVALID             # infinite times log2 e
     assert call(batch=-1) == INVALID and call(longest=-1) == INVALID and call(max_q=-1) == INVALID
     assert call(batch=0, q=None) == OK and call(total=0) == OK and call(max_q=0) == OK
     assert call(q=None) == INVALID and call(cache=None) == INVALID and call(tables=None) == INVALID
