@@ -102,9 +102,8 @@ __device__ __forceinline__ int cost_units(int len) {
 // wave per SIMD.
 template <int D>
 constexpr int pipeline_depth() { return D >= 256 ? 2 : 3; }
-// Steps of the 4-bit cache in registers.
-template <int D>
-constexpr int kv4_pipeline_depth() { return 2; }
+// Steps of the 4-bit cache in registers (of four blocks at D = 128: 17 KB a wave).
+constexpr int kKv4PipelineDepth = 2;
 
 // kv heads of a workgroup's group, one per wave; the 4 / heads waves of each
 // head take ranges of their own.  Four, unless that leaves one wave in 20 or
@@ -517,6 +516,12 @@ __device__ __forceinline__ void compute_block(KVRegs<D>& r, const u32x4* qv, f32
 }
 
 // ---- the 4-bit cache (kv4_format.h) ----
+// Bound by the cache's bytes, 17 D / 16 per token and kv head, as long as the
+// instructions per block stay under their loads: one layer of 128 sequences of
+// 1500 tokens on average (28/4 heads, D = 128, 105 MB) 33.1 us, 29.8 when the
+// loads alone are issued; 32 x 2048 of 40/40 heads (357 MB) 63.2 us, 5.7 TB/s, and
+// 63.  One workgroup per CU, two steps ahead: two per CU take 36.4 and 65.7 us,
+// three steps in registers are slower as well.
 // K and V are converted to 16 bits, where code times scale is exact, so nothing
 // past the conversion differs from the 16-bit cache's arithmetic.  Per block of
 // 16 tokens, with lane l = 16 g + j:
@@ -2058,7 +2063,7 @@ int launch_combine(const AttnArgs& a, hipStream_t stream) {
 
 template <int DT, int D, bool PLANNED, bool FUSED, int PACK = 0>
 void launch_main(const AttnArgs& a, size_t lds, hipStream_t stream) {
-  constexpr int NBUF = PACK > 0 ? kv4_pipeline_depth<D>() : pipeline_depth<D>();
+  constexpr int NBUF = PACK > 0 ? kKv4PipelineDepth : pipeline_depth<D>();
   hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, PACK>),
                      dim3(a.n_wg), dim3(64 * kWaves), lds, stream, a);
 }

@@ -7,20 +7,36 @@
 // Rows.  The m queries of a sequence times the G query heads of one kv head
 // are rows r = i * G + (head in the group) that share that head's K and V.  32
 // consecutive rows are a wave's unit, W units a workgroup's tile.  A tile's
-// workgroup walks the sequence's keys 64 at a time: a wave loads one 16-token
-// block's codes into registers a tile ahead, converts them to 16 bits and
-// stores them to LDS, and every wave takes S = K.Q^T, the online softmax and
-// O += V^T.P^T of its rows from there (prefill_wave.h, 32x32x16 MFMA; P rounded
-// to 16 bits as in the prompt attention).  The conversion is shared by the
-// tile's W waves.
+// workgroup walks the sequence's keys 64 at a time: a wave holds one 16-token
+// block's codes in registers ahead of its tile, converts them to 16 bits, where
+// they are exact, and stores them to LDS; every wave takes S = K.Q^T, the online
+// softmax and O += V^T.P^T of its rows from there (prefill_wave.h, 32x32x16
+// MFMA, fp32 sums; P rounded to 16 bits as in the prompt attention: its error is
+// below the output's own).  The conversion, 190 instructions per 128 keys and
+// wave, is shared by the tile's units, so few rows pay for it most.  By the rows
+// of a sequence (varlen_shape):
+//   up to 64      four waves, two units; two key tiles per step, one per pair of
+//                 waves, joined at the end;
+//   up to 256     four waves, four units, two workgroups per CU;
+//   more          eight waves in ping-pong, one workgroup per CU.
 //
 // Pieces.  When the batch has too few tiles to fill the chip, a tile's keys are
 // cut into pieces of a workgroup each, which write fp32 partials (O, running
 // maximum in log2 units, sum) that a second kernel merges.  The cut is the same
-// for a sequence's tiles: `splits` ranges of ceil(n_kt / splits) key tiles,
+// for a sequence's tiles: `splits` ranges of ceil(n_kt / splits) key steps,
 // splits = ceil(n_kt / C), with one C for the batch that every workgroup
-// computes for itself: the batch's key tiles times row tiles divided by the
+// computes for itself: the batch's key steps times row tiles divided by the
 // pieces wanted.
+//
+// Bounds and measured.  Per cached token and kv head 17 D / 16 bytes are read
+// and 4 D G flops done per query, so past some 10 queries at G = 7 the products
+// bound it: 2048 queries over 16001 tokens (28/4 heads, D = 128) 467 us, 940
+// TFLOP/s (224 of 256 CUs hold a tile, at 87% of the rate of a large matrix
+// product each); 4 x 512 over 3800 tokens each 142 us, the longest sequence's;
+// two whole prompts of 2048 85 us.  Few queries are bound by the latency of
+// their steps, 1.7 us each of a lone workgroup (conversion, products and softmax
+// of a wave follow each other): 48 x 5 over 1000 tokens each (32/4) 28.5 us,
+// of which the merge 4.6.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
