@@ -122,6 +122,24 @@ def test_append_then_rows_is_the_identity_on_stored_values():
     assert np.array_equal(cache[2], before[2])
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_textbook_attention_is_torchs_in_64_bits(causal):
+    rng = np.random.default_rng(1)
+    k, v = rng.standard_normal((2, 6, 16, 2, 64))
+    tables, new, lens = [[3, 1, 0], [5], [4, 2]], [7, 3, 32], [40, 3, 32]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    q = rng.standard_normal((cu[-1], 6, 64))
+    got = k4.varlen_attention(q, k, v, tables, cu, lens, 0.2, causal)
+    for b, (m, n) in enumerate(zip(new, lens)):
+        mine = slice(cu[b], cu[b + 1])
+        rows = [torch.from_numpy(x[tables[b]].reshape(-1, 2, 64)[:n]).transpose(0, 1)
+                .repeat_interleave(3, 0) for x in (k, v)]
+        seen = torch.ones(m, n, dtype=torch.bool).tril(n - m) if causal else None
+        want = torch.nn.functional.scaled_dot_product_attention(
+            torch.from_numpy(q[mine]).transpose(0, 1), *rows, attn_mask=seen, scale=0.2)
+        assert np.allclose(got[mine], want.transpose(0, 1).numpy(), rtol=1e-12, atol=1e-12)
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
