@@ -373,8 +373,8 @@ struct TileIds {
 
 // A wave's unit of 32 rows.
 template <int DT, int D>
-struct RowUnit : WaveSoftmax<DT, D> {
-  using Base = WaveSoftmax<DT, D>;
+struct RowUnit : WaveSoftmax<DT, D, true> {
+  using Base = WaveSoftmax<DT, D, true>;
   using Base::DB;
   using Base::KS;
   using Base::lsum;

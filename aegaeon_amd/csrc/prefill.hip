@@ -117,13 +117,13 @@ struct PrefillArgs {
 // query q0 + col and, of the O^T accumulators, head dims 32 db + 8 g + 4 hh ..
 // + 3 in element 4 g .. 4 g + 3 of o[db].
 template <int DT, int D>
-struct WaveState : WaveSoftmax<DT, D> {
-  using WaveSoftmax<DT, D>::KS;
-  using WaveSoftmax<DT, D>::DB;
-  using WaveSoftmax<DT, D>::qv;
-  using WaveSoftmax<DT, D>::o;
-  using WaveSoftmax<DT, D>::m;
-  using WaveSoftmax<DT, D>::lsum;
+struct WaveState : WaveSoftmax<DT, D, false> {
+  using WaveSoftmax<DT, D, false>::KS;
+  using WaveSoftmax<DT, D, false>::DB;
+  using WaveSoftmax<DT, D, false>::qv;
+  using WaveSoftmax<DT, D, false>::o;
+  using WaveSoftmax<DT, D, false>::m;
+  using WaveSoftmax<DT, D, false>::lsum;
 
   __device__ __forceinline__ void init(const PrefillArgs& a, int h, int64_t s0, int len, int qi,
                                        int hh) {

@@ -84,8 +84,9 @@ inline FastDiv fast_div(int32_t d) {  // 1 <= d < 2^31
 // softmax.  Lane (col = l & 31, hh = l / 32) belongs to row col; it holds of
 // S^T's 32-key block sb the keys 32 sb + 8 (i / 4) + 4 hh + i % 4 (element i),
 // and of O^T head dims 32 db + 8 g + 4 hh .. + 3 in element 4 g .. 4 g + 3 of
-// o[db].
-template <int DT, int D>
+// o[db].  KEYLESS: a row may have seen no key beside one that has (in a prompt each
+// row sees its first tile's first).
+template <int DT, int D, bool KEYLESS>
 struct WaveSoftmax {
   static constexpr int KS = D / 16;  // k-steps of K.Q^T
   static constexpr int DB = D / 32;  // 32-row blocks of O^T
@@ -127,9 +128,8 @@ struct WaveSoftmax {
       m = fmaxf(m, bm);
     } else if (__builtin_amdgcn_ballot_w64(bm > m + kPfRescaleSlack)) {
       const float mn = fmaxf(m, bm);
-      // 0 while m = -inf; a query that has seen no key yet, beside one that
-      // has: 0 as well, of sums that are 0
-      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      // 0 while m = -inf (a row without a key: of sums that are 0)
+      const float alpha = __builtin_amdgcn_exp2f(m - (KEYLESS && mn == -INFINITY ? 0.f : mn));
       lsum *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
