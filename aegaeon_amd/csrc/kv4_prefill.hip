@@ -913,15 +913,17 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   s.pieces = jobs;
   s.least = s.long_rows ? kLeastLong : kLeastShort;
   // Workgroups that run at once.  With half as many row tiles or fewer, their keys
-  // are cut into at most as many pieces (8 x 64 queries over 4000, 64 tiles: 74 us,
-  // whole 169, and in one piece per place and one per tile, which need a second
-  // round, 100); with more only sequences of twice the average work of a place, as
+  // are cut into about as many pieces, of long rows at most as many (8 x 64 queries
+  // over 4000, 64 tiles: 67 us, whole 169, and in one piece per place and one per
+  // tile, which need a second round, 100; of short rows two share a CU and ends are
+  // uneven anyway: 48 x 5 over 1000, 192 tiles: 26.9, at most as many 28.4).  With
+  // more tiles only sequences of twice the average work of a place are cut, as
   // partials cost more than an uneven last round (2048 queries over 16001 tokens,
-  // 224 tiles: whole 460 us, cut in two 498; 4 x 512 over 3800 each: 140 and 155).
+  // 224 tiles: whole 460 us, cut in two 498; 4 x 512 over 3800 each: 141 and 155).
   // Four times as many tiles even out by themselves.
   const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (s.long_rows ? 1 : 2);
   if (jobs < 4 * slots && max_kt > s.least) {
-    s.target = jobs <= slots / 2 ? slots - jobs : slots / 2;
+    s.target = jobs > slots / 2 ? slots / 2 : s.long_rows ? slots - jobs : slots;
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     s.cut = jobs;
