@@ -810,7 +810,7 @@ __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(Varle
 // Eight threads take a row's columns, and 32 / R slices of them the pieces in
 // turn, which meet in LDS: with few rows each slice has few pieces and the loads
 // of all are one round trip.  (One slice: a query over 60000 tokens in 235 pieces
-// 62 us.)
+// 62 us; 32 slices cost 10 us more than 8, by the 32 steps in which they meet.)
 constexpr int kMerge4Threads = 256;
 template <int DT, int D, int W, int R>
 __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(VarlenArgs a) {
@@ -928,7 +928,10 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     s.cut = jobs;
     auto per_tile = [&](int64_t r) { return (std::min(max_rows, tile_rows) + r - 1) / r; };
-    s.merge_rows = jobs * per_tile(4) <= 4096 ? 4 : 32;
+    // Rows of a merge workgroup: 4 where a tile has many pieces (a query over 60000,
+    // 128 pieces: 27.3 us, of 16 rows 41.3), 16 where it has few (4 x 128 over 3000:
+    // 53.9, of 4 rows 57.4), 32 where there are many tiles, most of them uncut.
+    s.merge_rows = s.target >= 16 * jobs ? 4 : jobs * per_tile(16) <= 4096 ? 16 : 32;
     s.merge_per_tile = per_tile(s.merge_rows);
     s.ml_bytes = s.pieces * tile_rows * 8;
     s.cut_bytes = 256 + s.cut * (int64_t)sizeof(CutTile);
@@ -957,6 +960,7 @@ template <int DT, int D, int W>
 void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   const dim3 g((uint32_t)(s.cut * s.merge_per_tile)), t(kMerge4Threads);
   if (s.merge_rows == 4) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 4>), g, t, 0, st, a);
+  else if (s.merge_rows == 16) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 16>), g, t, 0, st, a);
   else hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 32>), g, t, 0, st, a);
 }
 template <int DT, int D>

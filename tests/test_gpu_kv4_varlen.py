@@ -110,7 +110,9 @@ def test_lengths(device, new, lens, Hq, Hkv, D):
 @pytest.mark.parametrize("new,lens,Hq,Hkv,D", [
     ([1200], [2500], 14, 2, 128),                      # eight-wave workgroups
     ([200] * 9, [1000] * 9, 8, 8, 64),                 # four waves, one key tile per step
-    ([64] * 40, [5000] + [100] * 39, 8, 8, 64)])       # two, one sequence cut of many
+    ([64] * 40, [5000] + [100] * 39, 8, 8, 64),        # two, one sequence cut of many
+    ([64] * 140, [70] * 139 + [5000], 8, 8, 64),       # of very many
+    ([300] * 140, [6000] + [300] * 139, 2, 2, 64)])
 def test_cut_sequences_of_many_rows(device, new, lens, Hq, Hkv, D):
     b = Batch(device, new, lens, Hq, Hkv, D, "bf16", sum(lens))
     b.check(b.run(0.1), 0.1)
