@@ -49,13 +49,13 @@ def kv4_cache(n_blocks: int, n_layers: int, n_kv_heads: int, head_dim: int,
 def _check_cache(c: torch.Tensor, layers: bool, head_dim: int) -> None:
     """A cache ``[N, L, Hkv, 2, R]`` (one layer: ``[N, Hkv, 2, R]``) whose
     heads are dense; the block and layer strides are free."""
+    shape, strides, r = c.shape, c.stride(), kv4_record_bytes(head_dim)
     names = "[N, L, Hkv, 2, R]" if layers else "[N, Hkv, 2, R]"
-    if c.dim() != (5 if layers else 4) or not c.is_cuda or c.dtype != torch.uint8:
+    if len(shape) != (5 if layers else 4) or not c.is_cuda or c.dtype != torch.uint8:
         raise ValueError(f"kv_cache must be a uint8 GPU tensor {names}")
-    r = kv4_record_bytes(head_dim)
-    if c.size(-1) != r or c.size(-2) != 2:
+    if shape[-1] != r or shape[-2] != 2:
         raise ValueError(f"kv_cache must be {names} with R = {r} bytes for head_dim {head_dim}")
-    if c.stride(-1) != 1 or c.stride(-2) != r or c.stride(-3) != 2 * r:
+    if strides[-1] != 1 or strides[-2] != r or strides[-3] != 2 * r:
         raise ValueError("kv_cache: each block must hold its heads' records densely")
 
 
@@ -196,40 +196,42 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
     either cache) and ``workspace`` (:func:`attention.attention_workspace`) are
     that function's; a sequence without tokens gives zeros.  New rows are
     appended by a call of their own, before this one."""
-    if plan is not None:
-        if plan.buffer.device != q.device:
-            raise ValueError(f"the plan lives on {plan.buffer.device}, the call on {q.device}")
+    shape, q_strides, dev = q.shape, q.stride(), q.device
+    if len(shape) != 3 or q_strides[2] != 1 or q_strides[1] != shape[2] or not q.is_cuda:
+        raise ValueError("q must be a GPU tensor [B, Hq, D] with dense heads")
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None:
+        raise ValueError("q must be bf16 or fp16")
+    B, Hq, D = shape
+    _check_cache(kv_cache, False, D)
+    N, Hkv = kv_cache.shape[:2]
+    if kv_cache.device != dev:
+        raise ValueError(f"kv_cache must be a GPU tensor on {dev} (got {kv_cache.device})")
+    if plan is not None:  # whose tables and lengths were checked when it was built
+        if plan.buffer.device != dev:
+            raise ValueError(f"the plan lives on {plan.buffer.device}, the call on {dev}")
         for given, held, name in ((block_tables, plan.block_tables, "block_tables"),
                                   (seq_lens, plan.seq_lens, "seq_lens")):
             if given is not None and given.data_ptr() != held.data_ptr():
                 raise ValueError(f"{name} is not the tensor the plan was built from")
-        block_tables, seq_lens = plan.block_tables, plan.seq_lens
-    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.size(2) or not q.is_cuda:
-        raise ValueError("q must be a GPU tensor [B, Hq, D] with dense heads")
-    if q.dtype not in _DTYPES:
-        raise ValueError("q must be bf16 or fp16")
-    B, Hq, D = q.shape
-    dev = q.device
-    _check_cache(kv_cache, False, D)
-    _check_on(kv_cache, "kv_cache", dev)
-    N, Hkv = kv_cache.shape[:2]
-    if plan is not None and (max_seq_len != plan.max_seq_len or n_workgroups != plan.n_workgroups
-                             or B != plan.batch or Hkv != plan.n_kv_heads):
-        raise ValueError("the plan was built for another batch, max_seq_len, kv-head count "
-                         "or workgroup count")
-    if block_tables is None or seq_lens is None:
-        raise ValueError("block_tables and seq_lens are required without a plan")
-    _check_on(block_tables, "block_tables", dev)
-    _check_on(seq_lens, "seq_lens", dev)
-    if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.size(0) != B \
-            or seq_lens.numel() != B:
-        raise ValueError("block_tables must be [B, max_blocks] and seq_lens [B] for q's batch")
-    sl = _int32_dense(seq_lens)
+        if max_seq_len != plan.max_seq_len or n_workgroups != plan.n_workgroups \
+                or B != plan.batch or Hkv != plan.n_kv_heads:
+            raise ValueError("the plan was built for another batch, max_seq_len, kv-head count "
+                             "or workgroup count")
+        sl = plan.seq_lens
+    else:
+        if block_tables is None or seq_lens is None:
+            raise ValueError("block_tables and seq_lens are required without a plan")
+        _check_on(block_tables, "block_tables", dev)
+        _check_on(seq_lens, "seq_lens", dev)
+        if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.size(0) != B \
+                or seq_lens.numel() != B:
+            raise ValueError("block_tables must be [B, max_blocks] and seq_lens [B] for q's batch")
+        sl = _int32_dense(seq_lens)
     out = _check_out(out, q)
     if B == 0:
         return out
     lib = _lib.load()
-    dtype = _DTYPES[q.dtype]
     with device_guard(dev):
         ws_bytes = lib.aegkv_paged_decode_attention_workspace_size(B, Hq, Hkv, D, max_seq_len,
                                                                    dtype, n_workgroups)
@@ -239,7 +241,7 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
         shared = _own_workspace(dev, stream) if workspace is None else None
         if workspace is not None:
             _check_workspace(workspace, ws_bytes, dev)
-        args = (out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), kv_cache.data_ptr(),
+        args = (out.data_ptr(), out.stride(0), q.data_ptr(), q_strides[0], kv_cache.data_ptr(),
                 kv_cache.stride(0), N)
         if plan is not None:
             if stream != plan.raw_stream:
@@ -263,7 +265,7 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
 
 def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return q.new_empty(q.shape)
     if out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != q.size(2):
         raise ValueError("out must have q's shape, with dense heads")
     if out.dtype != q.dtype:
