@@ -115,16 +115,17 @@ def varlen_attention(q: np.ndarray, k_rows: np.ndarray, v_rows: np.ndarray, tabl
         if m == 0 or n == 0:
             continue
         ids = np.asarray(tables[b][:-(-n // BLOCK)])
-        k = k_rows[ids].reshape(-1, hkv, dim)[:n]
-        v = v_rows[ids].reshape(-1, hkv, dim)[:n]
+        # (heads first and dense: numpy multiplies strided matrices without its BLAS)
+        k, v = (np.ascontiguousarray(x[ids].reshape(-1, hkv, dim)[:n].swapaxes(0, 1))
+                for x in (k_rows, v_rows))
         seen = np.ones((m, n), bool)
         if causal:
             seen = np.arange(n)[None, :] <= (n - m + np.arange(m))[:, None]
         for h in range(hq):
-            s = q[t0:t1, h] @ k[:, h * hkv // hq].T * scale
+            s = np.ascontiguousarray(q[t0:t1, h]) @ k[h * hkv // hq].T * scale
             s[~seen] = -np.inf
             top = s.max(-1, keepdims=True)
             p = np.exp(s - np.where(np.isfinite(top), top, 0))
             l = p.sum(-1, keepdims=True)
-            out[t0:t1, h] = np.where(l > 0, p @ v[:, h * hkv // hq] / np.where(l > 0, l, 1), 0)
+            out[t0:t1, h] = np.where(l > 0, p @ v[h * hkv // hq] / np.where(l > 0, l, 1), 0)
     return out
