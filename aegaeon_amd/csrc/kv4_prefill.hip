@@ -17,8 +17,9 @@
 // of a sequence (varlen_shape):
 //   up to 64      four waves, two units; two key tiles per step, one per pair of
 //                 waves, joined at the end;
-//   up to 256     four waves, four units, two workgroups per CU;
-//   more          eight waves in ping-pong, one workgroup per CU.
+//   more          four waves, four units, two workgroups per CU;
+//   past 256, few tiles of many keys, head_dim 128: eight waves in ping-pong, one
+//                 workgroup per CU.
 //
 // Pieces.  When the batch has too few tiles to fill the chip, a tile's keys are
 // cut into pieces of a workgroup each, which write fp32 partials (O, running
@@ -885,10 +886,16 @@ struct VarlenShape {
   int64_t o_bytes, ml_bytes, cut_bytes;
   int64_t workspace() const { return o_bytes + ml_bytes + cut_bytes; }
 };
-// More rows of a kv head than this take the ping-pong kernel (28/4 heads, 8 x 64
-// queries over 4000 tokens each, 448 rows: 77 us by four-wave workgroups, 73 by
-// eight; 8/8 heads, 4 x 256 over 2000, 256 rows: 37 and 58).
-constexpr int kLongRows = 256;
+// The ping-pong kernel takes rows past the four-wave kernel's two tiles when its row
+// tiles fit the CUs at once and leave each 32 key steps or more (head_dim 128, 28/4
+// heads, equal lengths, us, against four waves: 4 x 512 over 8000 tokens 239 and 259,
+// 1 x 1024 over 16000 247 and 270, 8/8 heads 14 x 512 over 8000 240 and 262).
+// Shorter or more numerous tiles do better with two workgroups per CU, which
+// overlap one's start and end with the other's steps (4 x 64 over 4000 51 and 40,
+// 18 x 128 over 1000 83 and 54, 48 prompts of 220 tokens 93 and 71), and so does
+// head_dim 64 always, whose steps are mostly softmax (8/8, 14 x 512 over 8000: 229
+// and 207, 16/1, 24 x 512 over 2000: 217 and 148).
+constexpr int kLongRows = 256, kLongSteps = 32;
 // A piece's key steps at least: its partials cost about what half of these do
 // (48 x 5 drafted tokens over 1000 each: 31 us, with 8 steps 35, with 2 still 31).
 constexpr int kLeastLong = 16, kLeastShort = 4;
@@ -900,30 +907,35 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   if (rc) return rc;
   const int64_t group = n_q_heads / n_kv_heads, max_rows = (int64_t)max_q * group;
   VarlenShape s{};
-  s.long_rows = max_rows > kLongRows;
+  const int64_t cus = std::max(1, ds->num_cu);
+  // row tiles: those that the tokens fill, and a part-filled one per sequence
+  auto jobs_of = [&](int64_t rows) {
+    return n_kv_heads * std::min(batch * ((max_rows + rows - 1) / rows),
+                                 total_q * group / rows + batch);
+  };
+  const int64_t long_jobs = jobs_of(kLongWaves4 * kUnitRows);
+  s.long_rows = head_dim == 128 && max_rows > kLongRows && long_jobs <= cus &&
+                long_jobs * ((max_len + kPfKTile - 1) / kPfKTile) >= kLongSteps * cus;
   s.key_tiles = max_rows <= kShortWaves4 / 2 * kUnitRows ? 2 : 1;
   const int64_t tile_rows =
       (s.long_rows ? kLongWaves4 : kShortWaves4 / s.key_tiles) * kUnitRows;
-  // row tiles: those that the tokens fill, and a part-filled one per sequence
-  const int64_t tiles = std::min(batch * ((max_rows + tile_rows - 1) / tile_rows),
-                                 total_q * group / tile_rows + batch);
-  const int64_t jobs = tiles * n_kv_heads;
+  const int64_t jobs = s.long_rows ? long_jobs : jobs_of(tile_rows);
   const int64_t step = (int64_t)s.key_tiles * kPfKTile;
   const int64_t max_kt = (max_len + step - 1) / step;
   s.pieces = jobs;
   s.least = s.long_rows ? kLeastLong : kLeastShort;
   // Workgroups that run at once.  With half as many row tiles or fewer, their keys
-  // are cut into about as many pieces, of long rows at most as many (8 x 64 queries
-  // over 4000, 64 tiles: 67 us, whole 169, and in one piece per place and one per
-  // tile, which need a second round, 100; of short rows two share a CU and ends are
-  // uneven anyway: 48 x 5 over 1000, 192 tiles: 26.9, at most as many 28.4).  With
-  // more tiles only sequences of twice the average work of a place are cut, as
-  // partials cost more than an uneven last round (2048 queries over 16001 tokens,
-  // 224 tiles: whole 460 us, cut in two 498; 4 x 512 over 3800 each: 141 and 155).
-  // Four times as many tiles even out by themselves.
-  const int64_t slots = (int64_t)std::max(1, ds->num_cu) * (s.long_rows ? 1 : 2);
+  // are cut into about as many pieces, but not more where a second round costs much:
+  // tiles of equal length into a whole number each, others into half a piece a tile
+  // less (2 x 256 queries over 4000, 112 tiles: 53 us, of as many pieces as places
+  // and more 66; of up to 64 rows the work is as uneven anyway: 48 x 5 over 1000, 192
+  // tiles: 26.9, so 28.4).  With more tiles only sequences of twice the average work
+  // of a place are cut, as partials cost more than an uneven last round (2048 queries
+  // over 16001 tokens, 224 tiles: whole 460 us, cut in two 498).  Four times as many
+  // tiles even out by themselves.
+  const int64_t slots = cus * (s.long_rows ? 1 : 2);
   if (jobs < 4 * slots && max_kt > s.least) {
-    s.target = jobs > slots / 2 ? slots / 2 : s.long_rows ? slots - jobs : slots;
+    s.target = jobs > slots / 2 ? slots / 2 : s.key_tiles > 1 ? slots : slots - jobs * 7 / 8;
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     s.cut = jobs;
@@ -966,12 +978,12 @@ void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   const dim3 g((uint32_t)s.pieces), four(64 * kShortWaves4), eight(64 * kLongWaves4);
-  if (s.long_rows) hipLaunchKernelGGL((kv4_varlen_long_kernel<DT, D>), g, eight, 0, st, a);
+  if (s.long_rows) hipLaunchKernelGGL((kv4_varlen_long_kernel<DT, 128>), g, eight, 0, st, a);
   else if (s.key_tiles == 2) hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 2>), g, four, 0, st, a);
   else hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 1>), g, four, 0, st, a);
   AEGKV_HIP_TRY(hipGetLastError());
   if (s.target > 0) {
-    if (s.long_rows) launch_merge<DT, D, kLongWaves4>(a, s, st);
+    if (s.long_rows) launch_merge<DT, 128, kLongWaves4>(a, s, st);
     else if (s.key_tiles == 2) launch_merge<DT, D, kShortWaves4 / 2>(a, s, st);
     else launch_merge<DT, D, kShortWaves4>(a, s, st);
     AEGKV_HIP_TRY(hipGetLastError());

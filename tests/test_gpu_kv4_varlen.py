@@ -108,14 +108,53 @@ def test_lengths(device, new, lens, Hq, Hkv, D):
 
 
 @pytest.mark.parametrize("new,lens,Hq,Hkv,D", [
-    ([1200], [2500], 14, 2, 128),                      # eight-wave workgroups
-    ([200] * 9, [1000] * 9, 8, 8, 64),                 # four waves, one key tile per step
+    ([1200], [2500], 14, 2, 128),                      # four waves, one key tile per step
+    ([200] * 9, [1000] * 9, 8, 8, 64),
     ([64] * 40, [5000] + [100] * 39, 8, 8, 64),        # two, one sequence cut of many
     ([64] * 140, [70] * 139 + [5000], 8, 8, 64),       # of very many
     ([300] * 140, [6000] + [300] * 139, 2, 2, 64)])
 def test_cut_sequences_of_many_rows(device, new, lens, Hq, Hkv, D):
     b = Batch(device, new, lens, Hq, Hkv, D, "bf16", sum(lens))
     b.check(b.run(0.1), 0.1)
+
+
+# Few tiles of many rows and keys: eight-wave workgroups, whole (47 tiles of 256
+# rows and more per kv head) and cut.
+@pytest.mark.parametrize("new,lens", [([1, 300, 700], [50, 5000, 6200]), ([600], [6001]),
+                                      ([40, 300], [2000, 9000])])
+@pytest.mark.parametrize("dtype,causal", [("bf16", True), ("fp16", False)])
+def test_few_tiles_of_many_keys(device, new, lens, dtype, causal):
+    b = Batch(device, new, lens, 40, 2, 128, dtype, sum(lens))
+    b.check(b.run(-0.1, causal), -0.1, causal)
+
+
+def test_nan_and_unreadable_blocks_of_long_rows(device):
+    """As the tests below for fewer rows: a NaN of V shows in its dims of the rows
+    that attend to its token, and an unreadable block is masked."""
+    b = Batch(device, [600], [6001], 40, 2, 128, "bf16", 3)
+    token, grp = 5700, 2
+    dirty = b.dc.clone()
+    dirty[b.tables[0][token // 16], 1, 1, 8 * 128 + grp * 16 + token % 16] = 255
+    clean, out = b.run(0.1), b.run(0.1, cache=dirty)
+    seen = torch.zeros(out.shape, dtype=torch.bool, device=device)
+    seen[token - 5401:, 20:, 32 * grp:32 * grp + 32] = True
+    assert torch.isnan(out[seen].float()).all()
+    assert torch.equal(out[~seen].view(torch.int16), clean[~seen].view(torch.int16))
+    bad = b.bt.clone()
+    bad[0, token // 16] = b.dc.size(0)
+    gone = kv4.varlen_attention_kv4(b.dq, dirty, bad, b.dcu, b.sl, 600, 6001, 0.1)
+    k, v = (np.nan_to_num(x) for x in k4.rows(b.cache, 128))
+    rows = [np.ascontiguousarray(x[b.tables[0]].reshape(-1, 2, 128)[:6001].swapaxes(0, 1))
+            for x in (k, v)]
+    keep = np.arange(6001) // 16 != token // 16
+    q = ko.bits_to_float(b.q, "bf16")
+    want = np.zeros(q.shape)
+    for h in range(40):
+        s = np.ascontiguousarray(q[:, h]) @ rows[0][h // 20].T * 0.1
+        s[~(keep & (np.arange(6001) <= 5401 + np.arange(600)[:, None]))] = -np.inf
+        p = np.exp(s - s.max(-1, keepdims=True))
+        want[:, h] = p @ rows[1][h // 20] / p.sum(-1, keepdims=True)
+    within(gone.double().cpu().numpy(), want, "bf16")
 
 
 @pytest.mark.parametrize("first", [1, 100, 300])
