@@ -31,13 +31,13 @@
 //
 // Bounds and measured.  Per cached token and kv head 17 D / 16 bytes are read
 // and 4 D G flops done per query, so past some 10 queries at G = 7 the products
-// bound it: 2048 queries over 16001 tokens (28/4 heads, D = 128) 467 us, 940
-// TFLOP/s (224 of 256 CUs hold a tile, at 87% of the rate of a large matrix
+// bound it: 2048 queries over 16001 tokens (28/4 heads, D = 128) 462 us, 950
+// TFLOP/s (224 of 256 CUs hold a tile, at 90% of the rate of a large matrix
 // product each); 4 x 512 over 3800 tokens each 142 us, the longest sequence's;
-// two whole prompts of 2048 85 us.  Few queries are bound by the latency of
+// two whole prompts of 2048 80 us.  Few queries are bound by the latency of
 // their steps, 1.7 us each of a lone workgroup (conversion, products and softmax
-// of a wave follow each other): 48 x 5 over 1000 tokens each (32/4) 28.5 us,
-// of which the merge 4.6.
+// of a wave follow each other): 48 x 5 over 1000 tokens each (32/4) 26.2 us,
+// of which the merge 4.4.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
