@@ -943,7 +943,8 @@ int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
     // Rows of a merge workgroup: 4 where a tile has many pieces (a query over 60000,
     // 128 pieces: 27.3 us, of 16 rows 41.3), 16 where it has few (4 x 128 over 3000:
     // 53.9, of 4 rows 57.4), 32 where there are many tiles, most of them uncut.
-    s.merge_rows = s.target >= 16 * jobs ? 4 : jobs * per_tile(16) <= 4096 ? 16 : 32;
+    s.merge_rows = s.target >= 16 * jobs ? 4
+                   : s.long_rows || jobs * per_tile(16) <= 4096 ? 16 : 32;
     s.merge_per_tile = per_tile(s.merge_rows);
     s.ml_bytes = s.pieces * tile_rows * 8;
     s.cut_bytes = 256 + s.cut * (int64_t)sizeof(CutTile);
@@ -971,9 +972,13 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
 template <int DT, int D, int W>
 void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   const dim3 g((uint32_t)(s.cut * s.merge_per_tile)), t(kMerge4Threads);
-  if (s.merge_rows == 4) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 4>), g, t, 0, st, a);
-  else if (s.merge_rows == 16) hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 16>), g, t, 0, st, a);
-  else hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 32>), g, t, 0, st, a);
+  if (s.merge_rows == 4) {
+    hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 4>), g, t, 0, st, a);
+  } else if (s.merge_rows == 16) {
+    hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 16>), g, t, 0, st, a);
+  } else if constexpr (W < kLongWaves4) {
+    hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 32>), g, t, 0, st, a);
+  }
 }
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {

@@ -121,7 +121,7 @@ def test_cut_sequences_of_many_rows(device, new, lens, Hq, Hkv, D):
 # Few tiles of many rows and keys: eight-wave workgroups, whole (47 tiles of 256
 # rows and more per kv head) and cut.
 @pytest.mark.parametrize("new,lens", [([1, 300, 700], [50, 5000, 6200]), ([600], [6001]),
-                                      ([40, 300], [2000, 9000])])
+                                      ([40, 300], [2000, 9600])])
 @pytest.mark.parametrize("dtype,causal", [("bf16", True), ("fp16", False)])
 def test_few_tiles_of_many_keys(device, new, lens, dtype, causal):
     b = Batch(device, new, lens, 40, 2, 128, dtype, sum(lens))
