@@ -11,8 +11,9 @@
 // block's codes in registers ahead of its tile, converts them to 16 bits, where
 // they are exact, and stores them to LDS; every wave takes S = K.Q^T, the online
 // softmax and O += V^T.P^T of its rows from there (prefill_wave.h, 32x32x16
-// MFMA, fp32 sums; P rounded to 16 bits as in the prompt attention: its error is
-// below the output's own).  The conversion, 190 instructions per 128 keys and
+// MFMA, fp32 sums; P rounded to 16 bits as in the prompt attention: a weight is off
+// by half a step at most, as the output is by its own rounding; the sum of the
+// weights is of the unrounded ones).  The conversion, 190 instructions per 128 keys and
 // wave, is shared by the tile's units, so few rows pay for it most.  By the rows
 // of a sequence (varlen_shape):
 //   up to 64      four waves, two units; two key tiles per step, one per pair of
@@ -83,7 +84,7 @@ struct VarlenArgs {
   int32_t least;             // least key tiles of a piece
   int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
   float* part_o;             // [n_pieces][32 W][D]
-  float2* part_ml;           // [n_pieces][32 W] (running max in log2 units, sum)
+  float2* part_ml;           // [n_pieces][32 W] (running max less kTop in log2 units, sum)
   int32_t* n_cut;            // row tiles that are cut, and one CutTile each: written
   CutTile* cut;              // by the main kernel (target > 0) for the merge
   int32_t max_cut;           // bound of them

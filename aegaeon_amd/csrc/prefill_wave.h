@@ -24,11 +24,17 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr int kPfKTile = 64;                 // keys per step
 constexpr float kPfRescaleSlack = 8.f;
 
+// kTop: log2 of the weight of a row's largest score (where nothing was rescaled
+// lately up to kPfRescaleSlack more).  fp16 holds weights up to 2^15, so that its
+// subnormals, off by 2^-25 at most, begin 2^21 below the largest weight: with 2^0 for
+// it thousands of keys of 2^-25 each were rounded away beside one key, while the sum
+// of the weights counted them.
 template <int DT>
 struct PfOps;
 
 template <>
 struct PfOps<AEGKV_DTYPE_BF16> {
+  static constexpr float kTop = 0.f;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -41,6 +47,7 @@ struct PfOps<AEGKV_DTYPE_BF16> {
 
 template <>
 struct PfOps<AEGKV_DTYPE_FP16> {
+  static constexpr float kTop = 7.f;
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -92,7 +99,7 @@ struct WaveSoftmax {
   static constexpr int DB = D / 32;  // 32-row blocks of O^T
   u32x4 qv[KS];                      // Q^T operand: dims 16 ks + 8 hh .. +7
   f32x16 o[DB];
-  float m, lsum;
+  float m, lsum;  // m: the running maximum less kTop (log2 units); lsum: of this lane's keys
 
   // online softmax of a masked S^T tile into the P^T operands of its four
   // 16-key steps
@@ -123,7 +130,9 @@ struct WaveSoftmax {
     // to the shuffle; the four-wave kernel 0-2% faster with it.)
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(bm), __float_as_uint(bm),
                                                      false, false);
-    bm = fmaxf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), bm) * scale_log2;
+    bm = fmaxf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), bm);
+    if constexpr (PfOps<DT>::kTop == 0.f) bm *= scale_log2;
+    else bm = __builtin_fmaf(bm, scale_log2, -PfOps<DT>::kTop);
     if (first) {
       m = fmaxf(m, bm);
     } else if (__builtin_amdgcn_ballot_w64(bm > m + kPfRescaleSlack)) {
