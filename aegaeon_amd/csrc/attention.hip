@@ -177,11 +177,16 @@ __device__ __forceinline__ int64_t active_ranges(const RangeRule& r, int64_t tot
 
 constexpr float kRescaleSlack = 8.f;  // log2 headroom of the lazy softmax rescale
 
+// kTop: log2 of the weight of a row's largest score (between rescales up to
+// kRescaleSlack more).  fp16 holds weights up to 2^15, so that the low parts' bits
+// end 2^32 below the largest weight: with 2^0 for it thousands of keys of 2^-25 each
+// were rounded away beside one key, while the sum of the weights counted them.
 template <int DT>
 struct Elem;
 
 template <>
 struct Elem<AEGKV_DTYPE_BF16> {
+  static constexpr float kTop = 0.f;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -204,6 +209,7 @@ struct Elem<AEGKV_DTYPE_BF16> {
 
 template <>
 struct Elem<AEGKV_DTYPE_FP16> {
+  static constexpr float kTop = 7.f;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -248,7 +254,7 @@ struct AttnArgs {
   int64_t out_bstride;  // elements
   int4* desc;           // merge descriptors (see merge_desc)
   float* part_o;        // [slots][hpg][D]
-  float2* part_ml;      // [slots][hpg] (running max in log2 units, sum)
+  float2* part_ml;      // [slots][hpg] (running max less kTop in log2 units, sum)
   uint32_t ml_bytes, o_bytes;  // sizes of the two partial regions (< 2^31)
   int32_t stage_slots;  // finished pieces a wave holds in LDS (0: stored at once)
   int32_t stage_off;    // byte offset of the staging area in dynamic LDS
@@ -641,7 +647,9 @@ __device__ __forceinline__ void unpack_columns(const f32x4* packed, f32x4* acc) 
 
 // P's operands of one block.  16-bit parts in a register's low half belong to
 // the even dims of V's pairs, in the high half to the odd ones.  low_part, odd:
-// this lane's column (PACK 2, 4).
+// this lane's column (PACK 2, 4).  Two parts of bf16, cut off, hold 16 bits of a
+// weight, below the output's rounding; of fp16 22 bits, down to 2^-25 (2^-32 of the
+// largest weight, Elem::kTop).
 template <int DT, int PACK>
 struct Weights4 {
   static constexpr int N = 4 / PACK;  // operands: (even, odd) of the high part, of the other
@@ -727,7 +735,9 @@ __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const
   for (int u = 0; u < kStep4; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) bm = fmaxf(bm, sc[u][i]);
-  bm = max_over_g(bm) * scale_log2;
+  bm = max_over_g(bm);
+  if constexpr (E::kTop == 0.f) bm *= scale_log2;
+  else bm = __builtin_fmaf(bm, scale_log2, -E::kTop);
   if (__builtin_amdgcn_ballot_w64(bm > m + kRescaleSlack)) {  // lazy rescaling, as in compute_block
     const float mn = fmaxf(m, bm);
     // 0 while m = -inf (beside another head's first finite score too)

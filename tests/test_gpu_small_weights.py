@@ -99,3 +99,15 @@ def test_prompts(device, n, batch, Hq, D):
     rows = np.unique(np.concatenate([[0, 2, 3, 4, 63, 64, 65, n - 1], rng.integers(0, n, 40)]))
     for b in range(batch):
         _check(out[b, torch.from_numpy(rows).to(device)], q[rows], k, v, rows + 1, 11)
+
+
+@pytest.mark.parametrize("Hq,D", [(4, 64), (7, 128), (16, 128), (2, 256)])
+@pytest.mark.parametrize("nwg", [0, 1])
+def test_decode_over_the_4_bit_cache(device, Hq, D, nwg):
+    rng = np.random.default_rng(Hq + D)
+    n = 40001
+    cache, bt, sl, k, v = _cache4(rng, device, n, D, 3)
+    q = _queries(rng, 1, Hq, D)
+    out = kv4.paged_decode_attention_kv4(torch.from_numpy(q).to(device), cache, bt, sl, SCALE, n,
+                                         n_workgroups=nwg)
+    _check(out, q, k, v, [n], 22)
