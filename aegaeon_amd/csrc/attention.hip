@@ -470,10 +470,12 @@ __device__ __forceinline__ void compute_block(KVRegs<D>& r, const u32x4* qv, f32
   float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
   bm = fmaxf(bm, __shfl_xor(bm, 16));
   bm = fmaxf(bm, __shfl_xor(bm, 32));
-  // Lazy rescaling: exponents are taken against a reference max m that moves
-  // only when a block's max exceeds it by more than kRescaleSlack (log2 units),
-  // so p <= 2^kRescaleSlack (exact in bf16/fp16, harmless in fp32) and the
-  // accumulators are rescaled in a rare branch instead of on every block.
+  if constexpr (E::kTop != 0.f) bm -= E::kTop;
+  // Lazy rescaling: exponents are taken against a reference m, a max less kTop,
+  // that moves only when a block's exceeds it by more than kRescaleSlack (log2
+  // units), so p <= 2^(kTop + kRescaleSlack) (within fp16's range, harmless in
+  // fp32) and the accumulators are rescaled in a rare branch instead of on every
+  // block.
   if (__builtin_amdgcn_ballot_w64(bm > m + kRescaleSlack)) {
     const float mn = fmaxf(m, bm);
     const float alpha = __builtin_amdgcn_exp2f(m - mn);  // 0 while m = -inf

@@ -111,3 +111,28 @@ def test_decode_over_the_4_bit_cache(device, Hq, D, nwg):
     out = kv4.paged_decode_attention_kv4(torch.from_numpy(q).to(device), cache, bt, sl, SCALE, n,
                                          n_workgroups=nwg)
     _check(out, q, k, v, [n], 22)
+
+
+@pytest.mark.parametrize("Hq,D", [(4, 64), (7, 128), (2, 256)])
+@pytest.mark.parametrize("nwg", [0, 1])
+@pytest.mark.parametrize("appending", [False, True])
+def test_decode(device, Hq, D, nwg, appending):
+    rng = np.random.default_rng(Hq + D)
+    n = 40001
+    k, v = _rows(rng, n, D, 3)
+    q = _queries(rng, 1, Hq, D)
+    blocks = -(-n // 16)
+    caches = torch.zeros(2, blocks * 16, 1, D, dtype=torch.float16, device=device)
+    held = n - 1 if appending else n
+    for c, x in zip(caches, (k, v)):
+        c[:held, 0] = torch.from_numpy(x[:held]).to(device)
+    new = {}
+    if appending:
+        new = {name: torch.from_numpy(x[-1].reshape(1, 1, D)).to(device)
+               for name, x in (("key", k), ("value", v))}
+    kc, vc = caches.view(2, blocks, 16, 1, D)
+    bt = torch.arange(blocks, dtype=torch.int32, device=device)[None]
+    sl = torch.tensor([n], dtype=torch.int32, device=device)
+    out = A.paged_decode_attention(torch.from_numpy(q).to(device), kc, vc, bt, sl, SCALE, n,
+                                   n_workgroups=nwg, **new)
+    _check(out, q, k, v, [n], 22)
