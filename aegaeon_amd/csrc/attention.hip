@@ -2134,6 +2134,8 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
   if (batch < 0 || max_seq_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || max_blocks < 0 ||
       n_blocks < 0 || n_workgroups < 0)
     return AEGKV_ERR_INVALID_ARG;
+  // (times a score of zero, or of a masked token, an infinite one would give NaN)
+  if (kv4 && !std::isfinite(scale * 1.4426950408889634f)) return AEGKV_ERR_INVALID_ARG;
   if (n_q_heads % n_kv_heads) return AEGKV_ERR_INVALID_ARG;
   if (block_size != kBlockSize || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
       n_q_heads / n_kv_heads > 16 || (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16))

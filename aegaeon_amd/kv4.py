@@ -194,8 +194,9 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
     ``out [B, Hq, D]``, both of the type the cache was written from.  Tables,
     lengths, ``n_workgroups``, ``plan`` (a :class:`attention.DecodePlan` serves
     either cache) and ``workspace`` (:func:`attention.attention_workspace`) are
-    that function's; a sequence without tokens gives zeros.  New rows are
-    appended by a call of their own, before this one."""
+    that function's; a sequence without tokens gives zeros.  ``scale``: any
+    number that stays finite times log2 e.  New rows are appended by a call of
+    their own, before this one."""
     shape, q_strides, dev = q.shape, q.stride(), q.device
     if len(shape) != 3 or q_strides[2] != 1 or q_strides[1] != shape[2] or not q.is_cuda:
         raise ValueError("q must be a GPU tensor [B, Hq, D] with dense heads")

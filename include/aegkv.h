@@ -445,7 +445,8 @@ int aegkv_kv4_gather_tokens(const void* cache, int64_t cache_block_stride,
 /* aegkv_paged_decode_attention over a layer of the 4-bit cache: its arguments,
  * limits, workspace (aegkv_paged_decode_attention_workspace_size) and plans
  * (aegkv_paged_decode_plan), with one cache in place of two.  q and out are of
- * the type that the cache was written from. */
+ * the type that the cache was written from; scale is any that stays finite times
+ * log2 e. */
 int aegkv_kv4_decode_attention(void* out, int64_t out_batch_stride, const void* q,
                                int64_t q_batch_stride, const void* cache,
                                int64_t cache_block_stride, int64_t n_blocks,
