@@ -964,8 +964,10 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   if ((head_dim != 64 && head_dim != 128) ||
       (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16))
     return AEGKV_ERR_UNSUPPORTED;
-  // rows of a sequence in 32 bits, a tile further
-  if ((int64_t)max_q * (n_q_heads / n_kv_heads) > INT32_MAX / 2 || max_len > INT32_MAX - kPfKTile)
+  // in 32 bits: the rows of a sequence, a tile further; its keys, the end of a step of
+  // two tiles and two tiles of loads ahead further
+  if ((int64_t)max_q * (n_q_heads / n_kv_heads) > INT32_MAX / 2 ||
+      max_len > INT32_MAX - 4 * kPfKTile)
     return AEGKV_ERR_UNSUPPORTED;
   return AEGKV_OK;
 }

@@ -5,7 +5,7 @@ import pytest
 
 from aegaeon_amd import _lib
 
-INVALID = -1
+INVALID, UNSUPPORTED = -1, -6
 
 
 @pytest.fixture(scope="module")
@@ -33,3 +33,12 @@ def test_decode_refuses_a_scale_that_overflows(lib, ptr, scale):
     assert lib.aegkv_kv4_decode_attention_planned(p, 1024, p, 1024, p, 17 * 4 * 128, 8, p, 1 << 16,
                                                   p, 2, 64, 8, 4, 128, scale, 0, 8, p, 1 << 30,
                                                   None) == INVALID
+
+
+def test_several_queries_refuse_lengths_whose_last_step_passes_32_bits(lib):
+    """A step of two key tiles ends up to 127 keys past the last one, the loads ahead
+    two tiles further."""
+    size = lib.aegkv_kv4_varlen_attention_workspace_size
+    for longest in (2 ** 31 - 1, 2 ** 31 - 65, 2 ** 31 - 128, 2 ** 31 - 256):
+        for new in (1, 20, 600):
+            assert size(1, new, new, longest, 8, 2, 128, 0) == UNSUPPORTED
