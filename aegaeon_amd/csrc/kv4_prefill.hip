@@ -44,6 +44,7 @@
 #include <type_traits>
 
 #include "aegkv_internal.h"
+#include "kv4_cut.h"
 #include "kv4_format.h"
 #include "prefill_wave.h"
 
@@ -127,9 +128,6 @@ struct LocateLds {
   int sum[16], cut[16];
   int found[11];
 };
-__device__ __forceinline__ int ranges_of(int n_kt, int span) {
-  return max(1, (n_kt + span - 1) / span);
-}
 // The piece numbered blockIdx.x, found by all NT threads, each summing its own
 // sequences.  False: there are fewer.  The first workgroup writes n_cut.
 template <int W, int KS, int NT>
