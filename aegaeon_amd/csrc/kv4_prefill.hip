@@ -55,15 +55,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int kUnitRows = 32;   // rows of a wave
 constexpr int kTileBlocks = kPfKTile / kKv4Tokens;
-constexpr int kShortWaves4 = 4;
-
-// A row tile whose keys are cut: its rows [row0, row1) of kv head `head`, the first
-// of its pieces, which follow each other.
-struct CutTile {
-  int32_t t0, head, row0, row1, piece0, pieces;
-};
+static_assert(kKeyTile == kPfKTile, "the key tiles of the cut");
 
 struct VarlenArgs {
   const uint8_t* q;
@@ -156,8 +149,7 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, LocateLds& x, Piece&
 #pragma unroll
     for (int w = 0; w < NW; ++w) cost += x.cost[w];
     cost *= a.n_kv_heads;
-    span = (int)min((cost + a.target - 1) / a.target, (int64_t)INT32_MAX);
-    span = max(span, a.least);
+    span = span_of(cost, a.target, a.least);
   }
   int count = 0, cuts = 0;  // this thread's pieces and cut row tiles
   auto add = [&](const SeqWork& s, int& pieces, int& cut) {
@@ -695,7 +687,6 @@ __global__ __launch_bounds__(64 * kShortWaves4, 2) void kv4_varlen_kernel(Varlen
 // go with the softmax: in slot 2j + 1 waves 0-3 convert a block of K_{j+1} each,
 // in slot 2j waves 4-7 one of V_j.  K_{j+1}'s stage was last read (as K_{j-1})
 // in slot 2j - 1 and is read from slot 2j + 2 on, V_j's as well.
-constexpr int kLongWaves4 = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kLongWaves4) void kv4_varlen_long_kernel(VarlenArgs a) {
   constexpr int W = kLongWaves4;
@@ -871,89 +862,6 @@ __global__ __launch_bounds__(kMerge4Threads) void kv4_varlen_merge_kernel(Varlen
               PfOps<DT>::pack(acc[k][2] * inv, acc[k][3] * inv)};
 }
 
-// The launch of a call: which kernel, how many pieces at most, and whether
-// sequences are cut.
-struct VarlenShape {
-  bool long_rows;
-  int key_tiles;    // of a step
-  int64_t pieces;   // bound of the pieces (the main grid)
-  int64_t target;   // pieces wanted (0: uncut)
-  int32_t least;    // key steps of a piece at least
-  int64_t cut;      // bound of the row tiles that are cut
-  int merge_rows;   // rows of a merge workgroup
-  int64_t merge_per_tile;  // merge workgroups of a row tile
-  int64_t o_bytes, ml_bytes, cut_bytes;
-  int64_t workspace() const { return o_bytes + ml_bytes + cut_bytes; }
-};
-// The ping-pong kernel takes rows past the four-wave kernel's two tiles when its row
-// tiles fit the CUs at once and leave each 32 key steps or more (head_dim 128, 28/4
-// heads, equal lengths, us, against four waves: 4 x 512 over 8000 tokens 239 and 259,
-// 1 x 1024 over 16000 247 and 270, 8/8 heads 14 x 512 over 8000 240 and 262).
-// Shorter or more numerous tiles do better with two workgroups per CU, which
-// overlap one's start and end with the other's steps (4 x 64 over 4000 51 and 40,
-// 18 x 128 over 1000 83 and 54, 48 prompts of 220 tokens 93 and 71), and so does
-// head_dim 64 always, whose steps are mostly softmax (8/8, 14 x 512 over 8000: 229
-// and 207, 16/1, 24 x 512 over 2000: 217 and 148).
-constexpr int kLongRows = 256, kLongSteps = 32;
-// A piece's key steps at least: its partials cost about what half of these do
-// (48 x 5 drafted tokens over 1000 each: 31 us, with 8 steps 35, with 2 still 31).
-constexpr int kLeastLong = 16, kLeastShort = 4;
-
-int varlen_shape(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
-                 int32_t n_kv_heads, int32_t head_dim, VarlenShape* out) {
-  DeviceState* ds = nullptr;
-  const int rc = current_device_state(&ds);
-  if (rc) return rc;
-  const int64_t group = n_q_heads / n_kv_heads, max_rows = (int64_t)max_q * group;
-  VarlenShape s{};
-  const int64_t cus = std::max(1, ds->num_cu);
-  // row tiles: those that the tokens fill, and a part-filled one per sequence
-  auto jobs_of = [&](int64_t rows) {
-    return n_kv_heads * std::min(batch * ((max_rows + rows - 1) / rows),
-                                 total_q * group / rows + batch);
-  };
-  const int64_t long_jobs = jobs_of(kLongWaves4 * kUnitRows);
-  s.long_rows = head_dim == 128 && max_rows > kLongRows && long_jobs <= cus &&
-                long_jobs * ((max_len + kPfKTile - 1) / kPfKTile) >= kLongSteps * cus;
-  s.key_tiles = max_rows <= kShortWaves4 / 2 * kUnitRows ? 2 : 1;
-  const int64_t tile_rows =
-      (s.long_rows ? kLongWaves4 : kShortWaves4 / s.key_tiles) * kUnitRows;
-  const int64_t jobs = s.long_rows ? long_jobs : jobs_of(tile_rows);
-  const int64_t step = (int64_t)s.key_tiles * kPfKTile;
-  const int64_t max_kt = (max_len + step - 1) / step;
-  s.pieces = jobs;
-  s.least = s.long_rows ? kLeastLong : kLeastShort;
-  // Workgroups that run at once.  With half as many row tiles or fewer, their keys
-  // are cut into about as many pieces, but not more where a second round costs much:
-  // tiles of equal length into a whole number each, others into half a piece a tile
-  // less (2 x 256 queries over 4000, 112 tiles: 53 us, of as many pieces as places
-  // and more 66; of up to 64 rows the work is as uneven anyway: 48 x 5 over 1000, 192
-  // tiles: 26.9, so 28.4).  With more tiles only sequences of twice the average work
-  // of a place are cut, as partials cost more than an uneven last round (2048 queries
-  // over 16001 tokens, 224 tiles: whole 460 us, cut in two 498).  Four times as many
-  // tiles even out by themselves.
-  const int64_t slots = cus * (s.long_rows ? 1 : 2);
-  if (jobs < 4 * slots && max_kt > s.least) {
-    s.target = jobs > slots / 2 ? slots / 2 : s.key_tiles > 1 ? slots : slots - jobs * 7 / 8;
-    // a sequence of cost x has at most x / span + its tiles
-    s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
-    s.cut = jobs;
-    auto per_tile = [&](int64_t r) { return (std::min(max_rows, tile_rows) + r - 1) / r; };
-    // Rows of a merge workgroup: 4 where a tile has many pieces (a query over 60000,
-    // 128 pieces: 27.3 us, of 16 rows 41.3), 16 where it has few (4 x 128 over 3000:
-    // 53.9, of 4 rows 57.4), 32 where there are many tiles, most of them uncut.
-    s.merge_rows = s.target >= 16 * jobs ? 4
-                   : s.long_rows || jobs * per_tile(16) <= 4096 ? 16 : 32;
-    s.merge_per_tile = per_tile(s.merge_rows);
-    s.ml_bytes = s.pieces * tile_rows * 8;
-    s.cut_bytes = 256 + s.cut * (int64_t)sizeof(CutTile);
-    s.o_bytes = s.pieces * tile_rows * head_dim * 4;
-  }
-  if (s.pieces > INT32_MAX / 2 || s.cut * s.merge_per_tile > INT32_MAX / 2) return AEGKV_ERR_UNSUPPORTED;
-  *out = s;
-  return AEGKV_OK;
-}
-
 int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
                  int32_t n_kv_heads, int32_t head_dim, int32_t dtype) {
   if (batch < 0 || total_q < 0 || max_q < 0 || max_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 ||
@@ -970,8 +878,19 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
   return AEGKV_OK;
 }
 
+int shape_of(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
+             int32_t n_kv_heads, int32_t head_dim, VarlenShape* s) {
+  DeviceState* ds = nullptr;
+  const int rc = current_device_state(&ds);
+  if (rc) return rc;
+  return varlen_shape(std::max(1, ds->num_cu), batch, total_q, max_q, max_len, n_q_heads,
+                      n_kv_heads, head_dim, s)
+             ? AEGKV_OK
+             : AEGKV_ERR_UNSUPPORTED;
+}
+
 template <int DT, int D, int W>
-void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
+int launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   const dim3 g((uint32_t)(s.cut * s.merge_per_tile)), t(kMerge4Threads);
   if (s.merge_rows == 4) {
     hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 4>), g, t, 0, st, a);
@@ -979,7 +898,11 @@ void launch_merge(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
     hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 16>), g, t, 0, st, a);
   } else if constexpr (W < kLongWaves4) {
     hipLaunchKernelGGL((kv4_varlen_merge_kernel<DT, D, W, 32>), g, t, 0, st, a);
+  } else {
+    return AEGKV_ERR_UNSUPPORTED;  // not of eight waves' few tiles (varlen_shape)
   }
+  AEGKV_HIP_TRY(hipGetLastError());
+  return AEGKV_OK;
 }
 template <int DT, int D>
 int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
@@ -989,10 +912,9 @@ int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
   else hipLaunchKernelGGL((kv4_varlen_kernel<DT, D, 1>), g, four, 0, st, a);
   AEGKV_HIP_TRY(hipGetLastError());
   if (s.target > 0) {
-    if (s.long_rows) launch_merge<DT, 128, kLongWaves4>(a, s, st);
-    else if (s.key_tiles == 2) launch_merge<DT, D, kShortWaves4 / 2>(a, s, st);
-    else launch_merge<DT, D, kShortWaves4>(a, s, st);
-    AEGKV_HIP_TRY(hipGetLastError());
+    if (s.long_rows) return launch_merge<DT, 128, kLongWaves4>(a, s, st);
+    if (s.key_tiles == 2) return launch_merge<DT, D, kShortWaves4 / 2>(a, s, st);
+    return launch_merge<DT, D, kShortWaves4>(a, s, st);
   }
   return AEGKV_OK;
 }
@@ -1013,7 +935,7 @@ int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q
   if (rc) return rc;
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return 0;
   VarlenShape s;
-  rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
   if (rc) return rc > 0 ? AEGKV_ERR_RUNTIME : rc;
   return s.workspace();
 }
@@ -1043,7 +965,7 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
     return AEGKV_ERR_MISALIGNED;
   if (((int64_t)max_seq_len + kKv4Tokens - 1) / kKv4Tokens > max_blocks) return AEGKV_ERR_INVALID_ARG;
   VarlenShape s;
-  rc = varlen_shape(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
   if (rc) return rc;
   if (s.target > 0 && (!workspace || workspace_bytes < (uint64_t)s.workspace()))
     return AEGKV_ERR_WORKSPACE;

@@ -1,8 +1,12 @@
 // The cut of the keys by the attention of several query tokens over the 4-bit cache
 // (csrc/kv4_cut.h), built with UndefinedBehaviorSanitizer by tests/test_kv4_cut.py.
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <random>
+#include <vector>
 
 #include "../../aegaeon_amd/csrc/kv4_cut.h"
 
@@ -28,8 +32,73 @@ static void ranges() {
     }
 }
 
+// Random batches against the shape that the host gives them by their bounds alone:
+// as many pieces, cut tiles and merge workgroups as the device can find, and a
+// merge kernel that exists.
+static void batches() {
+  std::mt19937_64 rng(7);
+  auto upto = [&](double hi) {  // 1 .. hi, evenly over the logarithm
+    return (int)std::exp(std::uniform_real_distribution<double>(0, std::log(hi + 0.999))(rng));
+  };
+  int64_t eight = 0, rows[3] = {}, cut_calls = 0;
+  for (int n = 0; n < 60000; ++n) {
+    const int cus = n % 3 ? 256 : upto(304), batch = upto(300), hkv = upto(40), group = upto(40);
+    const int dim = n & 1 ? 128 : 64;
+    const int top_q = upto(n % 5 ? 600 : 20000), top_len = upto(n % 7 ? 20000 : 3e5);
+    struct Seq {
+      int m, len;
+    };
+    std::vector<Seq> seqs(batch);
+    int64_t total = 0;
+    int max_q = 0, max_len = 0;
+    for (Seq& s : seqs) {
+      s.m = n % 11 ? upto(top_q + 1) - 1 : top_q;
+      s.len = n % 13 ? upto(top_len + 1) - 1 : top_len;
+      total += s.m;
+      max_q = std::max(max_q, s.m);
+      max_len = std::max(max_len, s.len);
+    }
+    if (total == 0) continue;
+    VarlenShape s;
+    if (!varlen_shape(cus, batch, total, max_q, max_len, hkv * group, hkv, dim, &s)) continue;
+    const int tile_rows = 32 * (s.long_rows ? 8 : 4 / s.key_tiles), step = 64 * s.key_tiles;
+    auto tiles_of = [&](const Seq& q) {
+      return ((int64_t)q.m * group + tile_rows - 1) / tile_rows * hkv;
+    };
+    auto steps_of = [&](const Seq& q) {  // (the last query sees every key)
+      return q.m > 0 ? (q.len + step - 1) / step : 0;
+    };
+    int64_t cost = 0, pieces = 0, cut = 0;
+    for (const Seq& q : seqs) cost += tiles_of(q) * steps_of(q);
+    const int span = s.target > 0 ? span_of(cost, s.target, s.least) : INT32_MAX;
+    for (const Seq& q : seqs) {
+      const int r = ranges_of(steps_of(q), span);
+      pieces += tiles_of(q) * r;
+      cut += r > 1 ? tiles_of(q) : 0;
+    }
+    CHECK(pieces <= s.pieces, "batch %d: %lld pieces, a grid of %lld", n, (long long)pieces,
+          (long long)s.pieces);
+    CHECK(cut <= s.cut, "batch %d: %lld tiles cut, room for %lld", n, (long long)cut, (long long)s.cut);
+    CHECK(s.workspace() == (s.target > 0 ? s.pieces * tile_rows * (4ll * dim + 8) + 256 + 24 * s.cut : 0),
+          "batch %d: a workspace of %lld", n, (long long)s.workspace());
+    eight += s.long_rows;
+    if (s.target == 0) continue;
+    cut_calls += cut > 0;
+    CHECK(s.merge_rows == 4 || s.merge_rows == 16 || (s.merge_rows == 32 && !s.long_rows),
+          "batch %d: %d rows of a merge workgroup", n, s.merge_rows);
+    CHECK(s.merge_rows * s.merge_per_tile >= std::min<int64_t>((int64_t)max_q * group, tile_rows),
+          "batch %d: %lld merge workgroups of %d rows", n, (long long)s.merge_per_tile, s.merge_rows);
+    ++rows[s.merge_rows == 4 ? 0 : s.merge_rows == 16 ? 1 : 2];
+  }
+  // the run took every form
+  CHECK(eight > 100 && cut_calls > 1000 && rows[0] > 100 && rows[1] > 100 && rows[2] > 100,
+        "%lld of eight waves, %lld cut, merges of 4 / 16 / 32 rows: %lld %lld %lld", (long long)eight,
+        (long long)cut_calls, (long long)rows[0], (long long)rows[1], (long long)rows[2]);
+}
+
 int main() {
   ranges();
+  batches();
   std::printf("ok\n");
   return 0;
 }
