@@ -60,11 +60,13 @@ constexpr int kLongRows = 256, kLongSteps = 32;
 // (48 x 5 drafted tokens over 1000 each: 31 us, with 8 steps 35, with 2 still 31).
 constexpr int kLeastLong = 16, kLeastShort = 4;
 
-// False: more pieces than a grid.
+// False: more pieces than a grid.  (Heads of up to 65535 and rows of a sequence of up
+// to 2^30: no product passes 64 bits.)
 inline bool varlen_shape(int64_t cus, int32_t batch, int64_t total_q, int32_t max_q,
                          int32_t max_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                          VarlenShape* out) {
   const int64_t group = n_q_heads / n_kv_heads, max_rows = (int64_t)max_q * group;
+  total_q = std::min<int64_t>(total_q, INT32_MAX);  // (cu_seqlens end there)
   VarlenShape s{};
   // row tiles: those that the tokens fill, and a part-filled one per sequence
   auto jobs_of = [&](int64_t rows) {

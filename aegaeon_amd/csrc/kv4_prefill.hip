@@ -868,7 +868,7 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
       n_q_heads % n_kv_heads)
     return AEGKV_ERR_INVALID_ARG;
   if ((head_dim != 64 && head_dim != 128) ||
-      (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16))
+      (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16) || n_q_heads > 65535)
     return AEGKV_ERR_UNSUPPORTED;
   // in 32 bits: the rows of a sequence, a tile further; its keys, the end of a step of
   // two tiles and two tiles of loads ahead further

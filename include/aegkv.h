@@ -483,7 +483,8 @@ int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, cons
  *   workspace: DEVICE scratch of aegkv_kv4_varlen_attention_workspace_size(...)
  *     bytes (0: none) for the partials of sequences whose keys several
  *     workgroups share; used as aegkv_paged_decode_attention's.
- * head_dim 64 or 128, n_q_heads a multiple of n_kv_heads. */
+ * head_dim 64 or 128, n_q_heads a multiple of n_kv_heads and below 65536,
+ * max_seq_len below 2^31 - 256. */
 int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q,
                                                   int32_t max_seqlen_q, int32_t max_seq_len,
                                                   int32_t n_q_heads, int32_t n_kv_heads,

@@ -96,7 +96,29 @@ static void batches() {
         (long long)cut_calls, (long long)rows[0], (long long)rows[1], (long long)rows[2]);
 }
 
+// The largest arguments that the entry points let through: no product wraps, and a
+// grid that fits or a refusal.
+static void extremes() {
+  const int32_t big = INT32_MAX;
+  for (const int32_t batch : {1, 1000, big})
+    for (const int64_t total : {(int64_t)1, (int64_t)big, (int64_t)1 << 40, INT64_MAX})
+      for (const int32_t hkv : {1, 255, 65535})
+        for (const int32_t group : {1, 257, 65535})
+          for (const int32_t max_len : {0, 4096, big - 256})
+            for (const int32_t max_q : {1, 64, 4096, big / 2 / group}) {
+              if ((int64_t)hkv * group > 65535 || (int64_t)max_q * group > big / 2) continue;
+              for (const int dim : {64, 128}) {
+                VarlenShape s;
+                if (!varlen_shape(256, batch, total, max_q, max_len, hkv * group, hkv, dim, &s)) continue;
+                CHECK(s.pieces > 0 && s.pieces <= big / 2 && s.workspace() >= 0 && s.cut >= 0,
+                      "batch %d, %lld tokens, %d x %d heads: %lld pieces", batch, (long long)total, hkv,
+                      group, (long long)s.pieces);
+              }
+            }
+}
+
 int main() {
+  extremes();
   ranges();
   batches();
   std::printf("ok\n");

@@ -42,3 +42,11 @@ def test_several_queries_refuse_lengths_whose_last_step_passes_32_bits(lib):
     for longest in (2 ** 31 - 1, 2 ** 31 - 65, 2 ** 31 - 128, 2 ** 31 - 256):
         for new in (1, 20, 600):
             assert size(1, new, new, longest, 8, 2, 128, 0) == UNSUPPORTED
+
+
+def test_several_queries_refuse_head_counts_past_65535(lib):
+    """As the decode attention does: the row tiles of larger ones would pass 64 bits."""
+    size = lib.aegkv_kv4_varlen_attention_workspace_size
+    assert size(1, 1, 1, 64, 65536, 1, 128, 0) == UNSUPPORTED
+    assert size(1, 1, 1, 64, 1 << 20, 1 << 20, 128, 0) == UNSUPPORTED
+    assert size(2 ** 31 - 1, 2 ** 63 - 1, 1, 64, 2 ** 31 - 1, 2 ** 31 - 1, 128, 0) == UNSUPPORTED
