@@ -86,16 +86,21 @@ inline bool varlen_shape(int64_t cus, int32_t batch, int64_t total_q, int32_t ma
   s.least = s.long_rows ? kLeastLong : kLeastShort;
   // Workgroups that run at once.  With half as many row tiles or fewer, their keys
   // are cut into about as many pieces, but not more where a second round costs much:
-  // tiles of equal length into a whole number each, others into half a piece a tile
-  // less (2 x 256 queries over 4000, 112 tiles: 53 us, of as many pieces as places
-  // and more 66; of up to 64 rows the work is as uneven anyway: 48 x 5 over 1000, 192
-  // tiles: 26.9, so 28.4).  With more tiles only sequences of twice the average work
-  // of a place are cut, as partials cost more than an uneven last round (2048 queries
-  // over 16001 tokens, 224 tiles: whole 460 us, cut in two 498).  Four times as many
-  // tiles even out by themselves.
+  // a tile's ranges are rounded up, so 7/8 of a piece a tile less (2 x 256 queries
+  // over 4000, 112 tiles: 53 us, of as many pieces as places and more 66; of up to 64
+  // rows the work is as uneven anyway: 48 x 5 over 1000, 192 tiles: 26.9, so 28.4).
+  // Eight waves have their CU to themselves, and a second round of them costs a whole
+  // one: no more pieces a tile than go into the places as a whole number (1 x 448 over
+  // 16001, 28/4 heads, 52 tiles of four pieces: 132 us, of five 201; four waves, whose
+  // second round overlaps the first, take the piece more: 2 x 698 over 12000, 16/1
+  // heads of 64, 176 tiles of three 140, of two 161).  With more tiles only sequences
+  // of twice the average work of a place are cut, as partials cost more than an uneven
+  // last round (2048 queries over 16001 tokens, 224 tiles: whole 460 us, cut in two
+  // 498).  Four times as many tiles even out by themselves.
   const int64_t slots = cus * (s.long_rows ? 1 : 2);
   if (jobs < 4 * slots && max_kt > s.least) {
     s.target = jobs > slots / 2 ? slots / 2 : s.key_tiles > 1 ? slots : slots - jobs * 7 / 8;
+    if (s.long_rows && jobs <= slots / 2) s.target = std::min(s.target, slots / jobs * jobs);
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     s.cut = jobs;

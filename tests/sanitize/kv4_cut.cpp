@@ -96,6 +96,31 @@ static void batches() {
         (long long)cut_calls, (long long)rows[0], (long long)rows[1], (long long)rows[2]);
 }
 
+// Sequences of one length under eight waves: their pieces fit the CUs at once wherever
+// the row tiles do twice.
+static void equal_lengths() {
+  int64_t cut = 0;
+  for (const int cus : {256, 304, 80})
+    for (const int heads : {1, 2, 4, 8, 5})
+      for (const int group : {1, 7, 8, 20})
+        for (int batch = 1; batch <= 8; batch *= 2)
+          for (const int len : {700, 4000, 16000, 60000, 131072})
+            for (int m = 1; m <= 1200; m += m < 40 ? 1 : 7) {
+              VarlenShape s;
+              if (m > len ||
+                  !varlen_shape(cus, batch, (int64_t)batch * m, m, len, heads * group, heads, 128, &s))
+                continue;
+              const int64_t tiles = (int64_t)(m * group + 255) / 256 * heads * batch;
+              if (!s.long_rows || s.target == 0 || tiles > cus / 2) continue;
+              const int steps = (len + 63) / 64;
+              const int64_t pieces = tiles * ranges_of(steps, span_of(tiles * steps, s.target, s.least));
+              CHECK(pieces <= cus, "%d x %d queries over %d, %d x %d heads: %lld pieces of %lld tiles, "
+                    "%d CUs", batch, m, len, heads, group, (long long)pieces, (long long)tiles, cus);
+              cut += pieces > tiles;
+            }
+  CHECK(cut > 1000, "%lld cut", (long long)cut);
+}
+
 // The largest arguments that the entry points let through: no product wraps, and a
 // grid that fits or a refusal.
 static void extremes() {
@@ -118,6 +143,7 @@ static void extremes() {
 }
 
 int main() {
+  equal_lengths();
   extremes();
   ranges();
   batches();
