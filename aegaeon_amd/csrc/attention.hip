@@ -102,7 +102,8 @@ __device__ __forceinline__ int cost_units(int len) {
 // wave per SIMD.
 template <int D>
 constexpr int pipeline_depth() { return D >= 256 ? 2 : 3; }
-// Steps of the 4-bit cache in registers (of four blocks at D = 128: 17 KB a wave).
+// Register sets of the 4-bit cache, a step each (of four blocks at D = 128: 17 KB a
+// wave).
 constexpr int kKv4PipelineDepth = 2;
 
 // kv heads of a workgroup's group, one per wave; the 4 / heads waves of each
@@ -524,12 +525,14 @@ __device__ __forceinline__ void compute_block(KVRegs<D>& r, const u32x4* qv, f32
 }
 
 // ---- the 4-bit cache (kv4_format.h) ----
-// Bound by the cache's bytes, 17 D / 16 per token and kv head, as long as the
-// instructions per block stay under their loads: one layer of 128 sequences of
-// 1500 tokens on average (28/4 heads, D = 128, 105 MB) 33.1 us, 29.8 when the
-// loads alone are issued; 32 x 2048 of 40/40 heads (357 MB) 63.2 us, 5.7 TB/s, and
-// 63.  One workgroup per CU, two steps ahead: two per CU take 36.4 and 65.7 us,
-// three steps in registers are slower as well.
+// Bound by the cache's bytes, 17 D / 16 per token and kv head, where waves have many
+// blocks: 32 x 2048 of 40/40 heads (357 MB) 63.2 us, 5.7 TB/s, and 63 when the loads
+// alone are issued.  With few, by the chain of a step's loads, whose block ids are
+// asked for one step before: one layer of 128 sequences of 1500 tokens on average
+// (28/4 heads, D = 128, 105 MB, 46 blocks a wave) 33.1 us, 29.8 for the loads with
+// that chain, 20.4 at a large copy's rate.  One workgroup per CU and two register
+// sets, so one step in flight during a step's compute: two workgroups per CU take
+// 36.4 and 65.7 us, three sets are slower as well.
 // K and V are converted to 16 bits, where code times scale is exact, so nothing
 // past the conversion differs from the 16-bit cache's arithmetic.  Per block of
 // 16 tokens, with lane l = 16 g + j:
@@ -1240,9 +1243,9 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
 }
 
 // attend_items over the 4-bit cache: the same items, ids, pieces and records,
-// in steps of up to step4() blocks that end where a piece does.  The step that
-// is loaded is NSET - 1 steps ahead of the one computed, across sequences: the
-// load side keeps a sequence position of its own, and hands a step's to the
+// in steps of up to step4() blocks that end where a piece does.  During a step's
+// compute the next NSET - 1 are in flight, across sequences, and its registers are
+// loaded again behind it: the load side keeps a sequence position of its own, and hands a step's to the
 // compute side with its registers.  Past the range a step loads nothing (empty
 // buffer ranges) and is not computed.
 template <int DT, int D, int NSET, int PACK, bool PLANNED>

@@ -53,8 +53,8 @@ struct VarlenShape {
 // Shorter or more numerous tiles do better with two workgroups per CU, which
 // overlap one's start and end with the other's steps (4 x 64 over 4000 51 and 40,
 // 18 x 128 over 1000 83 and 54, 48 prompts of 220 tokens 93 and 71), and so does
-// head_dim 64 always, whose steps are mostly softmax (8/8, 14 x 512 over 8000: 229
-// and 207, 16/1, 24 x 512 over 2000: 217 and 148).
+// head_dim 64 always (8/8, 14 x 512 over 8000: 229 and 207, 16/1, 24 x 512 over 2000:
+// 217 and 148).
 constexpr int kLongRows = 256, kLongSteps = 32;
 // A piece's key steps at least: its partials cost about what half of these do
 // (48 x 5 drafted tokens over 1000 each: 31 us, with 8 steps 35, with 2 still 31).
@@ -105,9 +105,14 @@ inline bool varlen_shape(int64_t cus, int32_t batch, int64_t total_q, int32_t ma
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
     s.cut = jobs;
     auto per_tile = [&](int64_t r) { return (std::min(max_rows, tile_rows) + r - 1) / r; };
-    // Rows of a merge workgroup: 4 where a tile has many pieces (a query over 60000,
-    // 128 pieces: 27.3 us, of 16 rows 41.3), 16 where it has few (4 x 128 over 3000:
-    // 53.9, of 4 rows 57.4), 32 where there are many tiles, most of them uncut.
+    // Rows of a merge workgroup.  4 where a tile has 16 pieces or more (28/4 heads over
+    // 16000 tokens, us with 4 and with 16 rows: 2 / 4 / 8 / 12 / 16 x 4 queries, of 64,
+    // 32, 16, 11, 8 pieces a tile, 21.3 and 24.5, 25.2 and 28.3, 33.4 and 34.6, 55.7 and
+    // 56.2, 51.4 and 50.9; 2 / 4 / 8 / 12 x 16, of 63, 31, 15, 10: 31.3 and 38.4, 39.3
+    // and 40.0, 54.5 and 53.6, 71.0 and 69.3), 16 where it has fewer, 32 where those
+    // would be more than 4096 workgroups, of tiles mostly uncut (16 and 32 rows: 100 x 64
+    // over 1500 on average, 12800: 227 and 225; 400 x 9 over 1000, 6400: 144 and 141;
+    // 256 x 9, 4096: 91.3 and 91.5).
     s.merge_rows = s.target >= 16 * jobs ? 4
                    : s.long_rows || jobs * per_tile(16) <= 4096 ? 16 : 32;
     s.merge_per_tile = per_tile(s.merge_rows);

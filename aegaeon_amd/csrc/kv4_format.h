@@ -35,7 +35,6 @@ namespace aegkv {
 
 constexpr int kKv4Group = 32;        // dims per scale
 constexpr int kKv4Tokens = 16;       // tokens per block
-constexpr int kKv4ScaleBias = 127;
 constexpr int kKv4ScaleMin = 2;      // e = -125
 constexpr uint32_t kKv4ScaleNan = 255;
 
