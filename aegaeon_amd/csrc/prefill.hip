@@ -15,7 +15,7 @@
 //     16 of the 32 keys of a block (keys 8(i/4) + 4(l/32) + i%4 of
 //     accumulator element i), its partner lane l ^ 32 the other 16;
 //   O^T[D x 32] += V^T[D x 64] . P^T[64 x 32]             D/32 x 4 MFMA 32x32x16
-//     with P rounded to 16 bits (as FlashAttention does) and taken straight
+//     with P rounded to 16 bits (PfOps::kTop) and taken straight
 //     from the S^T accumulators: elements 8j .. 8j+7 of a lane are the keys of
 //     k-step j, which are keys {4 hh .. 4 hh + 3, 8 + 4 hh .. 8 + 4 hh + 3} of
 //     the step's 16 (hh = l / 32), so V^T's A operand holds those keys.
