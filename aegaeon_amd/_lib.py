@@ -122,6 +122,26 @@ SIGNATURES: Dict[str, tuple] = {
                                            c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
                                            c_float, c_int32, c_int32, c_void_p, c_uint64,
                                            c_void_p]),
+    # append with the position rotation
+    "aegkv_rotary_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                                    c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                    c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                    c_int32, c_int32, c_void_p, c_void_p, c_int64, c_int64,
+                                    c_int32, c_int32, c_void_p]),
+    # the 8-bit cache
+    "aegkv_kv8_block_bytes": (c_int64, [c_int32, c_int32]),
+    "aegkv_kv8_append": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                 c_int64, c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32,
+                                 c_int32, c_int32, c_void_p]),
+    "aegkv_kv8_rotary_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                                        c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32,
+                                        c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                        c_int32, c_int32, c_void_p, c_int64, c_int64, c_int32,
+                                        c_void_p]),
+    "aegkv_kv8_gather_tokens": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32,
+                                        c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                                        c_int64, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                        c_void_p]),
     # block manager (host bookkeeping)
     "aegkv_bm_create": (c_int, [c_int64, c_int64, POINTER(c_void_p)]),
     "aegkv_bm_destroy": (None, [c_void_p]),

@@ -1,0 +1,686 @@
+// Writing and de-paging the 8-bit KV cache (kv8_format.h) on gfx950:
+//  - kv8_append: slot-mapped write of new 16-bit K/V rows, one layer or every
+//    layer of a step in one launch, or one layer's rows turned by their positions
+//    on the way, with the queries turned beside them (rotary_rows.h);
+//  - kv8_gather: block-table-driven de-page of sequences into contiguous 16-bit
+//    [sum(len), Hkv, D] buffers.
+// A wave takes one block of one head and side, a lane the 8 dims 8 c .. of the
+// tokens 4 g .. 4 g + 3 (lane = 16 g + c; D = 64: c < 8; D = 256: and dims 128
+// further): a block's maximum is a reduction within the wave, and V's words, four
+// tokens of a dim, come together in one lane's registers.
+#include <algorithm>
+
+#include "aegkv_internal.h"
+#include "kv8_format.h"
+#include "rotary_rows.h"
+#include "wave_scan.h"
+
+namespace aegkv {
+namespace {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kAppend8Threads = 256;
+// How a call turns its keys and queries: not at all, pairs half a row apart, neighbours.
+constexpr int kStill = 0, kHalves = 1, kNeighbours = 2;
+
+struct Append8Args {
+  HeadRows k, v;             // sources (dst unused)
+  int64_t k_layer_b, v_layer_b;
+  const int64_t* slots;
+  uint8_t* cache;
+  int64_t blk_b, layer_b;    // cache byte strides
+  int64_t n_slots;           // n_blocks * 16
+  int64_t scales_at;         // kv8_scales_at
+  uint32_t n_tokens, n_heads;
+  uint32_t window;           // tokens whose runs a wave takes, 1 .. 16
+  uint32_t n_windows;
+  uint32_t n_waves;          // that write the cache: layers * windows * heads * 2
+  // a rotating call (q.src != nullptr): then the tasks of the queries, and of the
+  // keys to out_key
+  RotaryTable r;
+  HeadRows q, ok;
+  uint32_t q_tasks, ok_tasks;  // per token
+  uint32_t n_tasks;            // waves in all
+};
+
+// The largest of the wave's values, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));  // row_ror 4
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));  // row_ror 8
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max(b[0], b[1]);
+}
+
+// Four floats to a word of codes.  clamp: |x| may exceed 448 only where the exponent
+// is held at its top; NaN stays NaN (the comparisons keep it).
+__device__ __forceinline__ float code_range(float x) {
+  x = x > kKv8Largest ? kKv8Largest : x;
+  return x < -kKv8Largest ? -kKv8Largest : x;
+}
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(code_range(a), code_range(b), 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(code_range(c), code_range(d), w, true);
+  return (uint32_t)w;
+}
+__device__ __forceinline__ void floats4(uint32_t w, float (&f)[4]) {
+  const f32x2 a = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false));
+  const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true));
+  f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
+}
+// infinities to NaN (magnitude bits `u`)
+__device__ __forceinline__ float not_infinite(float x, uint32_t u) {
+  return u >= 0x7f800000u ? __builtin_nanf("") : x;
+}
+
+// One run: the tokens of lanes i .. i + n - 1 of the window, all of block blk.
+// src[k]: the lane of the window whose token goes to place 4 g + k (-1: none).
+template <int DT, int D, int TURN>
+__device__ __forceinline__ void append_run(const Append8Args& a, uint32_t layer, uint32_t head,
+                                           bool value, int64_t tok_at_lane0, int64_t blk,
+                                           const int (&src)[4], bool anew) {
+  constexpr int NC = D > 128 ? D / 128 : 1;  // chunks of a lane
+  constexpr bool INTER = TURN == kNeighbours;
+  const int lane = threadIdx.x & 63, g = lane >> 4, c0 = lane & 15;
+  const bool idle = D < 128 && c0 >= D / 8;
+  const HeadRows& h = value ? a.v : a.k;
+  const uint8_t* rows = h.src + layer * (value ? a.v_layer_b : a.k_layer_b) + (int64_t)head * D * 2;
+  uint8_t* rec = a.cache + blk * a.blk_b + layer * a.layer_b;
+  uint8_t* scale = rec + a.scales_at + 4 * head;
+  rec += (int64_t)(2 * head + (value ? 1 : 0)) * kv8_side_bytes(D);
+  int old = Kv8Elem<DT>::kLow;
+  if (!anew) old = scale[value ? 1 : 0];
+  float f[NC][4][8];
+  uint32_t top = 0;
+  bool bad = false;
+#pragma unroll
+  for (int q = 0; q < NC; ++q) {
+    const int c = c0 + 16 * q;
+    u32x4 x[4], y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = y[k] = u32x4{0u, 0u, 0u, 0u};
+      if (src[k] >= 0 && !idle) {
+        const uint8_t* p = rows + (tok_at_lane0 + src[k]) * h.src_tok_b;
+        x[k] = *reinterpret_cast<const u32x4*>(p + 16 * c);
+        if (TURN != kStill && !value && chunk_turns(a.r, c))
+          y[k] = *reinterpret_cast<const u32x4*>(p + 16 * partner_chunk<INTER>(a.r, c));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      bool turned = false;
+      if constexpr (TURN != kStill) {
+        if (src[k] >= 0 && !idle && !value && chunk_turns(a.r, c)) {
+          turn_chunk<DT, INTER>(
+              x[k], y[k], load_angles<INTER>(a.r, a.r.positions[tok_at_lane0 + src[k]], c),
+              f[q][k]);
+          turned = true;
+        }
+      }
+      if (!turned) unpack8<DT>(x[k], f[q][k]);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const uint32_t u = __float_as_uint(f[q][k][d]) & 0x7fffffffu;
+        bad |= u >= 0x7f800000u;
+        top = max(top, u >= 0x7f800000u ? 0u : u);
+        f[q][k][d] = not_infinite(f[q][k][d], u);
+      }
+    }
+  }
+  top = wave_max(top);
+  const bool nan = __builtin_amdgcn_ballot_w64(bad) != 0;
+  const int held = __builtin_amdgcn_readfirstlane(old);  // (0 in a cache never written)
+  old = min(max(held, Kv8Elem<DT>::kLow), Kv8Elem<DT>::kTop);
+  const int own = kv8_scale_byte<DT>(top);
+  const int now = anew ? own : max(old, own);
+  const float inv = kv8_scale((uint32_t)(254 - now));  // 2^-e
+  const bool rescale = !anew && now > old;             // uniform
+  const float down = kv8_scale((uint32_t)max(127 + old - now, 0));
+  if (!idle) {
+#pragma unroll
+    for (int q = 0; q < NC; ++q) {
+      const int c = c0 + 16 * q;
+      // new codes, of places without a new token 0
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) f[q][k][d] *= inv;
+      if (!value) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          u32x2* p = reinterpret_cast<u32x2*>(rec + kv8_k_byte(4 * g + k, c));
+          u32x2 w = {codes4(f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3]),
+                     codes4(f[q][k][4], f[q][k][5], f[q][k][6], f[q][k][7])};
+          if (rescale && src[k] < 0) {
+            const u32x2 o = *p;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float t[4];
+              floats4(o[i], t);
+              w[i] = codes4(t[0] * down, t[1] * down, t[2] * down, t[3] * down);
+            }
+          }
+          if (anew || rescale || src[k] >= 0) *p = w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint8_t* p = rec + kv8_v_byte<D>(g, 2 * c + i);
+          u32x4 w;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            w[d] = codes4(f[q][0][4 * i + d], f[q][1][4 * i + d], f[q][2][4 * i + d],
+                          f[q][3][4 * i + d]);
+          if (rescale) {
+            const u32x4 o = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              float t[4];
+              floats4(o[d], t);
+              const uint32_t r = codes4(t[0] * down, t[1] * down, t[2] * down, t[3] * down);
+              uint32_t mine = 0;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mine |= src[k] >= 0 ? 0xffu << (8 * k) : 0u;
+              w[d] = (w[d] & mine) | (r & ~mine);
+            }
+          }
+          if (anew || rescale || (src[0] >= 0 && src[1] >= 0 && src[2] >= 0 && src[3] >= 0)) {
+            *reinterpret_cast<u32x4*>(p) = w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (src[k] >= 0) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) p[4 * d + k] = (uint8_t)(w[d] >> (8 * k));
+              }
+          }
+        }
+      }
+    }
+  }
+  if (lane == 0) {
+    if (anew || now != held) scale[value ? 1 : 0] = (uint8_t)now;
+    if (value && (anew || nan)) scale[2] = nan ? 1 : 0;
+  }
+}
+
+// A wave of the cache's writers: a head and side of the runs that begin in its
+// window of tokens.  A run is tokens next to each other in the call whose slots lie
+// in one block.
+template <int DT, int D, int TURN>
+__device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id) {
+  const bool value = id & 1;
+  uint32_t rest = id >> 1;
+  const uint32_t head = rest % a.n_heads;
+  rest /= a.n_heads;
+  const uint32_t win = rest % a.n_windows, layer = rest / a.n_windows;
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  // lane i: token `first` + i, the one before the window in lane 0
+  const int64_t first = (int64_t)win * a.window - 1, tok = first + lane;
+  int64_t s = -1;
+  if (tok >= 0 && tok < a.n_tokens) s = a.slots[tok];
+  const bool in = s >= 0 && s < a.n_slots;
+  const int blk = in ? (int)(s / kKv8Tokens) : -1, off = (int)(s & (kKv8Tokens - 1));
+  const int before = __shfl_up(blk, 1);
+  uint64_t heads = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= (int)a.window && in &&
+                                               blk != before);
+  while (heads) {  // uniform
+    const int i = __builtin_ctzll(heads);
+    heads &= heads - 1;
+    const int b = __builtin_amdgcn_readlane(blk, i);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(blk == b) >> i;
+    const int n = ~same ? __builtin_ctzll(~same) : 64;  // tokens of the run (i > 0: below 64)
+    const int off0 = __builtin_amdgcn_readlane(off, i);
+    int src[4];
+    bool anew;
+    const uint64_t run = n < 64 ? (1ull << n) - 1 : ~0ull;
+    const uint64_t in_order = __builtin_amdgcn_ballot_w64(off == off0 + lane - i) >> i;
+    if ((in_order & run) == run) {  // one place after the other
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 4 * g + k - off0;
+        src[k] = r >= 0 && r < n ? i + r : -1;
+      }
+      anew = off0 == 0;
+    } else {  // of two tokens for one place the later one
+#pragma unroll
+      for (int k = 0; k < 4; ++k) src[k] = -1;
+      anew = false;
+      for (int x = i; x < i + n; ++x) {
+        const int o = __builtin_amdgcn_readlane(off, x);
+        anew |= o == 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) src[k] = o == 4 * g + k ? x : src[k];
+      }
+    }
+    append_run<DT, D, TURN>(a, layer, head, value, first, b, src, anew);
+  }
+}
+
+template <int DT, int D, int TURN>
+__global__ __launch_bounds__(kAppend8Threads) void kv8_append_kernel(Append8Args a) {
+  uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (kAppend8Threads / 64) +
+                                               (threadIdx.x >> 6));
+  if (id >= a.n_tasks) return;
+  if (id < a.n_waves) {
+    append_window<DT, D, TURN>(a, id);
+    return;
+  }
+  if constexpr (TURN != kStill) {
+    id -= a.n_waves;
+    const uint32_t per = a.q_tasks + a.ok_tasks, tok = id / per;
+    const int part = (int)(id - tok * per);
+    if (part < (int)a.q_tasks)
+      turn_heads<DT, TURN == kNeighbours>(a.q, a.r, true, (int)tok, part, D / 8, nullptr);
+    else
+      turn_heads<DT, TURN == kNeighbours>(a.ok, a.r, true, (int)tok, part - (int)a.q_tasks, D / 8, nullptr);
+  }
+}
+
+// De-page: a tile is one block of one sequence in a pass of 8 / (head, side) units,
+// two per wave.  Each workgroup scans the batch's block counts into LDS and walks
+// its layer's tiles round-robin; the next tile's block id and output row are fetched
+// while the current one's loads are in flight.
+constexpr int kGather8Threads = 256;
+constexpr int kGather8MaxBatch = 1024;  // sequences per launch (LDS scan)
+constexpr int kGather8PerWave = 2;      // units of a wave in a tile (D = 64: twice that)
+constexpr int kGather8WorkgroupsPerCu = 16;
+
+struct Gather8Args {
+  const uint8_t* cache;
+  int64_t blk_b, layer_b, scales_at;
+  int64_t n_blocks;
+  const int32_t* block_tables;
+  int32_t max_blocks;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens;
+  uint8_t* out_k;
+  uint8_t* out_v;
+  int64_t out_tokens;   // capacity of the output in tokens
+  int64_t out_layer_b;
+  int32_t max_seq_len;
+  int32_t batch;        // <= kGather8MaxBatch
+  int32_t n_heads;
+  int32_t passes;       // of a block
+};
+
+// The 8 dims of chunk c of tokens 4 g + k of K: eight bytes of each token.
+__device__ __forceinline__ void load_k8(const uint8_t* side, int g, int c, u32x2 (&w)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    w[k] = *reinterpret_cast<const u32x2*>(side + kv8_k_byte(4 * g + k, c));
+}
+// Those of V, from words of one dim and four tokens.
+template <int D>
+__device__ __forceinline__ void load_v8(const uint8_t* side, int g, int c, u32x4 (&w)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = *reinterpret_cast<const u32x4*>(side + kv8_v_byte<D>(g, 2 * c + i));
+}
+__device__ __forceinline__ void by_token(const u32x4 (&w)[2], u32x2 (&t)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // (a.0 b.0 a.1 b.1) of two dims, then of four
+    const uint32_t a = __builtin_amdgcn_perm(w[i][1], w[i][0], 0x05010400u);
+    const uint32_t b = __builtin_amdgcn_perm(w[i][1], w[i][0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[i][3], w[i][2], 0x05010400u);
+    const uint32_t d = __builtin_amdgcn_perm(w[i][3], w[i][2], 0x07030602u);
+    t[0][i] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    t[1][i] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    t[2][i] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    t[3][i] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+  }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(kGather8Threads) void kv8_gather_kernel(Gather8Args a) {
+  using E = Kv8Elem<DT>;
+  __shared__ int32_t pre[kGather8MaxBatch + 1];  // first block of each sequence
+  __shared__ int32_t lens[kGather8MaxBatch];
+  __shared__ int32_t wsum[kGather8Threads / 64];
+  constexpr int PER = kGather8MaxBatch / kGather8Threads;
+  const int t = threadIdx.x, B = a.batch;
+  int cnt[PER], run = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {  // loads issued together, clamped in bounds
+    const int b = t * PER + k;
+    const int raw = a.seq_lens[min(b, B - 1)];
+    const int len = b < B ? min(max(raw, 0), a.max_seq_len) : 0;
+    if (b < B) lens[b] = len;
+    cnt[k] = (len + kKv8Tokens - 1) / kKv8Tokens;
+    run += cnt[k];
+  }
+  const int incl = wave_prefix(run);
+  if ((t & 63) == 63) wsum[t >> 6] = incl;
+  __syncthreads();
+  int excl = incl - run;
+  for (int w = 0; w < (t >> 6); ++w) excl += wsum[w];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int b = t * PER + k;
+    if (b <= B) pre[b] = excl;
+    excl += cnt[k];
+  }
+  if (t == kGather8Threads - 1) pre[B] = excl;  // total (B may equal the capacity)
+  __syncthreads();
+  const uint32_t total = (uint32_t)pre[B] * a.passes;
+  uint32_t at = blockIdx.x;
+  if (at >= total) return;  // uniform
+
+  auto locate = [&](uint32_t x, int& b, int& j, int& ps) {
+    const int r = (int)(x / (uint32_t)a.passes);
+    ps = (int)(x - (uint32_t)r * a.passes);
+    int lo = 0, hi = B - 1;  // the last sequence whose first block is <= r
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pre[mid] <= r) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    j = r - pre[lo];
+  };
+  // a wave's units: D = 64 two at once, of 32 lanes each; D = 256 in two halves
+  constexpr int UW = D == 64 ? 2 : 1, NC = D == 256 ? 2 : 1, LC = D == 64 ? 8 : 16;
+  const int lane = t & 63, wave = t >> 6;
+  const int g = lane / LC & 3, c0 = lane % LC, sub = D == 64 ? lane >> 5 : 0;
+  const int64_t row_b = (int64_t)a.n_heads * D * 2;
+  const int layer = (int)blockIdx.y;
+  int b, j, ps;
+  locate(at, b, j, ps);
+  int32_t id = a.block_tables[(int64_t)b * a.max_blocks + j];
+  int64_t row0 = a.cu_seqlens[b];
+  while (true) {
+    const int64_t row = row0 + (int64_t)j * kKv8Tokens;
+    int n_tok = min(kKv8Tokens, lens[b] - j * kKv8Tokens);
+    if (row < 0 || row >= a.out_tokens || id < 0 || id >= a.n_blocks) n_tok = 0;
+    else n_tok = (int)min((int64_t)n_tok, a.out_tokens - row);
+    const uint8_t* blk = a.cache + (int64_t)max(id, 0) * a.blk_b + layer * a.layer_b;
+    u32x2 kw[kGather8PerWave][NC][4];
+    u32x4 vw[kGather8PerWave][NC][2];
+    uint32_t sb[kGather8PerWave];
+    bool have[kGather8PerWave];
+    int unit[kGather8PerWave];
+#pragma unroll
+    for (int u = 0; u < kGather8PerWave; ++u) {
+      // units: K of every head, then V of every head; a wave's follow each other
+      const int x = ((ps * (kGather8Threads / 64) + wave) * kGather8PerWave + u) * UW + sub;
+      unit[u] = x;
+      have[u] = x < 2 * a.n_heads && 4 * g < n_tok;
+      sb[u] = 0;
+      if (have[u]) {
+        const bool value = x >= a.n_heads;
+        const int head = value ? x - a.n_heads : x;
+        const uint8_t* side = blk + (int64_t)(2 * head + (value ? 1 : 0)) * kv8_side_bytes(D);
+        sb[u] = blk[a.scales_at + 4 * head + (value ? 1 : 0)];
+#pragma unroll
+        for (int q = 0; q < NC; ++q) {
+          if (value) load_v8<D>(side, g, c0 + 16 * q, vw[u][q]);
+          else load_k8(side, g, c0 + 16 * q, kw[u][q]);
+        }
+      }
+    }
+    const uint32_t an = at + gridDim.x;
+    const bool more = an < total;
+    int nb, nj, nps;
+    locate(more ? an : at, nb, nj, nps);
+    const int32_t nid = a.block_tables[(int64_t)nb * a.max_blocks + nj];
+    const int64_t nrow0 = a.cu_seqlens[nb];
+#pragma unroll
+    for (int u = 0; u < kGather8PerWave; ++u) {
+      if (!have[u]) continue;
+      const bool value = unit[u] >= a.n_heads;
+      const int head = value ? unit[u] - a.n_heads : unit[u];
+      const float s = kv8_scale(sb[u]);
+      uint8_t* out = (value ? a.out_v : a.out_k) + layer * a.out_layer_b + (row + 4 * g) * row_b +
+                     (int64_t)head * D * 2;
+#pragma unroll
+      for (int q = 0; q < NC; ++q) {
+        u32x2 w[4];
+        if (value) {
+          by_token(vw[u][q], w);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = kw[u][q][k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const u32x4 x = {E::template dq<false>(w[k][0], s), E::template dq<true>(w[k][0], s),
+                           E::template dq<false>(w[k][1], s), E::template dq<true>(w[k][1], s)};
+          if (4 * g + k < n_tok)
+            __builtin_nontemporal_store(
+                x, reinterpret_cast<u32x4*>(out + k * row_b + 16 * (c0 + 16 * q)));
+        }
+      }
+    }
+    if (!more) break;
+    at = an;
+    b = nb;
+    j = nj;
+    ps = nps;
+    id = nid;
+    row0 = nrow0;
+  }
+}
+
+bool head_dim_ok(int32_t d) { return d == 64 || d == 128 || d == 256; }
+bool dtype_ok(int32_t t) { return t == AEGKV_DTYPE_BF16 || t == AEGKV_DTYPE_FP16; }
+
+template <int DT, int TURN>
+void launch_append(const Append8Args& a, int32_t head_dim, hipStream_t st) {
+  constexpr uint32_t kWavesOf = kAppend8Threads / 64;
+  const dim3 g((a.n_tasks + kWavesOf - 1) / kWavesOf), t(kAppend8Threads);
+  if (head_dim == 64) hipLaunchKernelGGL((kv8_append_kernel<DT, 64, TURN>), g, t, 0, st, a);
+  else if (head_dim == 128) hipLaunchKernelGGL((kv8_append_kernel<DT, 128, TURN>), g, t, 0, st, a);
+  else hipLaunchKernelGGL((kv8_append_kernel<DT, 256, TURN>), g, t, 0, st, a);
+}
+template <int DT>
+void launch_gather(const Gather8Args& a, int32_t head_dim, dim3 g, hipStream_t st) {
+  const dim3 t(kGather8Threads);
+  if (head_dim == 64) hipLaunchKernelGGL((kv8_gather_kernel<DT, 64>), g, t, 0, st, a);
+  else if (head_dim == 128) hipLaunchKernelGGL((kv8_gather_kernel<DT, 128>), g, t, 0, st, a);
+  else hipLaunchKernelGGL((kv8_gather_kernel<DT, 256>), g, t, 0, st, a);
+}
+
+// Tokens of a wave's window.  A wave looks for the runs that begin there and writes
+// them one after the other, so 1 is best while the waves fit the chip; of a prompt,
+// 15 of 16 tokens begin none.
+constexpr uint64_t kAppend8Waves = 16384;
+uint32_t window_of(uint64_t waves_of_one) {
+  uint32_t w = 1;
+  while (w < 16 && waves_of_one > kAppend8Waves * w) w *= 2;
+  return w;
+}
+
+// The part of a call that both appends share: checks of the cache and the rows, and
+// the waves that write.  (1: nothing to do)
+int append_args(Append8Args& a, const void* key, const void* value, int64_t key_token_stride,
+                int64_t value_token_stride, int64_t key_layer_stride, int64_t value_layer_stride,
+                const int64_t* slot_mapping, int64_t n_tokens, void* cache,
+                int64_t cache_block_stride, int64_t cache_layer_stride, int64_t n_blocks,
+                int32_t n_layers, int32_t n_kv_heads, int32_t head_dim, int32_t dtype) {
+  if (n_tokens < 0 || n_layers <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_blocks < 0)
+    return AEGKV_ERR_INVALID_ARG;
+  if (!head_dim_ok(head_dim) || !dtype_ok(dtype) || n_kv_heads > kKv8MaxHeads ||
+      n_blocks > INT32_MAX)
+    return AEGKV_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return AEGKV_OK;
+  if (!key || !value || !slot_mapping || (!cache && n_blocks > 0)) return AEGKV_ERR_INVALID_ARG;
+  if (!aligned16(key) || !aligned16(value) || !aligned16(cache) || key_token_stride % 8 ||
+      value_token_stride % 8 || key_layer_stride % 8 || value_layer_stride % 8 ||
+      cache_block_stride % 16 || cache_layer_stride % 16)
+    return AEGKV_ERR_MISALIGNED;
+  // waves of windows of one token, counted in 128 bits so that no product wraps
+  const unsigned __int128 waves = (unsigned __int128)(uint64_t)n_layers * 2 *
+                                  (uint64_t)n_kv_heads * (uint64_t)n_tokens;
+  if (n_tokens > INT32_MAX || waves > INT32_MAX) return AEGKV_ERR_UNSUPPORTED;
+  a.k = HeadRows{static_cast<const uint8_t*>(key), nullptr, key_token_stride * 2, 0, n_kv_heads};
+  a.v = HeadRows{static_cast<const uint8_t*>(value), nullptr, value_token_stride * 2, 0,
+                 n_kv_heads};
+  a.k_layer_b = key_layer_stride * 2;
+  a.v_layer_b = value_layer_stride * 2;
+  a.slots = slot_mapping;
+  a.cache = static_cast<uint8_t*>(cache);
+  a.blk_b = cache_block_stride;
+  a.layer_b = cache_layer_stride;
+  a.n_slots = n_blocks * kKv8Tokens;
+  a.scales_at = kv8_scales_at(n_kv_heads, head_dim);
+  a.n_tokens = (uint32_t)n_tokens;
+  a.n_heads = (uint32_t)n_kv_heads;
+  a.window = window_of((uint64_t)waves);
+  a.n_windows = (a.n_tokens + a.window - 1) / a.window;
+  a.n_waves = n_blocks > 0 ? (uint32_t)n_layers * 2 * a.n_heads * a.n_windows : 0;
+  a.r = RotaryTable{};
+  a.q = a.ok = HeadRows{};
+  a.q_tasks = a.ok_tasks = 0;
+  a.n_tasks = a.n_waves;
+  return AEGKV_OK;
+}
+
+}  // namespace
+}  // namespace aegkv
+
+using namespace aegkv;
+
+extern "C" {
+
+int64_t aegkv_kv8_block_bytes(int32_t n_kv_heads, int32_t head_dim) {
+  if (n_kv_heads <= 0) return AEGKV_ERR_INVALID_ARG;
+  if (!head_dim_ok(head_dim) || n_kv_heads > kKv8MaxHeads) return AEGKV_ERR_UNSUPPORTED;
+  return kv8_layer_bytes(n_kv_heads, head_dim);
+}
+
+int aegkv_kv8_append(const void* key, const void* value, int64_t key_token_stride,
+                     int64_t value_token_stride, int64_t key_layer_stride,
+                     int64_t value_layer_stride, const int64_t* slot_mapping, int64_t n_tokens,
+                     void* cache, int64_t cache_block_stride, int64_t cache_layer_stride,
+                     int64_t n_blocks, int32_t n_layers, int32_t n_kv_heads, int32_t head_dim,
+                     int32_t dtype, aegkv_stream_t stream) {
+  Append8Args a{};
+  const int rc = append_args(a, key, value, key_token_stride, value_token_stride, key_layer_stride,
+                             value_layer_stride, slot_mapping, n_tokens, cache, cache_block_stride,
+                             cache_layer_stride, n_blocks, n_layers, n_kv_heads, head_dim, dtype);
+  if (rc) return rc;
+  if (a.n_tasks == 0) return AEGKV_OK;
+  if (dtype == AEGKV_DTYPE_BF16)
+    launch_append<AEGKV_DTYPE_BF16, kStill>(a, head_dim, (hipStream_t)stream);
+  else
+    launch_append<AEGKV_DTYPE_FP16, kStill>(a, head_dim, (hipStream_t)stream);
+  AEGKV_HIP_TRY(hipGetLastError());
+  return AEGKV_OK;
+}
+
+int aegkv_kv8_rotary_append(const void* query, int64_t query_token_stride, void* out_query,
+                            int64_t out_query_token_stride, int32_t n_q_heads, const void* key,
+                            int64_t key_token_stride, const void* value,
+                            int64_t value_token_stride, void* out_key,
+                            int64_t out_key_token_stride, int32_t n_kv_heads, int32_t head_dim,
+                            const int64_t* slot_mapping, const int64_t* positions,
+                            int64_t n_tokens, const float* table, int64_t max_positions,
+                            int32_t rotary_dim, int32_t interleaved, void* cache,
+                            int64_t cache_block_stride, int64_t n_blocks, int32_t dtype,
+                            aegkv_stream_t stream) {
+  Append8Args a{};
+  int rc = append_args(a, key, value, key_token_stride, value_token_stride, 0, 0, slot_mapping,
+                       n_tokens, cache, cache_block_stride, 0, n_blocks, 1, n_kv_heads, head_dim,
+                       dtype);
+  if (rc) return rc;
+  if (n_q_heads <= 0) return AEGKV_ERR_INVALID_ARG;
+  a.r = RotaryTable{table, positions, max_positions, rotary_dim};
+  rc = check_rotary(a.r, head_dim);
+  if (rc) return rc;
+  if (n_q_heads > 65535) return AEGKV_ERR_UNSUPPORTED;
+  if (n_tokens == 0) return AEGKV_OK;
+  if (!query || !out_query || !positions || !table || max_positions == 0)
+    return AEGKV_ERR_INVALID_ARG;
+  if (!aligned16(query) || !aligned16(out_query) || !aligned16(out_key) || !aligned16(table) ||
+      query_token_stride % 8 || out_query_token_stride % 8 || out_key_token_stride % 8)
+    return AEGKV_ERR_MISALIGNED;
+  a.q = HeadRows{static_cast<const uint8_t*>(query), static_cast<uint8_t*>(out_query),
+                 query_token_stride * 2, out_query_token_stride * 2, n_q_heads};
+  a.ok = HeadRows{a.k.src, static_cast<uint8_t*>(out_key), a.k.src_tok_b,
+                  out_key_token_stride * 2, n_kv_heads};
+  a.q_tasks = (uint32_t)head_tasks(n_q_heads, head_dim / 8);
+  a.ok_tasks = out_key ? (uint32_t)head_tasks(n_kv_heads, head_dim / 8) : 0;
+  const uint64_t tasks = a.n_waves + (uint64_t)n_tokens * (a.q_tasks + a.ok_tasks);
+  if (tasks > INT32_MAX) return AEGKV_ERR_UNSUPPORTED;
+  a.n_tasks = (uint32_t)tasks;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == AEGKV_DTYPE_BF16)
+    interleaved ? launch_append<AEGKV_DTYPE_BF16, kNeighbours>(a, head_dim, st)
+                : launch_append<AEGKV_DTYPE_BF16, kHalves>(a, head_dim, st);
+  else
+    interleaved ? launch_append<AEGKV_DTYPE_FP16, kNeighbours>(a, head_dim, st)
+                : launch_append<AEGKV_DTYPE_FP16, kHalves>(a, head_dim, st);
+  AEGKV_HIP_TRY(hipGetLastError());
+  return AEGKV_OK;
+}
+
+int aegkv_kv8_gather_tokens(const void* cache, int64_t cache_block_stride,
+                            int64_t cache_layer_stride, int64_t n_blocks,
+                            const int32_t* block_tables, int32_t max_blocks,
+                            const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t batch,
+                            int32_t max_seq_len, void* out_key, void* out_value,
+                            int64_t out_tokens, int64_t out_layer_stride, int32_t n_layers,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                            aegkv_stream_t stream) {
+  if (batch < 0 || max_seq_len < 0 || n_layers <= 0 || n_kv_heads <= 0 || head_dim <= 0 ||
+      max_blocks < 0 || n_blocks < 0 || out_tokens < 0)
+    return AEGKV_ERR_INVALID_ARG;
+  if (!head_dim_ok(head_dim) || !dtype_ok(dtype) || n_kv_heads > kKv8MaxHeads)
+    return AEGKV_ERR_UNSUPPORTED;
+  if (batch == 0 || max_seq_len == 0 || out_tokens == 0) return AEGKV_OK;
+  if (!cache || !block_tables || !seq_lens || !cu_seqlens || !out_key || !out_value)
+    return AEGKV_ERR_INVALID_ARG;
+  if (!aligned16(cache) || !aligned16(out_key) || !aligned16(out_value) ||
+      cache_block_stride % 16 || cache_layer_stride % 16 || out_layer_stride % 8)
+    return AEGKV_ERR_MISALIGNED;
+  const int64_t blocks_needed = ((int64_t)max_seq_len + kKv8Tokens - 1) / kKv8Tokens;
+  if (blocks_needed > max_blocks) return AEGKV_ERR_INVALID_ARG;
+  const int64_t per_tile = kGather8Threads / 64 * kGather8PerWave * (head_dim == 64 ? 2 : 1);
+  const int64_t passes = (2 * (int64_t)n_kv_heads + per_tile - 1) / per_tile;
+  if (n_layers > 65535 || blocks_needed * kGather8MaxBatch * passes > INT32_MAX)
+    return AEGKV_ERR_UNSUPPORTED;
+  DeviceState* ds = nullptr;
+  const int rc = current_device_state(&ds);
+  if (rc) return rc;
+  Gather8Args a;
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.blk_b = cache_block_stride;
+  a.layer_b = cache_layer_stride;
+  a.scales_at = kv8_scales_at(n_kv_heads, head_dim);
+  a.n_blocks = n_blocks;
+  a.max_blocks = max_blocks;
+  a.out_k = static_cast<uint8_t*>(out_key);
+  a.out_v = static_cast<uint8_t*>(out_value);
+  a.out_tokens = out_tokens;
+  a.out_layer_b = out_layer_stride * 2;
+  a.max_seq_len = max_seq_len;
+  a.n_heads = n_kv_heads;
+  a.passes = (int32_t)passes;
+  const int64_t max_grid = std::max<int64_t>(
+      1, ((int64_t)std::max(ds->num_cu, 1) * kGather8WorkgroupsPerCu + n_layers - 1) / n_layers);
+  for (int32_t b0 = 0; b0 < batch; b0 += kGather8MaxBatch) {
+    const int32_t nb = std::min(kGather8MaxBatch, batch - b0);
+    a.batch = nb;
+    a.block_tables = block_tables + (int64_t)b0 * max_blocks;
+    a.seq_lens = seq_lens + b0;
+    a.cu_seqlens = cu_seqlens + b0;
+    const int64_t tiles_max = blocks_needed * nb * passes;  // bound of a layer's tiles
+    const dim3 grid((uint32_t)std::min(tiles_max, max_grid), (uint32_t)n_layers);
+    if (dtype == AEGKV_DTYPE_BF16)
+      launch_gather<AEGKV_DTYPE_BF16>(a, head_dim, grid, (hipStream_t)stream);
+    else
+      launch_gather<AEGKV_DTYPE_FP16>(a, head_dim, grid, (hipStream_t)stream);
+    AEGKV_HIP_TRY(hipGetLastError());
+  }
+  return AEGKV_OK;
+}
+
+}  // extern "C"

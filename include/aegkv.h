@@ -499,6 +499,99 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
                                int32_t causal, int32_t dtype, void* workspace,
                                uint64_t workspace_bytes, aegkv_stream_t stream);
 
+/* ---- append with the position rotation ------------------------------------
+ * Between a layer's projection and its attention the reference's models call
+ * vLLM's rotary embedding on queries and keys, then the append
+ * (aegaeon/aegaeon/worker.py:517-523); here both are one launch.  For token t
+ * with p = positions[t] the first rotary_dim dims of every head's query and key
+ * row turn by p's angles: dims i and i + rotary_dim/2 (interleaved != 0: 2 i and
+ * 2 i + 1) are a pair (x, y) that becomes (x cos - y sin, y cos + x sin) of angle
+ * i, in fp32, each operation rounded by itself, the result rounded once.
+ *   table: DEVICE float [max_positions][rotary_dim], cosines of a position's
+ *     rotary_dim/2 angles, then sines.  A position outside it turns its rows to
+ *     NaN.
+ *   out_query: the turned queries, out_key (may be NULL) the turned keys (a
+ *     prompt's own attention reads them); either may be its input (same pointer
+ *     and stride).  All tokens are written, also those whose slot is skipped.
+ *   The turned key rows and the value rows go to the cache as in
+ *     aegkv_kv_append (one layer; slots < 0 and past the pool are skipped).
+ * Token strides in elements, the heads of a token dense.  rotary_dim a multiple
+ * of 16, head_dim of 8 and at most 512, at most 65535 heads. */
+int aegkv_rotary_append(const void* query, int64_t query_token_stride, void* out_query,
+                        int64_t out_query_token_stride, int32_t n_q_heads, const void* key,
+                        int64_t key_token_stride, const void* value, int64_t value_token_stride,
+                        void* out_key, int64_t out_key_token_stride, int32_t n_kv_heads,
+                        int32_t head_dim, const int64_t* slot_mapping, const int64_t* positions,
+                        int64_t n_tokens, const float* table, int64_t max_positions,
+                        int32_t rotary_dim, int32_t interleaved, void* key_cache,
+                        void* value_cache, int64_t cache_block_stride, int64_t n_blocks,
+                        int32_t block_size, int32_t dtype, aegkv_stream_t stream);
+
+/* ---- the 8-bit KV cache ----------------------------------------------------
+ * No counterpart in the reference, whose caches are 16-bit.  Blocks of 16 tokens
+ * whose values of one layer, kv head and side (K or V) share an exponent: the
+ * least integer e with max|x| <= 448 * 2^e over the block's finite values, within
+ * [-117, 119] (bf16 rows) or [-15, 7] (fp16 rows).  A value is stored as the 8-bit
+ * float (1 sign, 4 exponent and 3 mantissa bits, bias 7, no infinities; NaN 0x7f and 0xff)
+ * nearest to x / 2^e (ties to even, at most 448), an infinity or NaN as 0xff; the
+ * stored value is code * 2^e, exact in the rows' 16-bit type.
+ *   An append to a block's first place begins the block: its exponent is the new
+ * tokens', its other tokens read as 0.  Other tokens join what the block holds: the
+ * exponent becomes the larger of its own and theirs, and when it rises the earlier
+ * tokens' values are rounded once more, to codes of the new exponent.  (A held
+ * exponent outside the bounds, which no append writes, counts as the nearer one.)
+ *   A block of one layer: per kv head 16 * head_dim bytes of K codes, then of V
+ *     codes; then 4 bytes per head: K's e + 127, V's, 1 where V holds a NaN, 0;
+ *     padded with unused bytes to a multiple of 128 (aegkv_kv8_block_bytes).
+ *     K codes: [chunk of 16 dims][16 tokens][16 dims].  V codes: [head_dim / 64][4]
+ *     [16 lanes j][4 dims][4 tokens], token 4 x (second index) + (last), dim
+ *     head_dim / 16 * j + 4 x (first index) + (fourth).
+ *   Storage [N][L][aegkv_kv8_block_bytes], so the byte-moving entries and the block
+ *     manager take it as any pool with L * aegkv_kv8_block_bytes per block.
+ * head_dim 64, 128 or 256, at most 256 kv heads; strides of the cache in bytes,
+ * multiples of 16. */
+
+/* Bytes of one block of one layer (or a status). */
+int64_t aegkv_kv8_block_bytes(int32_t n_kv_heads, int32_t head_dim);
+
+/* aegkv_kv_append into the 8-bit cache: key/value rows of `dtype` (strides in
+ * elements, the heads of a token dense), slots as there (negative ones and those
+ * past the pool are skipped).  The tokens of one block must follow each other in
+ * the call (as those of a prompt do), in any order within it; of two for one slot
+ * the later one counts.  (Tokens of a block that other tokens lie between may
+ * leave the block's values wrong, not those of other blocks.) */
+int aegkv_kv8_append(const void* key, const void* value, int64_t key_token_stride,
+                     int64_t value_token_stride, int64_t key_layer_stride,
+                     int64_t value_layer_stride, const int64_t* slot_mapping, int64_t n_tokens,
+                     void* cache, int64_t cache_block_stride, int64_t cache_layer_stride,
+                     int64_t n_blocks, int32_t n_layers, int32_t n_kv_heads, int32_t head_dim,
+                     int32_t dtype, aegkv_stream_t stream);
+
+/* aegkv_rotary_append into a layer of the 8-bit cache: the codes are those of the
+ * turned keys in fp32 (not rounded to 16 bits in between).  out_query may be query;
+ * out_key must not overlap key. */
+int aegkv_kv8_rotary_append(const void* query, int64_t query_token_stride, void* out_query,
+                            int64_t out_query_token_stride, int32_t n_q_heads, const void* key,
+                            int64_t key_token_stride, const void* value,
+                            int64_t value_token_stride, void* out_key,
+                            int64_t out_key_token_stride, int32_t n_kv_heads, int32_t head_dim,
+                            const int64_t* slot_mapping, const int64_t* positions,
+                            int64_t n_tokens, const float* table, int64_t max_positions,
+                            int32_t rotary_dim, int32_t interleaved, void* cache,
+                            int64_t cache_block_stride, int64_t n_blocks, int32_t dtype,
+                            aegkv_stream_t stream);
+
+/* aegkv_gather_tokens from the 8-bit cache: the values the codes stand for, in
+ * `dtype`, the type of the appended rows.  out_layer_stride in elements. */
+int aegkv_kv8_gather_tokens(const void* cache, int64_t cache_block_stride,
+                            int64_t cache_layer_stride, int64_t n_blocks,
+                            const int32_t* block_tables, int32_t max_blocks,
+                            const int32_t* seq_lens, const int32_t* cu_seqlens, int32_t batch,
+                            int32_t max_seq_len, void* out_key, void* out_value,
+                            int64_t out_tokens, int64_t out_layer_stride, int32_t n_layers,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                            aegkv_stream_t stream);
+
 /* ---- a8: node-wide block manager (host bookkeeping) ----------------------
  * Replaces the allocation and move bookkeeping of BlockManager
  * (aegaeon/aegaeon/block_manager.py:180-874).  Pure host code, no HIP calls;
