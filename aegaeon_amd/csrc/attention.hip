@@ -62,6 +62,7 @@
 
 #include "aegkv_internal.h"
 #include "kv4_format.h"
+#include "kv8_format.h"
 
 namespace aegkv {
 namespace {
@@ -102,9 +103,9 @@ __device__ __forceinline__ int cost_units(int len) {
 // wave per SIMD.
 template <int D>
 constexpr int pipeline_depth() { return D >= 256 ? 2 : 3; }
-// Register sets of the 4-bit cache, a step each (of four blocks at D = 128: 17 KB a
-// wave).
-constexpr int kKv4PipelineDepth = 2;
+// Register sets of the 4- and 8-bit caches, a step each (of four blocks at D = 128:
+// 17 KB a wave in 4 bits, 16 in 8).
+constexpr int kStepPipelineDepth = 2;
 
 // kv heads of a workgroup's group, one per wave; the 4 / heads waves of each
 // head take ranges of their own.  Four, unless that leaves one wave in 20 or
@@ -248,7 +249,8 @@ struct AttnArgs {
   int32_t n_ranges;  // n_wg * kWaves / heads
   RangeRule ranges;  // how many of them take part
   float scale_log2;  // softmax scale * log2(e)
-  int32_t scale_sign;        // 4-bit cache: its sign, 1, -1 or 0
+  int64_t scales_at;         // 8-bit cache: the heads' scale bytes in a block
+  int32_t scale_sign;        // 4- and 8-bit caches: its sign, 1, -1 or 0
   float abs_scale_log2;      // and magnitude (1 for 0)
   int32_t max_seq_len;  // host bound; longer device lengths are clamped to it
   uint16_t* out;
@@ -800,6 +802,209 @@ __device__ __forceinline__ void compute_step4(KV4Regs<D> (&r)[step4<D>()], const
   }
 }
 
+// attend_steps' view of the 4-bit cache.
+struct Steps4 {
+  template <int D>
+  using Regs = KV4Regs<D>;
+  template <int D>
+  static constexpr int step() { return step4<D>(); }
+  template <int D, int PACK>
+  static constexpr int tiles() { return acc_tiles<D, PACK>(); }
+  template <int D>
+  static __device__ __forceinline__ int dim(int ks, int g) { return kv4_dim<D>(ks, g); }
+  template <int D>
+  static __device__ __forceinline__ void load(const AttnArgs& a, Regs<D>& r, int id, bool ok, int h,
+                                              int lane) {
+    const uint8_t* p =
+        reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id : 0) * a.blk_stride) +
+        (int64_t)h * 17 * D;
+    load_block4<D>(r, byte_range(p, ok ? 17 * D : 0u), lane);
+  }
+  template <int DT, int D, int PACK>
+  static __device__ __forceinline__ void compute(Regs<D> (&r)[step<D>()], const u32x4* qv,
+                                                 f32x4* acc, float& m, float& lsum, int tok0,
+                                                 int limit, uint32_t skip, int g,
+                                                 float scale_log2) {
+    compute_step4<DT, D, PACK>(r, qv, acc, m, lsum, tok0, limit, skip, g, scale_log2);
+  }
+};
+
+// ---- the 8-bit cache (kv8_format.h) ----
+// As the 4-bit cache: K and V are converted to 16 bits, where code times scale is
+// exact, two codes per instruction, and everything past that is the 16-bit cache's
+// arithmetic.  Per block of 16 tokens, with lane l = 16 g + j:
+//   S^T[16 tok x 16 heads] = K . Q^T: the lane's 16 bytes of a load are dims 64 i +
+//     16 g .. + 15 of token j, two k-steps of the 16-bit MFMA; the query's dims
+//     run in the same order.
+//   O^T[D x 16 heads] += V^T . P^T: a word of V is one dim of the tokens 4 g .. 4 g
+//     + 3, which P^T's lane (head j, g) has too, so two conversions are half of a
+//     lane's operand.  PACK = 1: the contraction's other half takes V again against
+//     P's low part (P in two 16-bit parts, as above).  PACK = 2 (8 query heads per kv
+//     head or fewer): the columns 8 + head take the low part, and the other half the
+//     next block, half as many products.
+
+// Codes and scale bytes of one block for one lane.
+template <int D>
+struct KV8Regs {
+  static constexpr int NW = D / 16;  // words of codes of a side
+  uint32_t k[NW], v[NW];             // v[t]: dim D/16 j + t
+  uint32_t s;                        // the head's bytes: K's scale, V's
+};
+template <int D>
+__device__ __forceinline__ int kv8_dim(int ks, int g) {
+  return 64 * (ks >> 1) + 16 * g + 8 * (ks & 1);
+}
+// One block of one kv head: r is the layer's block from the head's codes on (or
+// empty), scale its scale bytes' offset there.
+template <int D>
+__device__ __forceinline__ void load_block8(KV8Regs<D>& b, __amdgpu_buffer_rsrc_t r, int scale,
+                                            int lane) {
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(r, 1024 * i + 16 * lane, 0, kNt);
+    const u32x4 v =
+        __builtin_amdgcn_raw_buffer_load_b128(r, 16 * D + 1024 * i + 16 * lane, 0, kNt);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      b.k[4 * i + w] = k[w];
+      b.v[4 * i + w] = v[w];
+    }
+  }
+  b.s = __builtin_amdgcn_raw_buffer_load_b32(r, scale, 0, 0);
+}
+
+inline int pack8_for(int32_t group) { return group <= 8 ? 2 : 1; }
+
+// A step of up to step8() consecutive blocks of one sequence (see compute_step4).
+template <int D>
+constexpr int step8() { return D >= 256 ? 2 : 4; }
+template <int DT, int D, int PACK>
+__device__ __forceinline__ void compute_step8(KV8Regs<D> (&r)[step8<D>()], const u32x4* qv,
+                                              f32x4* acc, float& m, float& lsum, int tok0,
+                                              int limit, uint32_t skip, int g, float scale_log2) {
+  using E = Elem<DT>;
+  using C = Kv8Elem<DT>;
+  constexpr int S = step8<D>(), NT = D / 16;
+  f32x4 sc[S];
+#pragma unroll
+  for (int u = 0; u < S; ++u) {
+    const float s = kv8_scale(r[u].s & 0xffu);
+    sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) {
+      const uint32_t w0 = r[u].k[2 * ks], w1 = r[u].k[2 * ks + 1];
+      sc[u] = E::mfma(u32x4{C::template dq<false>(w0, s), C::template dq<true>(w0, s),
+                            C::template dq<false>(w1, s), C::template dq<true>(w1, s)},
+                      qv[ks], sc[u]);
+    }
+  }
+  if (skip != 0 || tok0 + 16 * S > limit) {  // uniform
+    const int last = limit - tok0 - 4 * g;   // this lane's tokens 16 u + i below it
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      uint32_t keep = 0;  // V's stale bytes, maybe NaN, to zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = 16 * u + i < last;
+        sc[u][i] = in && !(skip >> u & 1) ? sc[u][i] : -INFINITY;
+        keep |= in ? 0xffu << (8 * i) : 0u;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) r[u].v[t] &= keep;
+    }
+  }
+  float bm = sc[0][0];
+#pragma unroll
+  for (int u = 0; u < S; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bm = fmaxf(bm, sc[u][i]);
+  bm = max_over_g(bm);
+  if constexpr (E::kTop == 0.f) bm *= scale_log2;
+  else bm = __builtin_fmaf(bm, scale_log2, -E::kTop);
+  if (__builtin_amdgcn_ballot_w64(bm > m + kRescaleSlack)) {  // lazy rescaling, as in compute_block
+    const float mn = fmaxf(m, bm);
+    // 0 while m = -inf (beside another head's first finite score too)
+    const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    lsum *= alpha;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] *= alpha;
+    m = mn;
+  }
+  const bool low_part = (threadIdx.x & 8) != 0;
+  const float nms = m == -INFINITY ? 0.f : -m;  // -inf only while every token is masked
+  uint32_t hi[S][2], lo[S][2];                  // P's parts, two tokens a word
+#pragma unroll
+  for (int u = 0; u < S; ++u) {
+    float p[4];
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][i], scale_log2, nms));
+      E::split(p[i], h[i], l[i]);
+    }
+    lsum += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      hi[u][i] = h[2 * i] | (h[2 * i + 1] << 16);
+      lo[u][i] = l[2 * i] | (l[2 * i + 1] << 16);
+    }
+  }
+  if constexpr (PACK == 1) {
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      const float s = kv8_scale(r[u].s >> 8 & 0xffu);
+      const u32x4 w = {hi[u][0], hi[u][1], lo[u][0], lo[u][1]};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint32_t a = C::template dq<false>(r[u].v[t], s), b = C::template dq<true>(r[u].v[t], s);
+        acc[t] = E::mfma(u32x4{a, b, a, b}, w, acc[t]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < S; u += 2) {
+      const float s = kv8_scale(r[u].s >> 8 & 0xffu), s2 = kv8_scale(r[u + 1].s >> 8 & 0xffu);
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = low_part ? lo[u + (i >> 1)][i & 1] : hi[u + (i >> 1)][i & 1];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        acc[t] = E::mfma(
+            u32x4{C::template dq<false>(r[u].v[t], s), C::template dq<true>(r[u].v[t], s),
+                  C::template dq<false>(r[u + 1].v[t], s2), C::template dq<true>(r[u + 1].v[t], s2)},
+            w, acc[t]);
+    }
+  }
+}
+
+// attend_steps' view of the 8-bit cache.
+struct Steps8 {
+  template <int D>
+  using Regs = KV8Regs<D>;
+  template <int D>
+  static constexpr int step() { return step8<D>(); }
+  template <int D, int PACK>
+  static constexpr int tiles() { return D / 16; }
+  template <int D>
+  static __device__ __forceinline__ int dim(int ks, int g) { return kv8_dim<D>(ks, g); }
+  template <int D>
+  static __device__ __forceinline__ void load(const AttnArgs& a, Regs<D>& r, int id, bool ok, int h,
+                                              int lane) {
+    const int codes = h * 2 * kv8_side_bytes(D), scale = (int)a.scales_at + 4 * h - codes;
+    const uint8_t* p =
+        reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id : 0) * a.blk_stride) + codes;
+    load_block8<D>(r, byte_range(p, ok ? (uint32_t)scale + 4 : 0u), scale, lane);
+  }
+  template <int DT, int D, int PACK>
+  static __device__ __forceinline__ void compute(Regs<D> (&r)[step<D>()], const u32x4* qv,
+                                                 f32x4* acc, float& m, float& lsum, int tok0,
+                                                 int limit, uint32_t skip, int g,
+                                                 float scale_log2) {
+    compute_step8<DT, D, PACK>(r, qv, acc, m, lsum, tok0, limit, skip, g, scale_log2);
+  }
+};
+
 // Calls f(integral_constant<int, k>) for k = 0, 1, ... until one returns true
 // (fully unrolled: k is a compile-time constant in every call).
 template <typename F, int... Ks>
@@ -1242,18 +1447,18 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
   flush();
 }
 
-// attend_items over the 4-bit cache: the same items, ids, pieces and records,
-// in steps of up to step4() blocks that end where a piece does.  During a step's
+// attend_items over the 4- or 8-bit cache (F: Steps4, Steps8): the same items, ids,
+// pieces and records, in steps of up to F::step() blocks that end where a piece does.  During a step's
 // compute the next NSET - 1 are in flight, across sequences, and its registers are
 // loaded again behind it: the load side keeps a sequence position of its own, and hands a step's to the
 // compute side with its registers.  Past the range a step loads nothing (empty
 // buffer ranges) and is not computed.
-template <int DT, int D, int NSET, int PACK, bool PLANNED>
-__device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* s_bcum,
-                                              const int32_t* s_len, uint8_t* stage, int4* meta,
-                                              int range, int grp, int hl, int b0, int i0, int i1,
-                                              bool have_first, int id_first) {
-  constexpr int KS = D / 32, DPL = D / 16, kStep4 = step4<D>();
+template <class F, int DT, int D, int NSET, int PACK, bool PLANNED>
+__device__ __forceinline__ void attend_steps(const AttnArgs& a, const int32_t* s_bcum,
+                                             const int32_t* s_len, uint8_t* stage, int4* meta,
+                                             int range, int grp, int hl, int b0, int i0, int i1,
+                                             bool have_first, int id_first) {
+  constexpr int KS = D / 32, DPL = D / 16, kStep = F::template step<D>();
   const int lane = threadIdx.x & 63;
   const int h = grp * a.heads + hl;
   if (h >= a.n_kv_heads) return;  // wave past the last kv head (uniform)
@@ -1283,20 +1488,20 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
   int ids = PLANNED && have_first ? id_first : load_ids();
   const int jq = j % (16 / PACK);
   const uint16_t* q_lane =
-      a.q + (int64_t)(h * a.group + (jq < a.group ? jq : 0)) * D + kv4_dim<D>(0, g);
+      a.q + (int64_t)(h * a.group + (jq < a.group ? jq : 0)) * D + F::template dim<D>(0, g);
   struct Step {
     int n;          // blocks (0: past the range)
     uint32_t skip;  // blocks not to attend: unreadable, or past n
     u32x4 q[KS];    // the sequence's query, this lane's head
-    KV4Regs<D> kv[kStep4];
+    typename F::template Regs<D> kv[kStep];
   };
   Step st[NSET];
   auto load_step = [&](Step& s) {
-    s.n = min(kStep4, lend - il);
+    s.n = min(kStep, lend - il);
     s.skip = 0;
-    int id[kStep4];
+    int id[kStep];
 #pragma unroll
-    for (int u = 0; u < kStep4; ++u) id[u] = __builtin_amdgcn_readlane(ids, u);
+    for (int u = 0; u < kStep; ++u) id[u] = __builtin_amdgcn_readlane(ids, u);
     const uint16_t* qp = q_lane + (int64_t)bl * a.q_bstride;
     il += s.n;
     if (il == lend && il < i1) {
@@ -1307,22 +1512,19 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
     ids = load_ids();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      s.q[ks] = *reinterpret_cast<const u32x4*>(qp + (kv4_dim<D>(ks, 0) - kv4_dim<D>(0, 0)));
+      s.q[ks] = *reinterpret_cast<const u32x4*>(qp + (F::template dim<D>(ks, 0) - F::template dim<D>(0, 0)));
 #pragma unroll
-    for (int u = 0; u < kStep4; ++u) {
+    for (int u = 0; u < kStep; ++u) {
       const bool ok = u < s.n && id[u] >= 0 && id[u] < a.n_blocks;
       if (!ok) s.skip |= 1u << u;
-      const uint8_t* p =
-          reinterpret_cast<const uint8_t*>(a.kc + (int64_t)(ok ? id[u] : 0) * a.blk_stride) +
-          (int64_t)h * 17 * D;
-      load_block4<D>(s.kv[u], byte_range(p, ok ? 17 * D : 0u), lane);
+      F::template load<D>(a, s.kv[u], id[u], ok, h, lane);
     }
   };
 
   // the compute side
   int bc = b0, first = uni(s_bcum[b0]), cend = lend, len = uni(s_len[b0]), ic = i0;
   bool complete = first >= i0 && cend == uni(s_bcum[b0 + 1]);
-  constexpr int NT = acc_tiles<D, PACK>();
+  constexpr int NT = F::template tiles<D, PACK>();
   f32x4 acc[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1352,9 +1554,9 @@ __device__ __forceinline__ void attend_items4(const AttnArgs& a, const int32_t* 
 #pragma unroll
         for (int i = 0; i < 4; ++i) s.q[ks][i] = a.scale_sign < 0 ? s.q[ks][i] ^ 0x80008000u : 0u;
     }
-    compute_step4<DT, D, PACK>(s.kv, s.q, acc, m, lsum, (ic - first) * kBlockSize,
-                               min(len, (cend - first) * kBlockSize), s.skip, g,
-                               a.abs_scale_log2);
+    F::template compute<DT, D, PACK>(s.kv, s.q, acc, m, lsum, (ic - first) * kBlockSize,
+                                     min(len, (cend - first) * kBlockSize), s.skip, g,
+                                     a.abs_scale_log2);
     ic += s.n;
     if (ic == cend) {  // the piece of sequence bc in this range ends (uniform)
       float lt = lsum + __shfl_xor(lsum, 16);
@@ -1508,8 +1710,9 @@ __device__ __forceinline__ int items_before(const int32_t* cum, const int32_t* b
   return bcum[b] + min(max(p - cum[b] - kSegmentCost, 0), bcum[b + 1] - bcum[b]);
 }
 
-// PACK: 0, the 16-bit caches; 1, 2 or 4, the 4-bit cache (pack_for).
-template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, int PACK>
+// PACK: 0, the 16-bit caches; else the cache that F reads, 4-bit (1, 2 or 4: pack_for)
+// or 8-bit (1 or 2: pack8_for).
+template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, int PACK, class F>
 __global__ __launch_bounds__(64 * kWaves, D >= 256 ? 1 : 2) void
 paged_decode_attention_kernel(AttnArgs a) {
   // cum[batch + 1] (positions), len[batch], bcum[batch + 1] (blocks)
@@ -1561,8 +1764,8 @@ paged_decode_attention_kernel(AttnArgs a) {
       const int i1 = grp == uni(rec[1]) ? uni(rec[4]) : items;
       if (i1 <= i0) continue;
       if constexpr (PACK > 0)
-        attend_items4<DT, D, NBUF, PACK, true>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
-                                         i0, i1, first_pass, id_first);
+        attend_steps<F, DT, D, NBUF, PACK, true>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
+                                                 hl, b0, i0, i1, first_pass, id_first);
       else
         attend_items<DT, D, NBUF, true, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
                                                hl, b0, i0, i1, first_pass, id_first,
@@ -1604,8 +1807,8 @@ paged_decode_attention_kernel(AttnArgs a) {
     }
     if constexpr (PACK > 0) {
       if (i1 > i0)
-        attend_items4<DT, D, NBUF, PACK, false>(a, s_bcum, s_len, stage, s_meta[wave], range, grp, hl, b0,
-                                          i0, i1, false, 0);
+        attend_steps<F, DT, D, NBUF, PACK, false>(a, s_bcum, s_len, stage, s_meta[wave], range,
+                                                  grp, hl, b0, i0, i1, false, 0);
     } else if (i1 > i0)
       attend_items<DT, D, NBUF, false, FUSED>(a, s_bcum, s_len, stage, s_meta[wave], range, grp,
                                               hl, b0, i0, i1, false, 0, -1, s_over, nstage,
@@ -2076,10 +2279,10 @@ int launch_combine(const AttnArgs& a, hipStream_t stream) {
   return AEGKV_OK;
 }
 
-template <int DT, int D, bool PLANNED, bool FUSED, int PACK = 0>
+template <int DT, int D, bool PLANNED, bool FUSED, int PACK = 0, class F = Steps4>
 void launch_main(const AttnArgs& a, size_t lds, hipStream_t stream) {
-  constexpr int NBUF = PACK > 0 ? kKv4PipelineDepth : pipeline_depth<D>();
-  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, PACK>),
+  constexpr int NBUF = PACK > 0 ? kStepPipelineDepth : pipeline_depth<D>();
+  hipLaunchKernelGGL((paged_decode_attention_kernel<DT, D, NBUF, PLANNED, FUSED, PACK, F>),
                      dim3(a.n_wg), dim3(64 * kWaves), lds, stream, a);
 }
 template <int DT, int D, bool PLANNED>
@@ -2091,9 +2294,21 @@ void launch_main4(const AttnArgs& a, size_t lds, hipStream_t stream) {
   }
 }
 
+template <int DT, int D, bool PLANNED>
+void launch_main8(const AttnArgs& a, size_t lds, hipStream_t stream) {
+  if (pack8_for(a.group) == 2) launch_main<DT, D, PLANNED, false, 2, Steps8>(a, lds, stream);
+  else launch_main<DT, D, PLANNED, false, 1, Steps8>(a, lds, stream);
+}
+
+// What the caches hold a value in.
+enum class CacheBits { k16, k4, k8 };
+
 template <int DT, int D>
-int launch_attention(const AttnArgs& a, bool kv4, size_t lds, hipStream_t stream) {
-  if (kv4) {
+int launch_attention(const AttnArgs& a, CacheBits bits, size_t lds, hipStream_t stream) {
+  if (bits == CacheBits::k8) {
+    if (a.plan_wg) launch_main8<DT, D, true>(a, lds, stream);
+    else launch_main8<DT, D, false>(a, lds, stream);
+  } else if (bits == CacheBits::k4) {
     if (a.plan_wg) launch_main4<DT, D, true>(a, lds, stream);
     else launch_main4<DT, D, false>(a, lds, stream);
   } else if (a.plan_wg) {
@@ -2116,8 +2331,8 @@ int launch_attention(const AttnArgs& a, bool kv4, size_t lds, hipStream_t stream
 namespace aegkv {
 namespace {
 // Every entry point: `plan` (with plan_bytes) replaces the block tables when
-// given; kv4: both caches are the 4-bit cache, cache_block_stride in units of
-// two bytes.
+// given; bits: both caches are the 4- or 8-bit one unless it says 16,
+// cache_block_stride in units of two bytes.
 // The new token's K/V rows of an appending call (none: key == nullptr).
 struct NewRows {
   const void* key = nullptr;
@@ -2133,16 +2348,18 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
                   int32_t max_seq_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                   int32_t block_size, float scale, int32_t dtype, int32_t n_workgroups,
                   void* workspace, uint64_t workspace_bytes, aegkv_stream_t stream,
-                  const NewRows& nr = NewRows(), bool kv4 = false) {
+                  const NewRows& nr = NewRows(), CacheBits bits = CacheBits::k16) {
   if (batch < 0 || max_seq_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || max_blocks < 0 ||
       n_blocks < 0 || n_workgroups < 0)
     return AEGKV_ERR_INVALID_ARG;
   // (times a score of zero, or of a masked token, an infinite one would give NaN)
-  if (kv4 && !std::isfinite(scale * 1.4426950408889634f)) return AEGKV_ERR_INVALID_ARG;
+  if (bits != CacheBits::k16 && !std::isfinite(scale * 1.4426950408889634f))
+    return AEGKV_ERR_INVALID_ARG;
   if (n_q_heads % n_kv_heads) return AEGKV_ERR_INVALID_ARG;
   if (block_size != kBlockSize || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
       n_q_heads / n_kv_heads > 16 || (dtype != AEGKV_DTYPE_BF16 && dtype != AEGKV_DTYPE_FP16))
     return AEGKV_ERR_UNSUPPORTED;
+  if (bits == CacheBits::k8 && n_kv_heads > kKv8MaxHeads) return AEGKV_ERR_UNSUPPORTED;
   if (batch == 0) return AEGKV_OK;
   if (!out || !q || !key_cache || !value_cache || (!block_tables && !plan) || !seq_lens ||
       n_blocks == 0)
@@ -2195,6 +2412,7 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
   a.n_ranges = n_ranges;
   a.ranges = range_rule(n_wg, n_kv_heads, heads);
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.scales_at = kv8_scales_at(n_kv_heads, head_dim);
   a.scale_sign = scale < 0.f ? -1 : scale == 0.f ? 0 : 1;
   a.abs_scale_log2 = scale == 0.f ? 1.f : std::fabs(a.scale_log2);
   a.max_seq_len = max_seq_len;
@@ -2253,12 +2471,12 @@ int run_attention(void* out, int64_t out_batch_stride, const void* q, int64_t q_
     }
     const size_t lds = lds_bytes(a, ds->max_lds);
     switch (head_dim) {
-      case 64: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 64>(a, kv4, lds, st)
-                       : launch_attention<AEGKV_DTYPE_FP16, 64>(a, kv4, lds, st); break;
-      case 128: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 128>(a, kv4, lds, st)
-                        : launch_attention<AEGKV_DTYPE_FP16, 128>(a, kv4, lds, st); break;
-      default: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 256>(a, kv4, lds, st)
-                       : launch_attention<AEGKV_DTYPE_FP16, 256>(a, kv4, lds, st); break;
+      case 64: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 64>(a, bits, lds, st)
+                       : launch_attention<AEGKV_DTYPE_FP16, 64>(a, bits, lds, st); break;
+      case 128: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 128>(a, bits, lds, st)
+                        : launch_attention<AEGKV_DTYPE_FP16, 128>(a, bits, lds, st); break;
+      default: rc = bf ? launch_attention<AEGKV_DTYPE_BF16, 256>(a, bits, lds, st)
+                       : launch_attention<AEGKV_DTYPE_FP16, 256>(a, bits, lds, st); break;
     }
     if (rc) return rc;
   }
@@ -2511,7 +2729,7 @@ int aegkv_kv4_decode_attention(void* out, int64_t out_batch_stride, const void* 
                        cache_block_stride / 2, n_blocks, block_tables, max_blocks, nullptr, 0,
                        seq_lens, batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize,
                        scale, dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(),
-                       true);
+                       CacheBits::k4);
 }
 
 int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, const void* q,
@@ -2528,7 +2746,43 @@ int aegkv_kv4_decode_attention_planned(void* out, int64_t out_batch_stride, cons
   return run_attention(out, out_batch_stride, q, q_batch_stride, cache, cache,
                        cache_block_stride / 2, n_blocks, nullptr, 0, plan, plan_bytes, seq_lens,
                        batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize, scale,
-                       dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(), true);
+                       dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(),
+                       CacheBits::k4);
+}
+
+int aegkv_kv8_decode_attention(void* out, int64_t out_batch_stride, const void* q,
+                               int64_t q_batch_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* seq_lens, int32_t batch, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                               float scale, int32_t dtype, int32_t n_workgroups, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream) {
+  if (batch > 0 && !block_tables) return AEGKV_ERR_INVALID_ARG;
+  if (cache_block_stride & 15) return AEGKV_ERR_MISALIGNED;
+  return run_attention(out, out_batch_stride, q, q_batch_stride, cache, cache,
+                       cache_block_stride / 2, n_blocks, block_tables, max_blocks, nullptr, 0,
+                       seq_lens, batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize,
+                       scale, dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(),
+                       CacheBits::k8);
+}
+
+int aegkv_kv8_decode_attention_planned(void* out, int64_t out_batch_stride, const void* q,
+                                       int64_t q_batch_stride, const void* cache,
+                                       int64_t cache_block_stride, int64_t n_blocks,
+                                       const void* plan, uint64_t plan_bytes,
+                                       const int32_t* seq_lens, int32_t batch,
+                                       int32_t max_seq_len, int32_t n_q_heads,
+                                       int32_t n_kv_heads, int32_t head_dim, float scale,
+                                       int32_t dtype, int32_t n_workgroups, void* workspace,
+                                       uint64_t workspace_bytes, aegkv_stream_t stream) {
+  if (batch > 0 && !plan) return AEGKV_ERR_INVALID_ARG;
+  if (cache_block_stride & 15) return AEGKV_ERR_MISALIGNED;
+  return run_attention(out, out_batch_stride, q, q_batch_stride, cache, cache,
+                       cache_block_stride / 2, n_blocks, nullptr, 0, plan, plan_bytes, seq_lens,
+                       batch, max_seq_len, n_q_heads, n_kv_heads, head_dim, kBlockSize, scale,
+                       dtype, n_workgroups, workspace, workspace_bytes, stream, NewRows(),
+                       CacheBits::k8);
 }
 
 }  // extern "C"

@@ -19,7 +19,7 @@ stream.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Tuple
+from typing import Callable, Dict, Optional, Tuple
 
 import torch
 
@@ -197,6 +197,24 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
     that function's; a sequence without tokens gives zeros.  ``scale``: any
     number that stays finite times log2 e.  New rows are appended by a call of
     their own, before this one."""
+    return _paged_decode(_heads, "aegkv_kv4_decode_attention", "paged_decode_attention_kv4", q,
+                         kv_cache, block_tables, seq_lens, scale, max_seq_len, out, n_workgroups,
+                         workspace, plan)
+
+
+def _heads(c: torch.Tensor, head_dim: int) -> int:
+    """The kv heads of one layer ``[N, Hkv, 2, R]``."""
+    _check_cache(c, False, head_dim)
+    return c.size(1)
+
+
+def _paged_decode(heads_of: Callable[[torch.Tensor, int], int], entry: str, op: str,
+                  q: torch.Tensor, kv_cache: torch.Tensor, block_tables: Optional[torch.Tensor],
+                  seq_lens: Optional[torch.Tensor], scale: float, max_seq_len: int,
+                  out: Optional[torch.Tensor], n_workgroups: int,
+                  workspace: Optional[torch.Tensor], plan: Optional[DecodePlan]) -> torch.Tensor:
+    """Decode attention over one layer of a 4- or 8-bit cache: ``heads_of``
+    checks the cache and tells its kv heads, ``entry`` names the C entry."""
     shape, q_strides, dev = q.shape, q.stride(), q.device
     if len(shape) != 3 or q_strides[2] != 1 or q_strides[1] != shape[2] or not q.is_cuda:
         raise ValueError("q must be a GPU tensor [B, Hq, D] with dense heads")
@@ -204,8 +222,7 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
     if dtype is None:
         raise ValueError("q must be bf16 or fp16")
     B, Hq, D = shape
-    _check_cache(kv_cache, False, D)
-    N, Hkv = kv_cache.shape[:2]
+    Hkv = heads_of(kv_cache, D)
     if kv_cache.device != dev:
         raise ValueError(f"kv_cache must be a GPU tensor on {dev} (got {kv_cache.device})")
     if plan is not None:  # whose tables and lengths were checked when it was built
@@ -243,16 +260,16 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
         if workspace is not None:
             _check_workspace(workspace, ws_bytes, dev)
         args = (out.data_ptr(), out.stride(0), q.data_ptr(), q_strides[0], kv_cache.data_ptr(),
-                kv_cache.stride(0), N)
+                kv_cache.stride(0), kv_cache.size(0))
         if plan is not None:
             if stream != plan.raw_stream:
                 plan.wait_for_build(torch.cuda.current_stream(dev))
             args += (plan.buffer.data_ptr(), plan.nbytes)
-            call = lib.aegkv_kv4_decode_attention_planned
+            call = getattr(lib, entry + "_planned")
         else:
             bt = _int32_dense(block_tables)
             args += (bt.data_ptr(), bt.size(1))
-            call = lib.aegkv_kv4_decode_attention
+            call = getattr(lib, entry)
         with _OWN_WORKSPACE if shared is None else shared.lock:
             if shared is not None:
                 workspace = shared.at_least(ws_bytes, dev)
@@ -260,7 +277,7 @@ def paged_decode_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor,
                 workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             rc = call(*args, sl.data_ptr(), B, max_seq_len, Hq, Hkv, D, float(scale), dtype,
                       n_workgroups, workspace.data_ptr(), ws_bytes, stream)
-    _lib.check(rc, "paged_decode_attention_kv4")
+    _lib.check(rc, op)
     return out
 
 
@@ -299,6 +316,18 @@ def varlen_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: 
     64 or 128.  ``workspace``: :func:`varlen_attention_workspace` (reusable on
     one stream, by one thread at a time); by default one per (device, stream)
     that threads may share."""
+    return _varlen(_heads, "aegkv_kv4_varlen_attention", "varlen_attention_kv4", q, kv_cache,
+                   block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, scale, causal,
+                   out, workspace)
+
+
+def _varlen(heads_of: Callable[[torch.Tensor, int], int], entry: str, op: str, q: torch.Tensor,
+            kv_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+            seq_lens: torch.Tensor, max_seqlen_q: int, max_seq_len: int, scale: float,
+            causal: bool, out: Optional[torch.Tensor],
+            workspace: Optional[torch.Tensor]) -> torch.Tensor:
+    """Attention of several query tokens per sequence over one layer of a 4- or
+    8-bit cache (see :func:`_paged_decode`)."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens, Hq, D]")
     _check_rows(q, "q")
@@ -306,7 +335,7 @@ def varlen_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: 
         raise ValueError("q must be bf16 or fp16")
     T, Hq, D = q.shape
     dev = q.device
-    _check_cache(kv_cache, False, D)
+    Hkv = heads_of(kv_cache, D)
     _check_on(kv_cache, "kv_cache", dev)
     _check_on(block_tables, "block_tables", dev)
     _check_on(seq_lens, "seq_lens", dev)
@@ -319,10 +348,10 @@ def varlen_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: 
         return out
     bt, sl = _int32_dense(block_tables), _int32_dense(seq_lens)
     lib = _lib.load()
-    sizes = (int(max_seqlen_q), int(max_seq_len), Hq, kv_cache.size(1), D)
+    sizes = (int(max_seqlen_q), int(max_seq_len), Hq, Hkv, D)
     dtype = _DTYPES[q.dtype]
     with device_guard(dev):
-        ws_bytes = lib.aegkv_kv4_varlen_attention_workspace_size(B, T, *sizes, dtype)
+        ws_bytes = getattr(lib, entry + "_workspace_size")(B, T, *sizes, dtype)
         if ws_bytes < 0:
             _lib.check(int(ws_bytes), "varlen_attention_workspace")
         stream = raw_stream(dev)
@@ -336,13 +365,13 @@ def varlen_attention_kv4(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: 
                 workspace = shared.at_least(ws_bytes, dev)
             elif workspace is None and ws_bytes > 0:
                 workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            rc = lib.aegkv_kv4_varlen_attention(
+            rc = getattr(lib, entry)(
                 out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), kv_cache.data_ptr(),
                 kv_cache.stride(0), kv_cache.size(0), bt.data_ptr(), bt.size(1),
                 cu_seqlens_q.data_ptr(), sl.data_ptr(), B, T, *sizes, float(scale),
                 int(bool(causal)), dtype, workspace.data_ptr() if ws_bytes > 0 else None, ws_bytes,
                 stream)
-    _lib.check(rc, "varlen_attention_kv4")
+    _lib.check(rc, op)
     return out
 
 

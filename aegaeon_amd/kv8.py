@@ -9,7 +9,9 @@
   16-bit K/V rows, one layer or every layer of a step;
 * :func:`rotary_and_cache_kv8` — the same for one layer with keys and queries
   turned by their positions on the way;
-* :func:`gather_tokens_kv8` — the de-page back to 16-bit rows.
+* :func:`gather_tokens_kv8` — the de-page back to 16-bit rows;
+* :func:`paged_decode_attention_kv8` — decode attention, one query token per
+  sequence.
 
 Values (include/aegkv.h has the bytes): the 16 tokens of a block share a power of
 two per head and side (K or V), the rest of a value is an 8-bit float of three
@@ -25,8 +27,8 @@ import torch
 
 from . import _lib
 from ._gpu import device_guard, raw_stream
-from .attention import _DTYPES, _check_on, _int32_dense
-from .kv4 import _check_cu, _check_new_rows, _check_slots
+from .attention import _DTYPES, DecodePlan, _check_on, _int32_dense
+from .kv4 import _check_cu, _check_new_rows, _check_slots, _paged_decode
 from .rotary import _check_turned
 
 BLOCK_SIZE = 16
@@ -182,3 +184,26 @@ def gather_tokens_kv8(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_le
             raw_stream(dev))
     _lib.check(rc, "gather_tokens_kv8")
     return out_k, out_v
+
+
+def _layer_heads(c: torch.Tensor, head_dim: int) -> int:
+    return _kv_heads(c, False, head_dim)
+
+
+def paged_decode_attention_kv8(q: torch.Tensor, kv_cache: torch.Tensor,
+                               block_tables: Optional[torch.Tensor],
+                               seq_lens: Optional[torch.Tensor], scale: float, max_seq_len: int,
+                               out: Optional[torch.Tensor] = None, n_workgroups: int = 0,
+                               workspace: Optional[torch.Tensor] = None,
+                               plan: Optional[DecodePlan] = None) -> torch.Tensor:
+    """:func:`attention.paged_decode_attention` over one layer ``kv_cache
+    [N, R]`` of the 8-bit cache (any block stride): ``q [B, Hq, D]`` -> ``out
+    [B, Hq, D]``, both of the type the cache was written from.  Tables, lengths,
+    ``n_workgroups``, ``plan`` (a :class:`attention.DecodePlan` serves any of the
+    caches) and ``workspace`` (:func:`attention.attention_workspace`) are that
+    function's; a sequence without tokens gives zeros.  ``scale``: any number that
+    stays finite times log2 e.  New rows are appended by a call of their own,
+    before this one."""
+    return _paged_decode(_layer_heads, "aegkv_kv8_decode_attention", "paged_decode_attention_kv8",
+                         q, kv_cache, block_tables, seq_lens, scale, max_seq_len, out,
+                         n_workgroups, workspace, plan)

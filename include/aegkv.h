@@ -592,6 +592,29 @@ int aegkv_kv8_gather_tokens(const void* cache, int64_t cache_block_stride,
                             int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
                             aegkv_stream_t stream);
 
+/* aegkv_paged_decode_attention over a layer of the 8-bit cache: its arguments,
+ * limits, workspace (aegkv_paged_decode_attention_workspace_size) and plans
+ * (aegkv_paged_decode_plan), with one cache in place of two.  q and out are of
+ * the type that the cache was written from; scale is any that stays finite times
+ * log2 e. */
+int aegkv_kv8_decode_attention(void* out, int64_t out_batch_stride, const void* q,
+                               int64_t q_batch_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* seq_lens, int32_t batch, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                               float scale, int32_t dtype, int32_t n_workgroups, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream);
+int aegkv_kv8_decode_attention_planned(void* out, int64_t out_batch_stride, const void* q,
+                                       int64_t q_batch_stride, const void* cache,
+                                       int64_t cache_block_stride, int64_t n_blocks,
+                                       const void* plan, uint64_t plan_bytes,
+                                       const int32_t* seq_lens, int32_t batch,
+                                       int32_t max_seq_len, int32_t n_q_heads,
+                                       int32_t n_kv_heads, int32_t head_dim, float scale,
+                                       int32_t dtype, int32_t n_workgroups, void* workspace,
+                                       uint64_t workspace_bytes, aegkv_stream_t stream);
+
 /* ---- a8: node-wide block manager (host bookkeeping) ----------------------
  * Replaces the allocation and move bookkeeping of BlockManager
  * (aegaeon/aegaeon/block_manager.py:180-874).  Pure host code, no HIP calls;

@@ -238,6 +238,39 @@ def test_gather_host_checks(lib):
     assert call(longest=1 << 30, max_blocks=1 << 27) == UNSUP  # tiles past 32 bits
 
 
+def test_decode_host_checks(lib):
+    raw, p = _buf(1 << 16)
+
+    def attn(hq=28, hkv=4, d=128, dt=0, longest=64, max_blocks=4, ws=p, wsb=1 << 30, nwg=8, q=p,
+             cache=p, bs=16512, tables=p, blocks=8, scale=0.1):
+        return lib.aegkv_kv8_decode_attention(p, hq * d, q, hq * d, cache, bs, blocks, tables,
+                                              max_blocks, p, 2, longest, hq, hkv, d, scale, dt,
+                                              nwg, ws, wsb, None)
+
+    assert attn(hq=30) == INVALID and attn(d=96) == UNSUP and attn(dt=7) == UNSUP
+    assert attn(hq=34, hkv=2) == UNSUP       # 17 query heads per kv head
+    assert attn(hq=257, hkv=257, d=64) == UNSUP
+    assert attn(longest=100) == INVALID      # needs 7 blocks, the table has 4
+    assert attn(nwg=-1) == INVALID and attn(nwg=8193) == UNSUP
+    assert attn(cache=None) == INVALID and attn(tables=None) == INVALID and attn(blocks=0) == INVALID
+    assert attn(q=p + 2) == MISALIGNED and attn(cache=p + 8) == MISALIGNED
+    assert attn(bs=16520) == MISALIGNED
+    for bad in (float("nan"), float("inf"), 3e38):
+        assert attn(scale=bad) == INVALID
+    need = lib.aegkv_paged_decode_attention_workspace_size(2, 28, 4, 128, 64, 0, 8)
+    assert attn(ws=None) == WS and attn(wsb=need - 1) == WS
+
+    def planned(plan=p, nbytes=1 << 16, bs=16512):
+        return lib.aegkv_kv8_decode_attention_planned(p, 28 * 128, p, 28 * 128, p, bs, 8, plan,
+                                                      nbytes, p, 2, 64, 28, 4, 128, 0.1, 0, 8, p,
+                                                      1 << 30, None)
+
+    assert planned(plan=None) == INVALID
+    size = lib.aegkv_paged_decode_plan_size(2, 4, 64, 8)
+    assert planned(nbytes=size - 1) == INVALID
+    assert planned(bs=8) == MISALIGNED
+
+
 def test_python_entry_points_refuse_host_tensors():
     cache = kv8.kv8_cache(3, 2, 4, 128, device="cpu")
     assert cache.shape == (3, 2, 16512) and not cache.any()
@@ -255,3 +288,6 @@ def test_python_entry_points_refuse_host_tensors():
     with pytest.raises(ValueError):
         kv8.gather_tokens_kv8(cache, torch.zeros(1, 1, dtype=torch.int32),
                               torch.ones(1, dtype=torch.int32), 1, 1, 128)
+    with pytest.raises(ValueError):
+        kv8.paged_decode_attention_kv8(x[0], cache[:, 0], torch.zeros(5, 1, dtype=torch.int32),
+                                       torch.ones(5, dtype=torch.int32), 0.1, 1)
