@@ -22,8 +22,8 @@ LIB_PATH = PKG / "libaegkv.so"
 
 SOURCES = [
     "runtime.hip", "blocks.hip", "append.hip", "attention.hip", "inputs.hip",
-    "prefill.hip", "kv4.hip", "kv4_prefill.hip", "rotary.hip", "kv8.hip", "signals.hip",
-    "block_manager.cpp",
+    "prefill.hip", "kv4.hip", "kv4_prefill.hip", "rotary.hip", "kv8.hip",
+    "kv8_prefill.hip", "signals.hip", "block_manager.cpp",
 ]
 ARCH = "gfx950"
 

@@ -381,11 +381,18 @@ def varlen_attention_workspace(batch: int, total_q: int, max_seqlen_q: int, max_
                                device=None) -> Optional[torch.Tensor]:
     """A workspace for :func:`varlen_attention_kv4` calls of exactly these
     sizes on ``device`` (None when they need none)."""
+    return _varlen_workspace("aegkv_kv4_varlen_attention", batch, total_q, max_seqlen_q,
+                             max_seq_len, n_q_heads, n_kv_heads, head_dim, dtype, device)
+
+
+def _varlen_workspace(entry: str, batch: int, total_q: int, max_seqlen_q: int, max_seq_len: int,
+                      n_q_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype,
+                      device) -> Optional[torch.Tensor]:
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16 or float16")
     dev = _gpu(device)
     with device_guard(dev):
-        n = _lib.load().aegkv_kv4_varlen_attention_workspace_size(
+        n = getattr(_lib.load(), entry + "_workspace_size")(
             batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
             _DTYPES[dtype])
     if n < 0:

@@ -11,7 +11,9 @@
   turned by their positions on the way;
 * :func:`gather_tokens_kv8` — the de-page back to 16-bit rows;
 * :func:`paged_decode_attention_kv8` — decode attention, one query token per
-  sequence.
+  sequence;
+* :func:`varlen_attention_kv8` — attention of several query tokens per sequence: a
+  prompt's next chunk over what is cached of it, or drafted tokens.
 
 Values (include/aegkv.h has the bytes): the 16 tokens of a block share a power of
 two per head and side (K or V), the rest of a value is an 8-bit float of three
@@ -28,7 +30,8 @@ import torch
 from . import _lib
 from ._gpu import device_guard, raw_stream
 from .attention import _DTYPES, DecodePlan, _check_on, _int32_dense
-from .kv4 import _check_cu, _check_new_rows, _check_slots, _paged_decode
+from .kv4 import (_check_cu, _check_new_rows, _check_slots, _paged_decode, _varlen,
+                  _varlen_workspace)
 from .rotary import _check_turned
 
 BLOCK_SIZE = 16
@@ -207,3 +210,34 @@ def paged_decode_attention_kv8(q: torch.Tensor, kv_cache: torch.Tensor,
     return _paged_decode(_layer_heads, "aegkv_kv8_decode_attention", "paged_decode_attention_kv8",
                          q, kv_cache, block_tables, seq_lens, scale, max_seq_len, out,
                          n_workgroups, workspace, plan)
+
+
+def varlen_attention_kv8(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
+                         cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, max_seqlen_q: int,
+                         max_seq_len: int, scale: float, causal: bool = True,
+                         out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`kv4.varlen_attention_kv4` over one layer ``kv_cache [N, R]`` of the
+    8-bit cache: ``q [T, Hq, D]`` (any token stride, dense heads) -> ``out [T, Hq,
+    D]``, both of the type the cache was written from.  Sequence b's queries are
+    ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]`` (int32 on the GPU), the last of its
+    ``seq_lens[b]`` cached tokens (append them first); query i of m attends to keys
+    ``j <= seq_lens[b] - m + i``, all of them when not ``causal``, and gives zeros
+    without any.  ``max_seqlen_q`` and ``max_seq_len`` are host bounds: queries past
+    the first are left alone, keys past the second not attended.  head_dim 64 or
+    128.  ``workspace``: :func:`varlen_attention_workspace` (reusable on one stream,
+    by one thread at a time); by default one per (device, stream) that threads may
+    share."""
+    return _varlen(_layer_heads, "aegkv_kv8_varlen_attention", "varlen_attention_kv8", q, kv_cache,
+                   block_tables, cu_seqlens_q, seq_lens, max_seqlen_q, max_seq_len, scale, causal,
+                   out, workspace)
+
+
+def varlen_attention_workspace(batch: int, total_q: int, max_seqlen_q: int, max_seq_len: int,
+                               n_q_heads: int, n_kv_heads: int, head_dim: int,
+                               dtype: torch.dtype = torch.bfloat16,
+                               device=None) -> Optional[torch.Tensor]:
+    """A workspace for :func:`varlen_attention_kv8` calls of exactly these sizes
+    on ``device`` (None when they need none)."""
+    return _varlen_workspace("aegkv_kv8_varlen_attention", batch, total_q, max_seqlen_q,
+                             max_seq_len, n_q_heads, n_kv_heads, head_dim, dtype, device)

@@ -615,6 +615,23 @@ int aegkv_kv8_decode_attention_planned(void* out, int64_t out_batch_stride, cons
                                        int32_t dtype, int32_t n_workgroups, void* workspace,
                                        uint64_t workspace_bytes, aegkv_stream_t stream);
 
+/* aegkv_kv4_varlen_attention over a layer of the 8-bit cache: its arguments,
+ * limits, masks and workspace.  An infinity or NaN that was appended shows in the
+ * rows that attend to its token (of V: in that dim), and in no others. */
+int64_t aegkv_kv8_varlen_attention_workspace_size(int32_t batch, int64_t total_q,
+                                                  int32_t max_seqlen_q, int32_t max_seq_len,
+                                                  int32_t n_q_heads, int32_t n_kv_heads,
+                                                  int32_t head_dim, int32_t dtype);
+int aegkv_kv8_varlen_attention(void* out, int64_t out_token_stride, const void* q,
+                               int64_t q_token_stride, const void* cache,
+                               int64_t cache_block_stride, int64_t n_blocks,
+                               const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* cu_seqlens_q, const int32_t* seq_lens, int32_t batch,
+                               int64_t total_q, int32_t max_seqlen_q, int32_t max_seq_len,
+                               int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                               int32_t causal, int32_t dtype, void* workspace,
+                               uint64_t workspace_bytes, aegkv_stream_t stream);
+
 /* ---- a8: node-wide block manager (host bookkeeping) ----------------------
  * Replaces the allocation and move bookkeeping of BlockManager
  * (aegaeon/aegaeon/block_manager.py:180-874).  Pure host code, no HIP calls;
