@@ -46,12 +46,15 @@ struct Append8Args {
   uint32_t n_tasks;            // waves in all
 };
 
-// The largest of the wave's values, in every lane.
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+// The largest value of the lane's 16, and of the wave, in every lane.
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
   x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));   // lane ^ 1
   x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));   // lane ^ 2
   x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xf, 0xf, true));  // row_ror 4
-  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));  // row_ror 8
+  return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true));  // row_ror 8
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = row_max(x);
   const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   x = max(a[0], a[1]);
   const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
@@ -74,75 +77,105 @@ __device__ __forceinline__ void floats4(uint32_t w, float (&f)[4]) {
   const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true));
   f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
 }
-// infinities to NaN (magnitude bits `u`)
-__device__ __forceinline__ float not_infinite(float x, uint32_t u) {
-  return u >= 0x7f800000u ? __builtin_nanf("") : x;
+// The wave's part of a call: a head and side of a layer.
+struct Side {
+  const uint8_t* rows;  // of token 0
+  int64_t tok_b;
+  uint8_t* layer;       // the layer's part of block 0
+  int64_t codes, scale; // offsets there
+  bool value;
+};
+__device__ __forceinline__ Side side_of(const Append8Args& a, uint32_t layer, uint32_t head,
+                                        bool value, int dim) {
+  const HeadRows& h = value ? a.v : a.k;
+  return {h.src + layer * (value ? a.v_layer_b : a.k_layer_b) + (int64_t)head * dim * 2,
+          h.src_tok_b, a.cache + layer * a.layer_b,
+          (int64_t)(2 * head + (value ? 1 : 0)) * kv8_side_bytes(dim), a.scales_at + 4 * head,
+          value};
 }
 
-// One run: the tokens of lanes i .. i + n - 1 of the window, all of block blk.
-// src[k]: the lane of the window whose token goes to place 4 g + k (-1: none).
-template <int DT, int D, int TURN>
-__device__ __forceinline__ void append_run(const Append8Args& a, uint32_t layer, uint32_t head,
-                                           bool value, int64_t tok_at_lane0, int64_t blk,
-                                           const int (&src)[4], bool anew) {
-  constexpr int NC = D > 128 ? D / 128 : 1;  // chunks of a lane
+// Chunk c of four tokens' rows (tok < 0: none, zeros) in 32 bits, turned if they are
+// keys: the loads of all four are in flight together.  top: the largest of the
+// finite magnitudes' bits; bad: there are others, which become NaN.
+template <int DT, int TURN>
+__device__ __forceinline__ void load_rows(const Append8Args& a, const Side& s, const int64_t (&tok)[4],
+                                          int c, float (&f)[4][8], uint32_t (&top)[4],
+                                          bool (&bad)[4]) {
   constexpr bool INTER = TURN == kNeighbours;
-  const int lane = threadIdx.x & 63, g = lane >> 4, c0 = lane & 15;
-  const bool idle = D < 128 && c0 >= D / 8;
-  const HeadRows& h = value ? a.v : a.k;
-  const uint8_t* rows = h.src + layer * (value ? a.v_layer_b : a.k_layer_b) + (int64_t)head * D * 2;
-  uint8_t* rec = a.cache + blk * a.blk_b + layer * a.layer_b;
-  uint8_t* scale = rec + a.scales_at + 4 * head;
-  rec += (int64_t)(2 * head + (value ? 1 : 0)) * kv8_side_bytes(D);
-  int old = Kv8Elem<DT>::kLow;
-  if (!anew) old = scale[value ? 1 : 0];
-  float f[NC][4][8];
-  uint32_t top = 0;
-  bool bad = false;
+  const bool turns = TURN != kStill && !s.value && chunk_turns(a.r, c);
+  u32x4 x[4], y[4];
 #pragma unroll
-  for (int q = 0; q < NC; ++q) {
-    const int c = c0 + 16 * q;
-    u32x4 x[4], y[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[k] = y[k] = u32x4{0u, 0u, 0u, 0u};
-      if (src[k] >= 0 && !idle) {
-        const uint8_t* p = rows + (tok_at_lane0 + src[k]) * h.src_tok_b;
-        x[k] = *reinterpret_cast<const u32x4*>(p + 16 * c);
-        if (TURN != kStill && !value && chunk_turns(a.r, c))
-          y[k] = *reinterpret_cast<const u32x4*>(p + 16 * partner_chunk<INTER>(a.r, c));
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      bool turned = false;
-      if constexpr (TURN != kStill) {
-        if (src[k] >= 0 && !idle && !value && chunk_turns(a.r, c)) {
-          turn_chunk<DT, INTER>(
-              x[k], y[k], load_angles<INTER>(a.r, a.r.positions[tok_at_lane0 + src[k]], c),
-              f[q][k]);
-          turned = true;
-        }
-      }
-      if (!turned) unpack8<DT>(x[k], f[q][k]);
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const uint32_t u = __float_as_uint(f[q][k][d]) & 0x7fffffffu;
-        bad |= u >= 0x7f800000u;
-        top = max(top, u >= 0x7f800000u ? 0u : u);
-        f[q][k][d] = not_infinite(f[q][k][d], u);
-      }
+  for (int k = 0; k < 4; ++k) {
+    x[k] = y[k] = u32x4{0u, 0u, 0u, 0u};
+    if (tok[k] >= 0) {
+      const uint8_t* p = s.rows + tok[k] * s.tok_b;
+      x[k] = *reinterpret_cast<const u32x4*>(p + 16 * c);
+      if (turns) y[k] = *reinterpret_cast<const u32x4*>(p + 16 * partner_chunk<INTER>(a.r, c));
     }
   }
-  top = wave_max(top);
-  const bool nan = __builtin_amdgcn_ballot_w64(bad) != 0;
-  const int held = __builtin_amdgcn_readfirstlane(old);  // (0 in a cache never written)
-  old = min(max(held, Kv8Elem<DT>::kLow), Kv8Elem<DT>::kTop);
-  const int own = kv8_scale_byte<DT>(top);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (TURN != kStill && turns && tok[k] >= 0)
+      turn_chunk<DT, INTER>(x[k], y[k], load_angles<INTER>(a.r, a.r.positions[tok[k]], c), f[k]);
+    else
+      unpack8<DT>(x[k], f[k]);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const uint32_t u = __float_as_uint(f[k][d]) & 0x7fffffffu;
+      const bool odd = u >= 0x7f800000u;
+      bad[k] |= odd;
+      top[k] = max(top[k], odd ? 0u : u);
+      f[k][d] = odd ? __builtin_nanf("") : f[k][d];
+    }
+  }
+}
+// A held scale byte within the type's bounds.
+template <int DT>
+__device__ __forceinline__ int held_scale(int byte) {
+  return min(max(byte, Kv8Elem<DT>::kLow), Kv8Elem<DT>::kTop);
+}
+// A word of codes under an exponent that is larger by the factor's inverse.
+__device__ __forceinline__ uint32_t rescaled(uint32_t w, float down) {
+  float t[4];
+  floats4(w, t);
+  return codes4(t[0] * down, t[1] * down, t[2] * down, t[3] * down);
+}
+__device__ __forceinline__ float down_factor(int from, int to) {
+  return kv8_scale((uint32_t)max(127 + from - to, 0));
+}
+
+// One run: tokens of block blk; tok[k]: the one for place 4 g + k.
+template <int DT, int D, int TURN>
+__device__ __forceinline__ void append_run(const Append8Args& a, const Side& s, int64_t blk,
+                                           int64_t (&tok)[4], bool anew) {
+  constexpr int NC = D > 128 ? D / 128 : 1;  // chunks of a lane
+  const int lane = threadIdx.x & 63, g = lane >> 4, c0 = lane & 15;
+  const bool idle = D < 128 && c0 >= D / 8;
+  bool here[4];  // places that get a token
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (idle) tok[k] = -1;
+    here[k] = tok[k] >= 0;
+  }
+  uint8_t* rec = s.layer + blk * a.blk_b;
+  uint8_t* scale = rec + s.scale;
+  rec += s.codes;
+  int held = Kv8Elem<DT>::kLow;
+  if (!anew) held = scale[s.value ? 1 : 0];
+  float f[NC][4][8];
+  uint32_t top[4] = {};
+  bool bad[4] = {};
+#pragma unroll
+  for (int q = 0; q < NC; ++q) load_rows<DT, TURN>(a, s, tok, c0 + 16 * q, f[q], top, bad);
+  const bool nan = __builtin_amdgcn_ballot_w64(bad[0] || bad[1] || bad[2] || bad[3]) != 0;
+  const int own =
+      kv8_scale_byte<DT>(wave_max(max(max(top[0], top[1]), max(top[2], top[3]))));
+  held = __builtin_amdgcn_readfirstlane(held);  // (0 in a cache never written)
+  const int old = held_scale<DT>(held);
   const int now = anew ? own : max(old, own);
   const float inv = kv8_scale((uint32_t)(254 - now));  // 2^-e
   const bool rescale = !anew && now > old;             // uniform
-  const float down = kv8_scale((uint32_t)max(127 + old - now, 0));
+  const float down = down_factor(old, now);
   if (!idle) {
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
@@ -152,24 +185,22 @@ __device__ __forceinline__ void append_run(const Append8Args& a, uint32_t layer,
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int d = 0; d < 8; ++d) f[q][k][d] *= inv;
-      if (!value) {
+      if (!s.value) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           u32x2* p = reinterpret_cast<u32x2*>(rec + kv8_k_byte(4 * g + k, c));
           u32x2 w = {codes4(f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3]),
                      codes4(f[q][k][4], f[q][k][5], f[q][k][6], f[q][k][7])};
-          if (rescale && src[k] < 0) {
+          if (rescale && !here[k]) {
             const u32x2 o = *p;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float t[4];
-              floats4(o[i], t);
-              w[i] = codes4(t[0] * down, t[1] * down, t[2] * down, t[3] * down);
-            }
+            w = u32x2{rescaled(o[0], down), rescaled(o[1], down)};
           }
-          if (anew || rescale || src[k] >= 0) *p = w;
+          if (anew || rescale || here[k]) *p = w;
         }
       } else {
+        uint32_t mine = 0;  // bytes of a word that get a token
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mine |= here[k] ? 0xffu << (8 * k) : 0u;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint8_t* p = rec + kv8_v_byte<D>(g, 2 * c + i);
@@ -181,22 +212,14 @@ __device__ __forceinline__ void append_run(const Append8Args& a, uint32_t layer,
           if (rescale) {
             const u32x4 o = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              float t[4];
-              floats4(o[d], t);
-              const uint32_t r = codes4(t[0] * down, t[1] * down, t[2] * down, t[3] * down);
-              uint32_t mine = 0;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mine |= src[k] >= 0 ? 0xffu << (8 * k) : 0u;
-              w[d] = (w[d] & mine) | (r & ~mine);
-            }
+            for (int d = 0; d < 4; ++d) w[d] = (w[d] & mine) | (rescaled(o[d], down) & ~mine);
           }
-          if (anew || rescale || (src[0] >= 0 && src[1] >= 0 && src[2] >= 0 && src[3] >= 0)) {
+          if (anew || rescale || mine == 0xffffffffu) {
             *reinterpret_cast<u32x4*>(p) = w;
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (src[k] >= 0) {
+              if (here[k]) {
 #pragma unroll
                 for (int d = 0; d < 4; ++d) p[4 * d + k] = (uint8_t)(w[d] >> (8 * k));
               }
@@ -206,8 +229,105 @@ __device__ __forceinline__ void append_run(const Append8Args& a, uint32_t layer,
     }
   }
   if (lane == 0) {
-    if (anew || now != held) scale[value ? 1 : 0] = (uint8_t)now;
-    if (value && (anew || nan)) scale[2] = nan ? 1 : 0;
+    if (anew || now != held) scale[s.value ? 1 : 0] = (uint8_t)now;
+    if (s.value && (anew || nan)) scale[2] = nan ? 1 : 0;
+  }
+}
+
+// Up to 16 runs of one token each, as a decode step's: the lanes 16 g .. take the
+// window's tokens 4 k + g, every load of the four in flight together (28 layers of
+// 128 tokens of 4 heads of 128: 12.6 us, one run after the other 27.4; V's words read
+// and written whole instead of their bytes 12.1, but prompts, whose waves it leaves
+// fewer registers, 5-15% slower).  tok[k] (-1: none) goes to place off[k] of block
+// blk[k].
+template <int DT, int D, int TURN>
+__device__ __forceinline__ void append_singles(const Append8Args& a, const Side& s,
+                                               int64_t (&tok)[4], const int (&blk)[4],
+                                               const int (&off)[4]) {
+  constexpr int NC = D > 128 ? D / 128 : 1;
+  const int lane = threadIdx.x & 63, c0 = lane & 15;
+  const bool idle = D < 128 && c0 >= D / 8;
+  bool run[4];
+  uint8_t* rec[4];
+  int held[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    run[k] = tok[k] >= 0;
+    if (idle) tok[k] = -1;
+    rec[k] = s.layer + (int64_t)(run[k] ? blk[k] : 0) * a.blk_b;
+    held[k] = Kv8Elem<DT>::kLow;
+    if (run[k] && off[k] > 0) held[k] = rec[k][s.scale + (s.value ? 1 : 0)];
+  }
+  float f[NC][4][8];
+  uint32_t top[4] = {};
+  bool bad[4] = {};
+#pragma unroll
+  for (int q = 0; q < NC; ++q) load_rows<DT, TURN>(a, s, tok, c0 + 16 * q, f[q], top, bad);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool nan = (__builtin_amdgcn_ballot_w64(bad[k]) >> (lane & 48) & 0xffffu) != 0;
+    const int own = kv8_scale_byte<DT>(row_max(top[k]));
+    const bool anew = off[k] == 0;
+    const int old = held_scale<DT>(held[k]);
+    const int now = anew ? own : max(old, own);
+    const float inv = kv8_scale((uint32_t)(254 - now));
+    const float down = down_factor(old, now);
+    uint8_t* scale = rec[k] + s.scale;
+    uint8_t* side = rec[k] + s.codes;
+    if (run[k] && !idle) {
+#pragma unroll
+      for (int q = 0; q < NC; ++q) {
+        const int c = c0 + 16 * q;
+        uint32_t w[2];  // the token's codes, a byte a dim
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          w[i] = codes4(f[q][k][4 * i] * inv, f[q][k][4 * i + 1] * inv, f[q][k][4 * i + 2] * inv,
+                        f[q][k][4 * i + 3] * inv);
+        if (anew || now > old) {  // the whole block: zeros, or what it holds rounded once more
+          if (!s.value) {
+#pragma unroll 1
+            for (int r = 0; r < kKv8Tokens; ++r) {
+              u32x2* p = reinterpret_cast<u32x2*>(side + kv8_k_byte(r, c));
+              u32x2 o = {0u, 0u};
+              if (!anew) {
+                o = *p;
+                o = u32x2{rescaled(o[0], down), rescaled(o[1], down)};
+              }
+              *p = r == off[k] ? u32x2{w[0], w[1]} : o;
+            }
+          } else {
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+              const uint32_t sh = 8 * (off[k] & 3), mine = g == off[k] >> 2 ? 0xffu << sh : 0u;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                u32x4* p = reinterpret_cast<u32x4*>(side + kv8_v_byte<D>(g, 2 * c + i));
+                u32x4 o = {0u, 0u, 0u, 0u};
+                if (!anew) o = *p;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                  o[d] = ((w[i] >> (8 * d) << sh) & mine) |
+                         ((anew ? 0u : rescaled(o[d], down)) & ~mine);
+                *p = o;
+              }
+            }
+          }
+        } else if (!s.value) {
+          *reinterpret_cast<u32x2*>(side + kv8_k_byte(off[k], c)) = u32x2{w[0], w[1]};
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint8_t* p = side + kv8_v_byte<D>(off[k] >> 2, 2 * c + i) + (off[k] & 3);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) p[4 * d] = (uint8_t)(w[i] >> (8 * d));
+          }
+        }
+      }
+    }
+    if (run[k] && c0 == 0) {
+      if (anew || now != held[k]) scale[s.value ? 1 : 0] = (uint8_t)now;
+      if (s.value && (anew || nan)) scale[2] = nan ? 1 : 0;
+    }
   }
 }
 
@@ -228,9 +348,24 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
   if (tok >= 0 && tok < a.n_tokens) s = a.slots[tok];
   const bool in = s >= 0 && s < a.n_slots;
   const int blk = in ? (int)(s / kKv8Tokens) : -1, off = (int)(s & (kKv8Tokens - 1));
-  const int before = __shfl_up(blk, 1);
-  uint64_t heads = __builtin_amdgcn_ballot_w64(lane > 0 && lane <= (int)a.window && in &&
-                                               blk != before);
+  const int before = __shfl_up(blk, 1), behind = __shfl_down(blk, 1);  // (every lane active)
+  const bool begins = lane > 0 && lane <= (int)a.window && in && blk != before;
+  uint64_t heads = __builtin_amdgcn_ballot_w64(begins);
+  if (!heads) return;  // uniform
+  const Side side = side_of(a, layer, head, value, D);
+  if (a.window > 1 && __builtin_amdgcn_ballot_w64(begins && blk == behind) == 0) {
+    int64_t at[4];
+    int b[4], o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = 1 + 4 * k + g;  // the token's lane, at most 16
+      b[k] = __shfl(blk, i);
+      o[k] = __shfl(off, i);
+      at[k] = heads >> i & 1 ? first + i : -1;
+    }
+    append_singles<DT, D, TURN>(a, side, at, b, o);
+    return;
+  }
   while (heads) {  // uniform
     const int i = __builtin_ctzll(heads);
     heads &= heads - 1;
@@ -238,7 +373,7 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
     const uint64_t same = __builtin_amdgcn_ballot_w64(blk == b) >> i;
     const int n = ~same ? __builtin_ctzll(~same) : 64;  // tokens of the run (i > 0: below 64)
     const int off0 = __builtin_amdgcn_readlane(off, i);
-    int src[4];
+    int64_t at[4];
     bool anew;
     const uint64_t run = n < 64 ? (1ull << n) - 1 : ~0ull;
     const uint64_t in_order = __builtin_amdgcn_ballot_w64(off == off0 + lane - i) >> i;
@@ -246,21 +381,21 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 4 * g + k - off0;
-        src[k] = r >= 0 && r < n ? i + r : -1;
+        at[k] = r >= 0 && r < n ? first + i + r : -1;
       }
       anew = off0 == 0;
     } else {  // of two tokens for one place the later one
 #pragma unroll
-      for (int k = 0; k < 4; ++k) src[k] = -1;
+      for (int k = 0; k < 4; ++k) at[k] = -1;
       anew = false;
       for (int x = i; x < i + n; ++x) {
         const int o = __builtin_amdgcn_readlane(off, x);
         anew |= o == 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) src[k] = o == 4 * g + k ? x : src[k];
+        for (int k = 0; k < 4; ++k) at[k] = o == 4 * g + k ? first + x : at[k];
       }
     }
-    append_run<DT, D, TURN>(a, layer, head, value, first, b, src, anew);
+    append_run<DT, D, TURN>(a, side, b, at, anew);
   }
 }
 
@@ -489,9 +624,9 @@ void launch_gather(const Gather8Args& a, int32_t head_dim, dim3 g, hipStream_t s
 }
 
 // Tokens of a wave's window.  A wave looks for the runs that begin there and writes
-// them one after the other, so 1 is best while the waves fit the chip; of a prompt,
-// 15 of 16 tokens begin none.
-constexpr uint64_t kAppend8Waves = 16384;
+// longer ones one after the other, so 1 is best while the waves fit the chip; of a
+// prompt 15 of 16 tokens begin none.
+constexpr uint64_t kAppend8Waves = 2048;
 uint32_t window_of(uint64_t waves_of_one) {
   uint32_t w = 1;
   while (w < 16 && waves_of_one > kAppend8Waves * w) w *= 2;

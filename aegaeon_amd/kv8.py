@@ -174,8 +174,9 @@ def gather_tokens_kv8(kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_le
         torch.cumsum(sl, 0, dtype=torch.int32, out=cu_seqlens[1:])
     else:
         _check_cu(cu_seqlens, "cu_seqlens", sl.numel(), dev)
-    out_k = torch.empty((count, total_tokens, H, head_dim), dtype=dtype, device=dev)
-    out_v = torch.empty_like(out_k)
+    # (views of one allocation: a microsecond less of the host)
+    out_k, out_v = torch.empty((2, count, total_tokens, H, head_dim), dtype=dtype,
+                               device=dev).unbind(0)
     if total_tokens == 0:
         return out_k, out_v
     with device_guard(dev):

@@ -11,7 +11,7 @@ Everything is enqueued on the current torch stream.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -33,22 +33,6 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
 
 
-def _check_table(table: torch.Tensor, head_dim: int, dev: torch.device) -> None:
-    _check_on(table, "table", dev)
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError("table must be a contiguous float32 tensor [positions, rotary_dim]")
-    if table.size(0) == 0 or table.size(1) == 0 or table.size(1) > head_dim:
-        raise ValueError(f"table must have rows of up to head_dim {head_dim} entries")
-
-
-def _check_token_ids(x: torch.Tensor, name: str, tokens: int, dev: torch.device) -> torch.Tensor:
-    _check_on(x, name, dev)
-    if x.dtype != torch.int64 or x.dim() != 1 or x.numel() < tokens:
-        raise ValueError(f"{name} must be an int64 GPU tensor with an entry for each of the "
-                         f"{tokens} tokens")
-    return x.contiguous()
-
-
 def _check_like(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
     if t.shape != x.shape or t.dtype != x.dtype:
         raise ValueError(f"{name} must have the shape and dtype {tuple(x.shape)}, {x.dtype}")
@@ -58,60 +42,68 @@ def _check_like(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def _span(t: torch.Tensor):
-    """First byte and the byte past the last of rows ``[T, H, D]``."""
-    first = t.data_ptr()
-    return first, first + ((t.size(0) - 1) * t.stride(0) + t.size(1) * t.size(2)) * 2
+    """First byte, the byte past the last and the token stride in bytes of rows
+    ``[T, H, D]``."""
+    T, H, D = t.shape
+    first, step = t.data_ptr(), 2 * t.stride(0)
+    return first, first + (T - 1) * step + 2 * H * D, step, 2 * H * D
 
 
-def _check_apart(t: torch.Tensor, x: torch.Tensor, name: str, of: str, same: bool) -> None:
-    """``t``, written, may be ``x``, read (``same``), or must not share bytes
-    with it."""
-    if same and t.data_ptr() == x.data_ptr() and t.stride() == x.stride():
-        return
-    (a, b), (c, d) = _span(t), _span(x)
-    # rows of one wider buffer (the slices of a fused projection) interleave
-    if a < d and c < b and not (t.stride(0) == x.stride(0) and _columns_apart(t, x)):
+def _check_apart(name: str, written, read, same: Tuple[str, ...]) -> None:
+    """``written``, a span, may be one of ``read``'s spans that ``same`` names,
+    and shares no byte with the others."""
+    a, b, step, row = written
+    for of, (c, d, other_step, other_row) in read.items():
+        if a >= d or c >= b or (of in same and a == c and step == other_step):
+            continue
+        # slices of one wider buffer (a fused projection's columns) lie side by side
+        if step == other_step and step > 0:
+            off = (c - a) % step
+            if off >= row and off + other_row <= step:
+                continue
         raise ValueError(f"{name} overlaps {of}")
-
-
-def _columns_apart(t: torch.Tensor, x: torch.Tensor) -> bool:
-    step = t.stride(0) * 2
-    if step == 0:
-        return False
-    off = (x.data_ptr() - t.data_ptr()) % step
-    return off >= t.size(1) * t.size(2) * 2 and off + x.size(1) * x.size(2) * 2 <= step
 
 
 def _check_turned(query, key, value, slot_mapping, positions, table, out, out_key, dev,
                   key_in_place: bool):
     """The arguments that both caches' calls share; (slots, positions, out)."""
-    for x, n in ((query, "query"), (key, "key"), (value, "value")):
-        if x.dim() != 3:
-            raise ValueError(f"{n} must be [tokens, heads, head_dim]")
-        _check_rows(x, n)
-        _check_on(x, n, dev)
-    T, _, D = query.shape
-    if key.size(0) != T or key.size(2) != D or value.shape != key.shape:
-        raise ValueError("key and value must be [T, Hkv, D] with query's tokens and head_dim")
-    if query.dtype not in _DTYPES or key.dtype != query.dtype or value.dtype != query.dtype:
+    qs, ks, dtype = query.shape, key.shape, query.dtype
+    if len(qs) != 3 or len(ks) != 3 or value.shape != ks or ks[0] != qs[0] or ks[2] != qs[2]:
+        raise ValueError("query must be [T, Hq, D], key and value [T, Hkv, D] with its tokens "
+                         "and head_dim")
+    if dtype not in _DTYPES or key.dtype != dtype or value.dtype != dtype:
         raise ValueError("query, key and value must share a bf16/fp16 dtype")
-    _check_table(table, D, dev)
-    slots = _check_token_ids(slot_mapping, "slot_mapping", T, dev)
-    positions = _check_token_ids(positions, "positions", T, dev)
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-    elif T > 0:
-        _check_like(out, query, "out")
-        _check_apart(out, query, "out", "query", True)
-        _check_apart(out, key, "out", "key", False)
-        _check_apart(out, value, "out", "value", False)
-    if out_key is not None and T > 0:
-        _check_like(out_key, key, "out_key")
-        _check_apart(out_key, key, "out_key", "key", key_in_place)
-        _check_apart(out_key, query, "out_key", "query", False)
-        _check_apart(out_key, value, "out_key", "value", False)
-        _check_apart(out_key, out, "out_key", "out", False)
-    return slots, positions, out
+    T, _, D = qs
+    index = dev.index
+    for x, n in ((query, "query"), (key, "key"), (value, "value")):
+        strides = x.stride()
+        if x.get_device() != index or strides[2] != 1 or strides[1] != D:
+            _check_on(x, n, dev)
+            _check_rows(x, n)
+    for x, n in ((slot_mapping, "slot_mapping"), (positions, "positions")):
+        if x.get_device() != index:
+            _check_on(x, n, dev)
+        if x.dtype != torch.int64 or x.dim() != 1 or x.numel() < T:
+            raise ValueError(f"{n} must be an int64 GPU tensor with an entry for each of the {T} "
+                             "tokens")
+    if table.get_device() != index:
+        _check_on(table, "table", dev)
+    ts = table.shape
+    if table.dtype != torch.float32 or len(ts) != 2 or not table.is_contiguous() or ts[0] == 0 \
+            or not 0 < ts[1] <= D:
+        raise ValueError("table must be a contiguous float32 tensor [positions, rotary_dim] with "
+                         f"rows of up to head_dim {D} entries")
+    if T > 0 and (out is not None or out_key is not None):
+        read = {"query": _span(query), "key": _span(key), "value": _span(value)}
+        if out is not None:
+            written = _span(_check_like(out, query, "out"))
+            _check_apart("out", written, read, ("query",))
+            read["out"] = written
+        if out_key is not None:
+            _check_apart("out_key", _span(_check_like(out_key, key, "out_key")), read,
+                         ("key",) if key_in_place else ())
+    return slot_mapping.contiguous(), positions.contiguous(), \
+        query.new_empty(qs) if out is None else out
 
 
 def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
