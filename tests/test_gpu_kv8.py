@@ -108,14 +108,26 @@ def test_append_of_every_16_bit_pattern(device, dtype, D, order):
 
 
 @pytest.mark.parametrize("slots", [
-    [20, 19, 18, 17], [31, 16, 20], [16, 16, 17], [21, 20, 20, 22, 20], [40, 21, 22, 41, 5, 0]])
+    [20, 19, 18, 17], [31, 16, 20], [16, 16, 17], [21, 20, 20, 22, 20], [40, 21, 22, 63, 5, 0]])
 def test_slots_in_any_order_within_a_block(device, slots):
-    """Descending, scattered, the same slot twice (the later row counts)."""
+    """Descending, scattered, the same slot twice (the later row counts), the tokens
+    of a block next to each other."""
     rng = np.random.default_rng(len(slots) + slots[0])
     cache = _filled(rng, 4, 2, 3, 128, "bf16")
     k, v = (_rows(rng, (2, len(slots), 3, 128), "bf16") for _ in range(2))
-    if slots == [40, 21, 22, 41, 5, 0]:  # block 2, block 1, block 2 again: only the
-        slots = [40, 21, 22, 63, 5, 0]   # tokens of a block next to each other are defined
+    dev = _append(device, k, v, cache, slots, "bf16")
+    assert np.array_equal(dev.cpu().numpy(), cache)
+
+
+@pytest.mark.parametrize("n", [46, 47, 48, 64, 200])
+@pytest.mark.parametrize("before", [0, 5])
+def test_places_given_many_times(device, n, before):
+    """The last row for each place counts, however many there are for one block: a
+    batch padded with rows for one slot."""
+    rng = np.random.default_rng(n + before)
+    cache = _filled(rng, 4, 2, 3, 128, "bf16")
+    slots = [0] * before + [int(x) for x in 16 + rng.integers(0, 16, n)] + [32] * n
+    k, v = (_rows(rng, (2, len(slots), 3, 128), "bf16") for _ in range(2))
     dev = _append(device, k, v, cache, slots, "bf16")
     assert np.array_equal(dev.cpu().numpy(), cache)
 
