@@ -32,7 +32,7 @@ from ._gpu import device_guard, raw_stream
 from .attention import _DTYPES, DecodePlan, _check_on, _int32_dense
 from .kv4 import (_check_cu, _check_new_rows, _check_slots, _paged_decode, _varlen,
                   _varlen_workspace)
-from .rotary import _check_turned
+from .rotary import _turn_args
 
 BLOCK_SIZE = 16
 MAX_KV_HEADS = 256
@@ -81,7 +81,7 @@ def reshape_and_cache_kv8(key: torch.Tensor, value: torch.Tensor, kv_cache: torc
     slots past the cache are skipped.  A row at a block's first token begins the
     block anew; others join what it holds, whose values are rounded once more
     where their size raises the block's exponent.  The rows of one block must
-    follow each other in the call."""
+    follow each other in the call; of several for one slot the last counts."""
     _check_new_rows(key, value, 3, "[T, Hkv, D]")
     _append(key.unsqueeze(0), value.unsqueeze(0), kv_cache.unsqueeze(1), slot_mapping,
             "reshape_and_cache_kv8")
@@ -124,23 +124,17 @@ def rotary_and_cache_kv8(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     8-bit cache, with :func:`reshape_and_cache_kv8`'s slots and blocks: returns the
     turned queries.  The codes are those of the turned keys in fp32, without a
     rounding to 16 bits between; ``out_key``, in 16 bits, must not be ``key``."""
-    slots, positions, out = _check_turned(query, key, value, slot_mapping, positions, table, out,
-                                          out_key, kv_cache.device, False)
-    T, Hq, D = query.shape
-    if _kv_heads(kv_cache, False, D) != key.size(1):
-        raise ValueError("key/value and kv_cache disagree on the kv heads")
-    if T == 0:
-        return out
     dev = kv_cache.device
+    args, out, keep = _turn_args(query, key, value, slot_mapping, positions, table, interleaved,
+                                 out, out_key, dev, False)
+    if _kv_heads(kv_cache, False, args[12]) != args[11]:
+        raise ValueError("key/value and kv_cache disagree on the kv heads")
+    if args[15] == 0:
+        return out
     with device_guard(dev):
-        rc = _lib.load().aegkv_kv8_rotary_append(
-            query.data_ptr(), query.stride(0), out.data_ptr(), out.stride(0), Hq, key.data_ptr(),
-            key.stride(0), value.data_ptr(), value.stride(0),
-            None if out_key is None else out_key.data_ptr(),
-            0 if out_key is None else out_key.stride(0), key.size(1), D, slots.data_ptr(),
-            positions.data_ptr(), T, table.data_ptr(), table.size(0), table.size(1),
-            int(bool(interleaved)), kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.size(0),
-            _DTYPES[query.dtype], raw_stream(dev))
+        rc = _lib.load().aegkv_kv8_rotary_append(*args, kv_cache.data_ptr(), kv_cache.stride(0),
+                                                 kv_cache.size(0), _DTYPES[query.dtype],
+                                                 raw_stream(dev))
     _lib.check(rc, "rotary_and_cache_kv8")
     return out
 

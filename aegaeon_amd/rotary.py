@@ -33,28 +33,19 @@ def rotary_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
     return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
 
 
-def _check_like(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
-    if t.shape != x.shape or t.dtype != x.dtype:
-        raise ValueError(f"{name} must have the shape and dtype {tuple(x.shape)}, {x.dtype}")
-    _check_rows(t, name)
-    _check_on(t, name, x.device)
-    return t
-
-
-def _span(t: torch.Tensor):
-    """First byte, the byte past the last and the token stride in bytes of rows
-    ``[T, H, D]``."""
-    T, H, D = t.shape
-    first, step = t.data_ptr(), 2 * t.stride(0)
-    return first, first + (T - 1) * step + 2 * H * D, step, 2 * H * D
+def _dense_rows(x: torch.Tensor, name: str, dev: torch.device, strides, head_dim: int) -> None:
+    if x.get_device() != dev.index or strides[2] != 1 or strides[1] != head_dim:
+        _check_on(x, name, dev)
+        _check_rows(x, name)
 
 
 def _check_apart(name: str, written, read, same: Tuple[str, ...]) -> None:
-    """``written``, a span, may be one of ``read``'s spans that ``same`` names,
-    and shares no byte with the others."""
-    a, b, step, row = written
-    for of, (c, d, other_step, other_row) in read.items():
-        if a >= d or c >= b or (of in same and a == c and step == other_step):
+    """``written``, rows given as (first byte, token stride, row bytes, byte past
+    the last), may be those of ``read`` that ``same`` names, and shares no byte with
+    the others."""
+    a, step, row, b = written
+    for of, (c, other_step, other_row, d) in read:
+        if a >= d or c >= b or (a == c and step == other_step and of in same):
             continue
         # slices of one wider buffer (a fused projection's columns) lie side by side
         if step == other_step and step > 0:
@@ -64,46 +55,74 @@ def _check_apart(name: str, written, read, same: Tuple[str, ...]) -> None:
         raise ValueError(f"{name} overlaps {of}")
 
 
-def _check_turned(query, key, value, slot_mapping, positions, table, out, out_key, dev,
-                  key_in_place: bool):
-    """The arguments that both caches' calls share; (slots, positions, out)."""
+def _turn_args(query, key, value, slot_mapping, positions, table, interleaved, out, out_key, dev,
+               key_in_place: bool):
+    """The checks that both caches' calls share: the leading arguments of the C
+    entries (kept to one look-up each: a decode step's call is bound by its host
+    time), the turned queries' tensor and what must outlive the call."""
     qs, ks, dtype = query.shape, key.shape, query.dtype
     if len(qs) != 3 or len(ks) != 3 or value.shape != ks or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("query must be [T, Hq, D], key and value [T, Hkv, D] with its tokens "
                          "and head_dim")
     if dtype not in _DTYPES or key.dtype != dtype or value.dtype != dtype:
         raise ValueError("query, key and value must share a bf16/fp16 dtype")
-    T, _, D = qs
-    index = dev.index
-    for x, n in ((query, "query"), (key, "key"), (value, "value")):
-        strides = x.stride()
-        if x.get_device() != index or strides[2] != 1 or strides[1] != D:
-            _check_on(x, n, dev)
-            _check_rows(x, n)
+    T, Hq, D = qs
+    Hkv = ks[1]
+    qt, kt, vt = query.stride(), key.stride(), value.stride()
+    _dense_rows(query, "query", dev, qt, D)
+    _dense_rows(key, "key", dev, kt, D)
+    _dense_rows(value, "value", dev, vt, D)
     for x, n in ((slot_mapping, "slot_mapping"), (positions, "positions")):
-        if x.get_device() != index:
+        if x.get_device() != dev.index:
             _check_on(x, n, dev)
         if x.dtype != torch.int64 or x.dim() != 1 or x.numel() < T:
             raise ValueError(f"{n} must be an int64 GPU tensor with an entry for each of the {T} "
                              "tokens")
-    if table.get_device() != index:
+    if table.get_device() != dev.index:
         _check_on(table, "table", dev)
     ts = table.shape
     if table.dtype != torch.float32 or len(ts) != 2 or not table.is_contiguous() or ts[0] == 0 \
             or not 0 < ts[1] <= D:
         raise ValueError("table must be a contiguous float32 tensor [positions, rotary_dim] with "
                          f"rows of up to head_dim {D} entries")
-    if T > 0 and (out is not None or out_key is not None):
-        read = {"query": _span(query), "key": _span(key), "value": _span(value)}
-        if out is not None:
-            written = _span(_check_like(out, query, "out"))
+    qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    q_row, k_row = 2 * Hq * D, 2 * Hkv * D
+    given, read = out is not None, ()
+    if (given or out_key is not None) and T > 0:
+        read = [("query", (qp, 2 * qt[0], q_row, qp + 2 * (T - 1) * qt[0] + q_row)),
+                ("key", (kp, 2 * kt[0], k_row, kp + 2 * (T - 1) * kt[0] + k_row)),
+                ("value", (vp, 2 * vt[0], k_row, vp + 2 * (T - 1) * vt[0] + k_row))]
+    if given:
+        ot = out.stride()
+        if out.shape != qs or out.dtype != dtype:
+            raise ValueError(f"out must have query's shape and dtype {tuple(qs)}, {dtype}")
+        _dense_rows(out, "out", dev, ot, D)
+        op, ot = out.data_ptr(), ot[0]
+        if T > 0:
+            if T > 1 and 2 * ot < q_row:
+                raise ValueError("out's rows overlap each other")
+            written = (op, 2 * ot, q_row, op + 2 * (T - 1) * ot + q_row)
             _check_apart("out", written, read, ("query",))
-            read["out"] = written
-        if out_key is not None:
-            _check_apart("out_key", _span(_check_like(out_key, key, "out_key")), read,
+            read.append(("out", written))
+    else:
+        out = query.new_empty(qs)
+        op, ot = out.data_ptr(), Hq * D
+    okp, okt = None, 0
+    if out_key is not None:
+        okt = out_key.stride()
+        if out_key.shape != ks or out_key.dtype != dtype:
+            raise ValueError(f"out_key must have key's shape and dtype {tuple(ks)}, {dtype}")
+        _dense_rows(out_key, "out_key", dev, okt, D)
+        okp, okt = out_key.data_ptr(), okt[0]
+        if T > 1 and 2 * okt < k_row:
+            raise ValueError("out_key's rows overlap each other")
+        if T > 0:
+            _check_apart("out_key", (okp, 2 * okt, k_row, okp + 2 * (T - 1) * okt + k_row), read,
                          ("key",) if key_in_place else ())
-    return slot_mapping.contiguous(), positions.contiguous(), \
-        query.new_empty(qs) if out is None else out
+    slots, positions = slot_mapping.contiguous(), positions.contiguous()
+    return (qp, qt[0], op, ot, Hq, kp, kt[0], vp, vt[0], okp, okt, Hkv, D, slots.data_ptr(),
+            positions.data_ptr(), T, table.data_ptr(), ts[0], ts[1], 1 if interleaved else 0), \
+        out, (slots, positions)
 
 
 def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -121,31 +140,26 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     table gives NaN.  Token strides are free, the heads of a token dense.
     ``out`` (default: a new tensor) may be ``query`` itself, ``out_key``, which
     gets the turned keys (default: not kept), ``key``; all tokens of both are
-    written, also those whose slot is skipped (negative or past the cache)."""
+    written, also those whose slot is skipped (negative or past the cache).  Of two
+    tokens for one slot either may be left there, in parts."""
     _check_cache_view(key_cache, "key_cache")
     _check_cache_view(value_cache, "value_cache")
     dev = key_cache.device
     _check_on(value_cache, "value_cache", dev)
-    slots, positions, out = _check_turned(query, key, value, slot_mapping, positions, table, out,
-                                          out_key, dev, True)
-    if key_cache.stride(0) != value_cache.stride(0) or key_cache.shape != value_cache.shape:
+    args, out, keep = _turn_args(query, key, value, slot_mapping, positions, table, interleaved,
+                                 out, out_key, dev, True)
+    shape, dtype, block_stride = key_cache.shape, query.dtype, key_cache.stride(0)
+    if block_stride != value_cache.stride(0) or shape != value_cache.shape:
         raise ValueError("key_cache and value_cache must share shape and block stride")
-    if key_cache.dtype != key.dtype or value_cache.dtype != key.dtype:
+    if key_cache.dtype != dtype or value_cache.dtype != dtype:
         raise ValueError("the rows and the caches must share one 16-bit dtype")
-    if key.shape[1:] != key_cache.shape[2:]:
+    N, bs, Hkv, D = shape
+    if args[11] != Hkv or args[12] != D:
         raise ValueError("key/value must be [T, Hkv, D] matching the cache view")
-    T, Hq, D = query.shape
-    if T == 0:
+    if args[15] == 0:
         return out
-    N, bs, Hkv, _ = key_cache.shape
     with device_guard(dev):
-        rc = _lib.load().aegkv_rotary_append(
-            query.data_ptr(), query.stride(0), out.data_ptr(), out.stride(0), Hq, key.data_ptr(),
-            key.stride(0), value.data_ptr(), value.stride(0),
-            None if out_key is None else out_key.data_ptr(),
-            0 if out_key is None else out_key.stride(0), Hkv, D, slots.data_ptr(),
-            positions.data_ptr(), T, table.data_ptr(), table.size(0), table.size(1),
-            int(bool(interleaved)), key_cache.data_ptr(), value_cache.data_ptr(),
-            key_cache.stride(0), N, bs, _DTYPES[query.dtype], raw_stream(dev))
+        rc = _lib.load().aegkv_rotary_append(*args, key_cache.data_ptr(), value_cache.data_ptr(),
+                                             block_stride, N, bs, _DTYPES[dtype], raw_stream(dev))
     _lib.check(rc, "rotary_and_cache")
     return out

@@ -583,6 +583,8 @@ def test_rotary_refusals(device):
     both("overlaps", q=wide[:3], out=wide[1:])
     both("overlaps", out_key=q[:, 2:4])
     both("overlaps", out_key=v)
+    both("overlap each other", out=q[:1].clone().expand(3, -1, -1))
+    both("overlap each other", out_key=k[:1].clone().expand(3, -1, -1))
     with pytest.raises(ValueError, match="overlaps"):
         kv8.rotary_and_cache_kv8(q, k, v, cache[:, 0], ids, ids, table, out_key=k)
     with pytest.raises(ValueError, match="heads"):
