@@ -58,6 +58,7 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <type_traits>
 #include <utility>
 
 #include "aegkv_internal.h"
@@ -1448,11 +1449,11 @@ __device__ __forceinline__ void attend_items(const AttnArgs& a, const int32_t* s
 }
 
 // attend_items over the 4- or 8-bit cache (F: Steps4, Steps8): the same items, ids,
-// pieces and records, in steps of up to F::step() blocks that end where a piece does.  During a step's
-// compute the next NSET - 1 are in flight, across sequences, and its registers are
-// loaded again behind it: the load side keeps a sequence position of its own, and hands a step's to the
-// compute side with its registers.  Past the range a step loads nothing (empty
-// buffer ranges) and is not computed.
+// pieces and records, in steps of up to F::step() blocks that end where a piece
+// does.  During a step's compute the next NSET - 1 are in flight, across sequences,
+// and its registers are loaded again behind it: the load side keeps a sequence
+// position of its own, and hands a step's to the compute side with its registers.
+// Past the range a step loads nothing (empty buffer ranges) and is not computed.
 template <class F, int DT, int D, int NSET, int PACK, bool PLANNED>
 __device__ __forceinline__ void attend_steps(const AttnArgs& a, const int32_t* s_bcum,
                                              const int32_t* s_len, uint8_t* stage, int4* meta,
@@ -1512,7 +1513,8 @@ __device__ __forceinline__ void attend_steps(const AttnArgs& a, const int32_t* s
     ids = load_ids();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
-      s.q[ks] = *reinterpret_cast<const u32x4*>(qp + (F::template dim<D>(ks, 0) - F::template dim<D>(0, 0)));
+      s.q[ks] = *reinterpret_cast<const u32x4*>(
+          qp + (F::template dim<D>(ks, 0) - F::template dim<D>(0, 0)));
 #pragma unroll
     for (int u = 0; u < kStep; ++u) {
       const bool ok = u < s.n && id[u] >= 0 && id[u] < a.n_blocks;
@@ -1710,10 +1712,20 @@ __device__ __forceinline__ int items_before(const int32_t* cum, const int32_t* b
   return bcum[b] + min(max(p - cum[b] - kSegmentCost, 0), bcum[b + 1] - bcum[b]);
 }
 
+// Waves per SIMD whose registers a kernel keeps within.  The 8-bit cache's two steps at
+// D = 128 are 136 registers a lane: with the scan of an unplanned call beside them they
+// pass the 256 of two waves (8 to 10 spilled: 128 sequences of 1500 tokens, 4 kv heads,
+// 51.5 us a call for 49.2, 32 of 1999, 40 heads, 114.9 for 107.5), and one workgroup per
+// CU is what is launched anyhow.
+template <int D, bool PLANNED, int PACK, class F>
+constexpr int waves_per_simd() {
+  return D >= 256 || (D == 128 && PACK > 0 && !PLANNED && std::is_same_v<F, Steps8>) ? 1 : 2;
+}
+
 // PACK: 0, the 16-bit caches; else the cache that F reads, 4-bit (1, 2 or 4: pack_for)
 // or 8-bit (1 or 2: pack8_for).
 template <int DT, int D, int NBUF, bool PLANNED, bool FUSED, int PACK, class F>
-__global__ __launch_bounds__(64 * kWaves, D >= 256 ? 1 : 2) void
+__global__ __launch_bounds__(64 * kWaves, (waves_per_simd<D, PLANNED, PACK, F>())) void
 paged_decode_attention_kernel(AttnArgs a) {
   // cum[batch + 1] (positions), len[batch], bcum[batch + 1] (blocks)
   extern __shared__ int32_t s_mem[];
