@@ -843,6 +843,13 @@ struct Steps4 {
 //     P's low part (P in two 16-bit parts, as above).  PACK = 2 (8 query heads per kv
 //     head or fewer): the columns 8 + head take the low part, and the other half the
 //     next block, half as many products.
+// Bound by the reads: a planned call's kernel takes 103 us over 32 x 1999 tokens of 40
+// heads of 128 (656 MB, 6.3 TB/s) and 39.8 over 128 sequences of 1500 on average, 4 kv
+// heads (196 MB, 4.9 TB/s: about 7 TB/s in between, the rest the cold first step, done
+// 7 us after the start, and XCDs that end 4 to 8 us apart, other ones from call to
+// call).  Measured and no better: three sets of registers (+9%), two blocks a step in
+// four sets (0), 32 or 64 ids held ahead (0), other cache policies (0 to +10%), 384 to
+// 768 workgroups (slower).
 
 // Codes and scale bytes of one block for one lane.
 template <int D>

@@ -1,5 +1,5 @@
-// How the attention of several query tokens over the 4-bit cache cuts its work into
-// workgroups: arithmetic alone, without device code.
+// How the attention of several query tokens over the 4- and the 8-bit
+// cache cuts its work into workgroups: arithmetic alone, without device code.
 #pragma once
 
 #include <algorithm>

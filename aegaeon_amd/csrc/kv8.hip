@@ -8,6 +8,13 @@
 // tokens 4 g .. 4 g + 3 (lane = 16 g + c; D = 64: c < 8; D = 256: and dims 128
 // further): a block's maximum is a reduction within the wave, and V's words, four
 // tokens of a dim, come together in one lane's registers.
+//   Both are bound by memory once they are large.  4 kv heads of 128, bf16:
+//   append    28 layers of a decode step of 128 tokens 12.5 us, of 256 20.0: latency of
+//             the chain slot, scale byte, new scale, and of the lines that V's bytes
+//             touch.  8 layers of 4 x 1024 tokens 21.7 us (100 MB, 4.6 TB/s).
+//   rotating  one layer beside 28 query heads: 128 tokens 5.5 us, 4000 of four prompts
+//             19.2 (71 MB, 3.7 TB/s: the keys' waves load partners and angles too).
+//   gather    128 sequences of 400 tokens on average 25.4 us (155 MB, 6.1 TB/s).
 #include <algorithm>
 
 #include "aegkv_internal.h"

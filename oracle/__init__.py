@@ -26,4 +26,7 @@ Pinning (what fixes each function independently of this file's formulas):
   kv4_oracle (the 4-bit cache)             - hand-computed codes, scale bytes and
       byte positions, every byte of a record written once
       (tests/test_kv4.py).
+  kv8_oracle (the 8-bit cache, rotation)   - torch's 8-bit float type, hand-computed
+      exponents and byte positions, every byte of a side written once, rotation as
+      a product of complex numbers (tests/test_kv8.py).
 """
