@@ -290,6 +290,52 @@ def test_a_decode_loop_of_turned_appends_and_attention(device):
             _check(out, want_q, cache[:, layer], tables, lens, 0.09, Hkv, D, "bf16")
 
 
+@pytest.mark.parametrize("planned", [False, True])
+def test_a_captured_step_equals_the_eager_one(device, planned):
+    """A step's append with rotation and its attention in one graph, replayed over
+    steps that cross block edges, a padded row among them: cache and outputs are
+    those of the eager calls, bit for bit."""
+    rng = np.random.default_rng(15)
+    Hq, Hkv, D, bound = 28, 4, 128, 64
+    lens = np.array([13, 30, 1, 0])
+    tables = _tables(rng, lens + 20, 12)
+    bt = torch.from_numpy(ko.pad_block_tables(tables)).to(device)
+    start = torch.from_numpy(_filled(rng, 12, 1, Hkv, D, "bf16")[:, 0]).to(device)
+    table = rotary.rotary_table(100, D, device=device)
+    T = len(lens)
+    q, k, v = (torch.zeros(T, h, D, dtype=torch.bfloat16, device=device) for h in (Hq, Hkv, Hkv))
+    slots, pos = (torch.zeros(T, dtype=torch.int64, device=device) for _ in range(2))
+    sl = torch.ones(T, dtype=torch.int32, device=device)
+
+    def step(cache):
+        turned = kv8.rotary_and_cache_kv8(q, k, v, cache, slots, pos, table)
+        plan = A.DecodePlan(bt, sl, bound, Hkv) if planned else None
+        return kv8.paged_decode_attention_kv8(turned, cache, bt, sl, 0.09, bound, plan=plan)
+
+    eager, captured = start.clone(), start.clone()
+    step(captured)  # what a first call sets up
+    captured.copy_(start)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(captured)
+    for _ in range(6):
+        active = lens > 0
+        lens = lens + active
+        for dst, h in ((q, Hq), (k, Hkv), (v, Hkv)):
+            dst.copy_(to_device_bits(_rows(rng, (T, h, D), "bf16"), "bf16", device))
+        slots.copy_(torch.tensor([t[(n - 1) // 16] * 16 + (n - 1) % 16 if n else -1
+                                  for t, n in zip(tables, lens.tolist())]))
+        pos.copy_(torch.from_numpy(np.maximum(lens - 1, 0)))
+        sl.copy_(torch.from_numpy(lens.astype(np.int32)))
+        want = step(eager)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, eager)
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+        assert not out[3].any()
+
+
 def test_refusals(device):
     cache = kv8.kv8_cache(4, 2, 4, 128, device)
     bt = torch.zeros(1, 2, dtype=torch.int32, device=device)
