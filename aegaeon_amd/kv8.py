@@ -83,8 +83,7 @@ def reshape_and_cache_kv8(key: torch.Tensor, value: torch.Tensor, kv_cache: torc
     where their size raises the block's exponent.  The rows of one block must
     follow each other in the call; of several for one slot the last counts."""
     _check_new_rows(key, value, 3, "[T, Hkv, D]")
-    _append(key.unsqueeze(0), value.unsqueeze(0), kv_cache.unsqueeze(1), slot_mapping,
-            "reshape_and_cache_kv8")
+    _append(key, value, kv_cache, slot_mapping, False, "reshape_and_cache_kv8")
 
 
 def append_kv8(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
@@ -93,12 +92,13 @@ def append_kv8(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
     ``key``/``value [L, T, Hkv, D]`` (token and layer strides free) into
     ``kv_cache [N, L, R]``."""
     _check_new_rows(key, value, 4, "[L, T, Hkv, D]")
-    _append(key, value, kv_cache, slot_mapping, "append_kv8")
+    _append(key, value, kv_cache, slot_mapping, True, "append_kv8")
 
 
-def _append(key, value, kv_cache, slot_mapping, op: str) -> None:
-    L, T, H, D = key.shape
-    if _kv_heads(kv_cache, True, D) != H or kv_cache.size(1) != L:
+def _append(key, value, kv_cache, slot_mapping, layers: bool, op: str) -> None:
+    T, H, D = key.shape[-3:]
+    L = key.size(0) if layers else 1
+    if _kv_heads(kv_cache, layers, D) != H or (layers and kv_cache.size(1) != L):
         raise ValueError("key/value and kv_cache disagree on the layers or kv heads")
     dev = kv_cache.device
     _check_on(key, "key", dev)
@@ -107,11 +107,12 @@ def _append(key, value, kv_cache, slot_mapping, op: str) -> None:
     if L == 0 or T == 0:
         return
     ks, vs, cs = key.stride(), value.stride(), kv_cache.stride()
+    k_layer, v_layer, c_layer = (ks[0], vs[0], cs[1]) if L > 1 else (0, 0, 0)
     with device_guard(dev):
         rc = _lib.load().aegkv_kv8_append(
-            key.data_ptr(), value.data_ptr(), ks[1], vs[1], ks[0] if L > 1 else 0,
-            vs[0] if L > 1 else 0, slots.data_ptr(), T, kv_cache.data_ptr(), cs[0],
-            cs[1] if L > 1 else 0, kv_cache.size(0), L, H, D, _DTYPES[key.dtype], raw_stream(dev))
+            key.data_ptr(), value.data_ptr(), ks[-3], vs[-3], k_layer, v_layer, slots.data_ptr(), T,
+            kv_cache.data_ptr(), cs[0], c_layer, kv_cache.size(0), L, H, D, _DTYPES[key.dtype],
+            raw_stream(dev))
     _lib.check(rc, op)
 
 
