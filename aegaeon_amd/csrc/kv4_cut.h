@@ -32,10 +32,43 @@ constexpr int ranges_of(int n_kt, int span) {
   return r > 1 ? (int)r : 1;
 }
 
+// The other cut, of eight-wave tiles (one workgroup per CU) that are fewer than the
+// CUs but more than half of them: a tile's first piece has `span` key steps, and what
+// is left of the tiles goes to the CUs that have none or are done.  Workgroups are dealt
+// to groups of 8 CUs in turn and stay there: of T tiles on P places a group has up to
+// m = ceil(8 T / P) first pieces, and its 8 - m other CUs take m remainders in
+// ceil(m / (8 - m)) rounds, so a span is rounds / (rounds + 1) of a tile (m = 8: a whole
+// one of average length, so that only longer ones are cut), and the average work of a
+// place at least; a piece costs kPieceStart steps beside its own (its start, its
+// partials).  Sequences of more steps get more pieces of `span`.  `cost`: key steps of
+// all tiles.  Us a pass of the 8-bit cache, uncut and so (28/4 heads of 128, bf16): 1250
+// queries over 16000 tokens (140 tiles) 463 and 341, 1500 (168) 464 and 376, 2048 (224)
+// 477 and 458 (a step takes 2.1 us with every CU at work, 1.85 with 224), 3 x 700 over
+// 6000 on average, ragged (240) 226 and 190, 8/8 heads, 14 x 512 over 8000 (224) 254 and
+// 257.
+constexpr int kPieceStart = 8;
+constexpr int uneven_span(int64_t cost, int64_t tiles, int64_t places, int least) {
+  if (tiles <= 0 || places <= 0) return INT32_MAX;
+  if (2 * tiles <= places) return span_of(2 * cost, places, least);
+  const int64_t whole = cost + kPieceStart * tiles, each = whole / tiles + 1;
+  const int64_t m = (8 * tiles + places - 1) / places, rounds = m < 8 ? 7 / (8 - m) : 0;
+  const int64_t even = (whole + places - 1) / places;
+  const int64_t part = m < 8 ? each * rounds / (rounds + 1) : each;
+  const int64_t span = even > part ? even : part;
+  return span > INT32_MAX ? INT32_MAX : (int)span;
+}
+// The pieces of n_kt key steps then; all have `span` steps but the last one, which has
+// more than kLeastRest, and up to as many more than `span`.
+constexpr int kLeastRest = 8;
+constexpr int uneven_ranges(int n_kt, int span) {
+  return n_kt - kLeastRest > span ? (n_kt - kLeastRest - 1) / span + 1 : 1;
+}
+
 // The launch of a call: which kernel, how many pieces at most, and whether
 // sequences are cut.
 struct VarlenShape {
   bool long_rows;
+  bool uneven;      // cut by uneven_span
   int key_tiles;    // of a step
   int64_t pieces;   // bound of the pieces (the main grid)
   int64_t target;   // pieces wanted (0: uncut)
@@ -61,10 +94,10 @@ constexpr int kLongRows = 256, kLongSteps = 32;
 constexpr int kLeastLong = 16, kLeastShort = 4;
 
 // False: more pieces than a grid.  (Heads of up to 65535 and rows of a sequence of up
-// to 2^30: no product passes 64 bits.)
+// to 2^30: no product passes 64 bits.)  uneven: the cache's kernels take that cut.
 inline bool varlen_shape(int64_t cus, int32_t batch, int64_t total_q, int32_t max_q,
                          int32_t max_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
-                         VarlenShape* out) {
+                         VarlenShape* out, bool uneven = false) {
   const int64_t group = n_q_heads / n_kv_heads, max_rows = (int64_t)max_q * group;
   total_q = std::min<int64_t>(total_q, INT32_MAX);  // (cu_seqlens end there)
   VarlenShape s{};
@@ -103,6 +136,13 @@ inline bool varlen_shape(int64_t cus, int32_t batch, int64_t total_q, int32_t ma
     if (s.long_rows && jobs <= slots / 2) s.target = std::min(s.target, slots / jobs * jobs);
     // a sequence of cost x has at most x / span + its tiles
     s.pieces = std::min(s.target + jobs, jobs * ((max_kt + s.least - 1) / s.least));
+    s.uneven = uneven && s.long_rows && jobs > slots / 2;
+    if (s.uneven) {
+      // (its cost is of the tiles' own steps, half of the sequences' at least; the span
+      // is a place's share of it at least)
+      s.target = slots;
+      s.pieces = jobs + 2 * slots;
+    }
     s.cut = jobs;
     auto per_tile = [&](int64_t r) { return (std::min(max_rows, tile_rows) + r - 1) / r; };
     // Rows of a merge workgroup.  4 where a tile has 16 pieces or more (28/4 heads over

@@ -34,6 +34,7 @@ __device__ __forceinline__ int v_chunk(int row, int c) {
 }
 
 struct Codes4 {
+  static constexpr bool kUneven = false;
   template <int D>
   using Regs = CodeRegs<D>;
   template <int D>
@@ -168,7 +169,7 @@ int64_t aegkv_kv4_varlen_attention_workspace_size(int32_t batch, int64_t total_q
                                                   int32_t max_seqlen_q, int32_t max_seq_len,
                                                   int32_t n_q_heads, int32_t n_kv_heads,
                                                   int32_t head_dim, int32_t dtype) {
-  return varlen_workspace(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads,
+  return varlen_workspace<Codes4>(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads,
                           head_dim, dtype);
 }
 

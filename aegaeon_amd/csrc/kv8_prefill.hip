@@ -5,9 +5,9 @@
 // 8 bytes of a dim's four tokens, and the operand V^T[32 dims x 16 keys] is one
 // ordinary 16-byte read per lane, without a transposing read.
 //   Bound by the products where rows are many (2048 queries over 16001 tokens, 28/4
-// heads, bf16: 473 us a pass, 930 TFLOP/s, 224 of the 256 CUs at work) and by the latency
-// of a piece's start and steps where they are few (48 x 5 over 1000 tokens, 32/4 heads:
-// 22.4 us and the merge's 4.4; 52 MB).  Measured and no better: V^T's rows permuted by
+// heads, bf16: 464 us a pass, 950 TFLOP/s) and by the latency of a piece's start and
+// steps where they are few (48 x 5 over 1000 tokens, 32/4 heads: 22.4 us and the merge's
+// 4.4; 52 MB).  Measured and no better: V^T's rows permuted by
 // one more bit (0 to +1.5%), reads four ahead (0), left to the compiler's order (+2%),
 // four key tiles a step for up to 32 rows (28.5 -> 39.0 us).
 #include "kv8_format.h"
@@ -31,6 +31,7 @@ struct CodeRegs8 {
 __device__ __forceinline__ int vt_chunk(int dim, int c) { return c ^ ((dim ^ dim >> 3) & 7); }
 
 struct Codes8 {
+  static constexpr bool kUneven = true;
   template <int D>
   using Regs = CodeRegs8<D>;
   template <int D>
@@ -160,7 +161,7 @@ int64_t aegkv_kv8_varlen_attention_workspace_size(int32_t batch, int64_t total_q
                                                   int32_t n_q_heads, int32_t n_kv_heads,
                                                   int32_t head_dim, int32_t dtype) {
   if (n_kv_heads > kKv8MaxHeads) return AEGKV_ERR_UNSUPPORTED;
-  return varlen_workspace(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads,
+  return varlen_workspace<Codes8>(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads,
                           head_dim, dtype);
 }
 

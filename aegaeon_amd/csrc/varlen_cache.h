@@ -30,7 +30,9 @@
 // for a sequence's tiles: `splits` ranges of ceil(n_kt / splits) key steps,
 // splits = ceil(n_kt / C), with one C for the batch that every workgroup
 // computes for itself: the batch's key steps times row tiles divided by the
-// pieces wanted.
+// pieces wanted.  Eight-wave tiles that fill more than half of the CUs are cut
+// unevenly (uneven_span), where the cache's operators ask for it (F::kUneven; the 4-bit
+// cache's came before that cut, and their results keep their bits).
 #pragma once
 
 #include <algorithm>
@@ -67,6 +69,7 @@ struct VarlenArgs {
   float scale_log2;          // |softmax scale| * log2(e), > 0 (1 for 0)
   int32_t scale_sign;        // of the scale: 1, -1 or 0
   int64_t target;            // pieces wanted (0: no sequence is cut)
+  bool uneven;               // the cut is uneven_span's, over `target` places
   int32_t least;             // least key tiles of a piece
   int32_t n_pieces;          // bound of the pieces: the main grid, and the partials' slots
   float* part_o;             // [n_pieces][32 W][D]
@@ -106,12 +109,13 @@ __device__ __forceinline__ SeqWork seq_work(const VarlenArgs& a, int b) {
 struct Piece {
   SeqWork s;
   int b, head, tile, split, splits, span, cut;
+  int slot;         // of its partials
 };
 
 struct LocateLds {
   int64_t cost[16];
-  int sum[16], cut[16];
-  int found[11];
+  int sum[16], cut[16], more[16];
+  int found[13];
 };
 // The piece numbered blockIdx.x, found by all NT threads, each summing its own
 // sequences.  False: there are fewer.  The first workgroup writes n_cut.
@@ -200,8 +204,114 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, LocateLds& x, Piece&
   const int q = f[1] / p.splits;
   p.split = f[1] - q * p.splits;
   p.cut = f[4] + q;
+  p.slot = index;
   p.tile = q / a.n_kv_heads;
   p.head = q - p.tile * a.n_kv_heads;
+  p.tile = p.s.tiles - 1 - p.tile;
+  return true;
+}
+// As locate, of an uneven cut (its number of pieces r is the sequence's; a tile may have
+// fewer, uneven_tile).  The first pieces of all tiles come first, in the order above,
+// then the others.
+template <int W, int NT>
+__device__ __forceinline__ bool locate_uneven(const VarlenArgs& a, LocateLds& x, Piece& p) {
+  constexpr int NW = NT / 64;
+  const int index = (int)blockIdx.x;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int per = (a.batch + NT - 1) / NT, b0 = min(t * per, a.batch), b1 = min(b0 + per, a.batch);
+  const SeqWork mine = seq_work<W, 1>(a, min(b0, a.batch - 1));
+  auto work = [&](int b) { return b == b0 ? mine : seq_work<W, 1>(a, b); };
+  int64_t cost = 0;
+  int tiles = 0;
+  for (int b = b0; b < b1; ++b) {
+    const SeqWork s = work(b);
+    // the mean of the first tile's steps and the last one's
+    const int q0 = a.by_group.div(max(min(s.rows, kUnitRows * W) - 1, 0));
+    const int k0 = a.causal ? min(s.off + q0 + 1, s.len) : s.len;
+    const int n0 = (max(k0, 0) + kPfKTile - 1) / kPfKTile;
+    cost += (int64_t)s.tiles * a.n_kv_heads * ((n0 + s.n_kt + 1) / 2);
+    tiles += s.tiles * a.n_kv_heads;
+  }
+  constexpr int kDigit = (1 << 25) - 1;
+  const int d0 = wave_prefix((int)cost & kDigit), d1 = wave_prefix((int)(cost >> 25) & kDigit),
+            d2 = wave_prefix((int)(cost >> 50)), mincl = wave_prefix(tiles);
+  if (lane == 63) {
+    x.cost[wave] = ((int64_t)d2 << 50) + ((int64_t)d1 << 25) + d0;
+    x.sum[wave] = mincl;
+  }
+  if (t == 0) x.found[0] = -1;
+  __syncthreads();
+  cost = 0;
+  int total = 0, mexcl = mincl - tiles;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    cost += x.cost[w];
+    total += x.sum[w];
+    mexcl += w < wave ? x.sum[w] : 0;
+  }
+  const int span = uneven_span(cost, total, a.target, a.least);
+  int cuts = 0, more = 0;  // this thread's cut row tiles and their further pieces
+  for (int b = b0; b < b1; ++b) {
+    const SeqWork s = work(b);
+    const int r = uneven_ranges(s.n_kt, span), n = s.tiles * a.n_kv_heads;
+    cuts += r > 1 ? n : 0;
+    more += n * (r - 1);
+  }
+  const int cincl = wave_prefix(cuts), eincl = wave_prefix(more);
+  if (lane == 63) {
+    x.cut[wave] = cincl;
+    x.more[wave] = eincl;
+  }
+  __syncthreads();
+  int cexcl = cincl - cuts, eexcl = eincl - more;
+  for (int w = 0; w < wave; ++w) {
+    cexcl += x.cut[w];
+    eexcl += x.more[w];
+  }
+  if (index == 0 && t == NT - 1)
+    *a.n_cut = total + eexcl + more <= a.n_pieces ? min(cexcl + cuts, a.max_cut) : 0;
+  const bool first = index < total;  // uniform
+  const int at = first ? index : index - total, own = first ? mexcl : eexcl;
+  if (at >= own && at < own + (first ? tiles : more)) {  // one thread
+    int left = at - own;
+    for (int b = b0; b < b1; ++b) {
+      const SeqWork s = work(b);
+      const int r = uneven_ranges(s.n_kt, span), n = s.tiles * a.n_kv_heads;
+      const int here = first ? n : n * (r - 1);
+      if (left < here) {
+        const int q = first ? left : left / (r - 1);
+        const int split = first ? 0 : 1 + left - q * (r - 1);
+        const int f[13] = {b,    q,     split, cexcl + q, cexcl + eexcl + q * r + split, s.t0,
+                           s.m, s.off, s.len, s.rows,    s.tiles,                       span,
+                           r};
+#pragma unroll
+        for (int i = 0; i < 13; ++i) x.found[i] = f[i];
+        break;
+      }
+      left -= here;
+      cexcl += r > 1 ? n : 0;
+      eexcl += n * (r - 1);
+    }
+  }
+  __syncthreads();
+  int f[13];
+#pragma unroll
+  for (int i = 0; i < 13; ++i) f[i] = __builtin_amdgcn_readfirstlane(x.found[i]);
+  p.b = f[0];
+  if (p.b < 0) return false;
+  p.split = f[2];
+  p.cut = f[3];
+  p.slot = f[4];
+  p.s.t0 = f[5];
+  p.s.m = f[6];
+  p.s.off = f[7];
+  p.s.len = f[8];
+  p.s.rows = f[9];
+  p.s.tiles = f[10];
+  p.span = f[11];
+  p.splits = f[12];
+  p.tile = f[1] / a.n_kv_heads;
+  p.head = f[1] - p.tile * a.n_kv_heads;
   p.tile = p.s.tiles - 1 - p.tile;
   return true;
 }
@@ -212,6 +322,14 @@ __device__ __forceinline__ void put_cut(const VarlenArgs& a, const Piece& p) {
   const int row0 = p.tile * W * kUnitRows;
   a.cut[p.cut] = {p.s.t0, p.head, row0, min(row0 + W * kUnitRows, p.s.rows), (int)blockIdx.x,
                   p.splits};
+}
+// That of an uneven cut, for a tile of `pieces` pieces itself (one: no rows to merge).
+template <int W>
+__device__ __forceinline__ void put_cut_uneven(const VarlenArgs& a, const Piece& p, int pieces) {
+  if (p.splits == 1 || p.split || threadIdx.x || p.cut >= a.max_cut) return;
+  const int row0 = p.tile * W * kUnitRows;
+  a.cut[p.cut] = {p.s.t0, p.head, row0, pieces > 1 ? min(row0 + W * kUnitRows, p.s.rows) : row0,
+                  p.slot, pieces};
 }
 
 // Nothing is scheduled across: the softmax would otherwise sink into the next
@@ -593,7 +711,10 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
   __shared__ int32_t s_first[D];
   __shared__ LocateLds s_loc;
   Piece p;
-  if (!locate<W, 1, 64 * W>(a, s_loc, p)) return;  // uniform
+  bool uneven = false;
+  if constexpr (F::kUneven) uneven = a.uneven;
+  if (uneven ? !locate_uneven<W, 64 * W>(a, s_loc, p) : !locate<W, 1, 64 * W>(a, s_loc, p))
+    return;  // uniform
   const SeqWork& s = p.s;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = w >> 2, u = w & 3;  // and the block of each tile that the wave converts
@@ -601,7 +722,15 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
   const int last_q = a.by_group.div(min(s.rows, (p.tile + 1) * W * kUnitRows) - 1);
   const int keys = a.causal ? min(s.off + last_q + 1, s.len) : s.len;
   const int kt0 = p.split * p.span;
-  const int n_kt = max(min(p.span, (max(keys, 0) + kPfKTile - 1) / kPfKTile - kt0), 0);
+  int n_kt = max(min(p.span, (max(keys, 0) + kPfKTile - 1) / kPfKTile - kt0), 0);
+  if (uneven) {  // the tile's own pieces: the last one has what is left of it
+    const int all = (max(keys, 0) + kPfKTile - 1) / kPfKTile;
+    const int pieces = uneven_ranges(all, p.span);
+    put_cut_uneven<W>(a, p, pieces);
+    if (p.split >= pieces) return;  // uniform
+    if (p.split == pieces - 1) n_kt = all - kt0;
+    p.splits = pieces;
+  }
 
   RowUnit<DT, D> unit;
   unit.init(a, s, p.head, p.tile * W + w);
@@ -690,9 +819,9 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
     find_nan<F, D>(a, table, head, s.len, kt0, kt0 + n_kt, s_first);
     unit.spoil(s_first);
   }
-  put_cut<W>(a, p);
-  if (p.splits > 1) unit.store_partial(a, ((int64_t)blockIdx.x * W + w) * kUnitRows);
-  else unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
+  if (!uneven) put_cut<W>(a, p);
+  if (p.splits == 1) unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
+  else if (p.slot < a.n_pieces) unit.store_partial(a, ((int64_t)p.slot * W + w) * kUnitRows);
 }
 
 // Merges the pieces of R rows of a cut sequence's kv head:
@@ -778,12 +907,12 @@ int varlen_check(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len,
 }
 
 int shape_of(int32_t batch, int64_t total_q, int32_t max_q, int32_t max_len, int32_t n_q_heads,
-             int32_t n_kv_heads, int32_t head_dim, VarlenShape* s) {
+             int32_t n_kv_heads, int32_t head_dim, bool uneven, VarlenShape* s) {
   DeviceState* ds = nullptr;
   const int rc = current_device_state(&ds);
   if (rc) return rc;
   return varlen_shape(std::max(1, ds->num_cu), batch, total_q, max_q, max_len, n_q_heads,
-                      n_kv_heads, head_dim, s)
+                      n_kv_heads, head_dim, s, uneven)
              ? AEGKV_OK
              : AEGKV_ERR_UNSUPPORTED;
 }
@@ -819,7 +948,8 @@ int launch_varlen(const VarlenArgs& a, const VarlenShape& s, hipStream_t st) {
 }
 
 // Workspace bytes of a call, or a status.
-inline int64_t varlen_workspace(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
+template <class F>
+int64_t varlen_workspace(int32_t batch, int64_t total_q, int32_t max_seqlen_q,
                                 int32_t max_seq_len, int32_t n_q_heads, int32_t n_kv_heads,
                                 int32_t head_dim, int32_t dtype) {
   int rc = varlen_check(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
@@ -827,7 +957,8 @@ inline int64_t varlen_workspace(int32_t batch, int64_t total_q, int32_t max_seql
   if (rc) return rc;
   if (batch == 0 || total_q == 0 || max_seqlen_q == 0) return 0;
   VarlenShape s;
-  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
+                F::kUneven, &s);
   if (rc) return rc > 0 ? AEGKV_ERR_RUNTIME : rc;
   return s.workspace();
 }
@@ -856,7 +987,8 @@ int run_varlen(void* out, int64_t out_token_stride, const void* q, int64_t q_tok
     return AEGKV_ERR_MISALIGNED;
   if (((int64_t)max_seq_len + kCacheTokens - 1) / kCacheTokens > max_blocks) return AEGKV_ERR_INVALID_ARG;
   VarlenShape s;
-  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim, &s);
+  rc = shape_of(batch, total_q, max_seqlen_q, max_seq_len, n_q_heads, n_kv_heads, head_dim,
+                F::kUneven, &s);
   if (rc) return rc;
   if (s.target > 0 && (!workspace || workspace_bytes < (uint64_t)s.workspace()))
     return AEGKV_ERR_WORKSPACE;
@@ -884,6 +1016,7 @@ int run_varlen(void* out, int64_t out_token_stride, const void* q, int64_t q_tok
   a.scale_sign = scale > 0 ? 1 : scale < 0 ? -1 : 0;
   a.scale_log2 = scale == 0 ? 1.f : std::fabs(scale) * 1.4426950408889634f;
   a.target = s.target;
+  a.uneven = s.uneven;
   a.least = s.least;
   a.n_pieces = (int32_t)s.pieces;
   uint8_t* ws = static_cast<uint8_t*>(workspace);

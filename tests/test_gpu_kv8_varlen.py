@@ -123,6 +123,70 @@ def test_few_tiles_of_many_keys(device, new, lens, dtype, causal):
     b.check(b.run(-0.1, causal), -0.1, causal)
 
 
+# More eight-wave tiles than half of the CUs (256 rows a tile, two kv heads): the first
+# pieces of all, then what is left of them.
+@pytest.mark.parametrize("new,lens,causal", [
+    ([900], [3900], True), ([900], [3900], False),          # 142 tiles of 256 places
+    ([1200], [3901], True), ([1400], [4000], True),         # 188, 220
+    ([500, 500, 500], [9000, 1000, 2500], True),            # 240, one sequence long
+    ([1300, 0, 3], [3800, 5000, 20], True)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_tiles_cut_unevenly(device, new, lens, causal, dtype):
+    b = Batch(device, new, lens, 40, 2, 128, dtype, sum(lens) + causal)
+    b.check(b.run(0.1, causal), 0.1, causal)
+
+
+def test_an_uneven_cut_of_bounds_far_past_the_batch(device):
+    """What is cut is found on the device: fewer queries than the bounds and the
+    tokens that the tensor has room for, rows behind the last left alone; the same
+    bits again, and with a workspace of the caller's."""
+    b = Batch(device, [250, 20], [5000, 3000], 40, 2, 128, "bf16", 3, extra=700)
+    outs = []
+    for ws in (None, None, kv8.varlen_attention_workspace(2, 970, 900, 5000, 40, 2, 128,
+                                                          torch.bfloat16, device)):
+        out = torch.full_like(b.dq, 7.0)
+        assert b.run(0.1, max_q=900, out=out, workspace=ws) is out
+        outs.append(out.cpu())
+    assert (outs[0][270:] == 7).all()
+    within(outs[0][:270].double().numpy(), b.want(0.1)[:270], "bf16")
+    for o in outs[1:]:
+        assert torch.equal(o.view(torch.int16), outs[0].view(torch.int16))
+
+
+def test_nan_and_unreadable_blocks_of_an_uneven_cut(device):
+    """In the first piece, in the remainder and at its edges."""
+    b = Batch(device, [1200], [3901], 40, 2, 128, "bf16", 6)
+    dirty = b.cache.copy()
+    lost = b.bt.clone()
+    span = 11 * 64  # some blocks of every part of the keys
+    masked = [0, 50, 100, 150, 200, 230, 243]
+    lost[0, masked] = -1
+    out = b.run(0.1, bt=lost)
+    keys = np.ones(3901, bool)
+    for m in masked:
+        keys[16 * m:16 * m + 16] = False
+    k, v = b.rows()
+    rows = np.concatenate([np.arange(16) + 16 * t for t in b.tables[0]])[:3901]
+    k, v = (x.reshape(-1, 2, 128)[rows] for x in (k, v))
+    q = ko.bits_to_float(b.q, "bf16").astype(np.float64)
+    want = np.empty((1200, 40, 128))
+    for h in range(40):
+        x = 0.1 * q[:, h] @ k[:, h // 20].T.astype(np.float64)
+        x[~(keys & (np.arange(3901) <= 2701 + np.arange(1200)[:, None]))] = -np.inf
+        p = np.exp(x - x.max(1, keepdims=True))
+        want[:, h] = (p / p.sum(1, keepdims=True)) @ v[:, h // 20]
+    within(out.double().cpu().numpy(), want, "bf16")
+    for token, dim in ((5, 3), (span * 4, 70), (3700, 127)):
+        _nan_at(b, dirty, 0, token, 1, dim, 1)
+    got = b.run(0.1, cache=torch.from_numpy(dirty).to(device)).cpu()
+    clean = b.run(0.1).cpu()
+    nan = torch.zeros(1200, 40, 128, dtype=torch.bool)
+    for token, dim in ((5, 3), (span * 4, 70), (3700, 127)):
+        nan[max(token - 2701, 0):, 20:, dim] = True
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[~nan], clean[~nan])
+
+
 def _nan_at(b, dirty, s, token, head, dim, side):
     """One value of a block NaN, as an append leaves it."""
     blk, D = b.tables[s][token // 16], b.D
