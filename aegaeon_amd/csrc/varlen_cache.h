@@ -544,10 +544,13 @@ struct RowUnit : WaveSoftmax<DT, D, true> {
       }
     }
   }
+  // ANEW: r0 + col is computed again, which held since init would be a register too many
+  // (in a kernel that has registers left that costs 0.4%).
+  template <bool ANEW = false>
   __device__ __forceinline__ void store_partial(const VarlenArgs& a, int64_t slot_row) const {
     const int lane = threadIdx.x & 63, hh = lane >> 5;
     int col = lane & 31;
-    asm volatile("" : "+v"(col));  // r0 + col anew: held since init it cost a register too many
+    if constexpr (ANEW) asm volatile("" : "+v"(col));
     const float lt = total();
     if (r0 + col >= rows) return;
     float* po = a.part_o + (slot_row + col) * D + 4 * hh;
@@ -708,7 +711,6 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
   static_assert(W / 2 * kUnitRows * D * 2 <= 2 * T_BYTES, "a half's outputs fit its stages");
   __shared__ __align__(16) uint8_t lds[4 * T_BYTES];  // two K stages, two V stages
   __shared__ uint32_t s_nan[W / 2];
-  __shared__ int32_t s_first[D];
   __shared__ LocateLds s_loc;
   Piece p;
   bool uneven = false;
@@ -816,12 +818,16 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
 #pragma unroll
   for (int i = 0; i < W / 2; ++i) nan |= s_nan[i] != 0;
   if (__builtin_amdgcn_readfirstlane(nan)) {
-    find_nan<F, D>(a, table, head, s.len, kt0, kt0 + n_kt, s_first);
-    unit.spoil(s_first);
+    // (in the stages' memory: an array beside them cost the whole kernel 1%)
+    int32_t* first = reinterpret_cast<int32_t*>(lds);
+    find_nan<F, D>(a, table, head, s.len, kt0, kt0 + n_kt, first);
+    unit.spoil(first);
+    VARLEN_BARRIER();  // before the outputs go there
   }
   if (!uneven) put_cut<W>(a, p);
   if (p.splits == 1) unit.store(a, s, lds + w * (kUnitRows * D * 2), p.head);
-  else if (p.slot < a.n_pieces) unit.store_partial(a, ((int64_t)p.slot * W + w) * kUnitRows);
+  else if (p.slot < a.n_pieces)
+    unit.template store_partial<F::kUneven>(a, ((int64_t)p.slot * W + w) * kUnitRows);
 }
 
 // Merges the pieces of R rows of a cut sequence's kv head:
