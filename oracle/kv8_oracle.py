@@ -9,6 +9,7 @@ textbook in float64 over the decoded rows.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Tuple
 
 import numpy as np
@@ -59,6 +60,7 @@ def byte_of(side: int, dim: int, r: int, d: int) -> int:
     return ((o // 4 * 4 + r // 4) * 16 + lane) * 16 + o % 4 * 4 + r % 4
 
 
+@lru_cache(maxsize=None)
 def _index(side: int, dim: int) -> np.ndarray:
     return np.array([[byte_of(side, dim, r, d) for d in range(dim)] for r in range(BLOCK)])
 
@@ -99,8 +101,7 @@ def _put(layer_block, side, H, D, h, new, dtype):
             e = held
         else:
             codes = encode(decode(codes, held), e)
-    for r, x in new.items():
-        codes[r] = encode(x, e)
+    codes[list(new)] = encode(np.stack(list(new.values())), e)
     layer_block[at] = codes
     layer_block[s + side] = e + 127
     if side == 1:
