@@ -105,7 +105,7 @@ __device__ __forceinline__ Side side_of(const Append8Args& a, uint32_t layer, ui
 // keys: the loads of all four are in flight together.  top: the largest of the
 // finite magnitudes' bits; bad: there are others, which become NaN.
 template <int DT, int TURN>
-__device__ __forceinline__ void load_rows(const Append8Args& a, const Side& s, const int64_t (&tok)[4],
+__device__ __forceinline__ void load_rows(const Append8Args& a, const Side& s, const int (&tok)[4],
                                           int c, float (&f)[4][8], uint32_t (&top)[4],
                                           bool (&bad)[4]) {
   constexpr bool INTER = TURN == kNeighbours;
@@ -115,7 +115,7 @@ __device__ __forceinline__ void load_rows(const Append8Args& a, const Side& s, c
   for (int k = 0; k < 4; ++k) {
     x[k] = y[k] = u32x4{0u, 0u, 0u, 0u};
     if (tok[k] >= 0) {
-      const uint8_t* p = s.rows + tok[k] * s.tok_b;
+      const uint8_t* p = s.rows + (int64_t)tok[k] * s.tok_b;
       x[k] = *reinterpret_cast<const u32x4*>(p + 16 * c);
       if (turns) y[k] = *reinterpret_cast<const u32x4*>(p + 16 * partner_chunk<INTER>(a.r, c));
     }
@@ -154,7 +154,7 @@ __device__ __forceinline__ float down_factor(int from, int to) {
 // One run: tokens of block blk; tok[k]: the one for place 4 g + k.
 template <int DT, int D, int TURN>
 __device__ __forceinline__ void append_run(const Append8Args& a, const Side& s, int64_t blk,
-                                           int64_t (&tok)[4], bool anew) {
+                                           int (&tok)[4], bool anew) {
   constexpr int NC = D > 128 ? D / 128 : 1;  // chunks of a lane
   const int lane = threadIdx.x & 63, g = lane >> 4, c0 = lane & 15;
   const bool idle = D < 128 && c0 >= D / 8;
@@ -249,7 +249,7 @@ __device__ __forceinline__ void append_run(const Append8Args& a, const Side& s, 
 // blk[k].
 template <int DT, int D, int TURN>
 __device__ __forceinline__ void append_singles(const Append8Args& a, const Side& s,
-                                               int64_t (&tok)[4], const int (&blk)[4],
+                                               int (&tok)[4], const int (&blk)[4],
                                                const int (&off)[4]) {
   constexpr int NC = D > 128 ? D / 128 : 1;
   const int lane = threadIdx.x & 63, c0 = lane & 15;
@@ -338,9 +338,57 @@ __device__ __forceinline__ void append_singles(const Append8Args& a, const Side&
   }
 }
 
+// Skipped rows (slots outside the cache) do not part a run: what lies behind them or
+// before them may be any number of rows away.  Both searches are uniform, 512 rows a
+// round trip, and rare: a wave makes one where the rows next to its own, up to the end of
+// its 64, are all skipped (a rotating call of 1000 tokens and 3096 skipped rows behind
+// them 16.1 us, 13.7 without the search; 100 single tokens and 156 such rows 5.7 for 5.1).
+constexpr int kSearchLoads = 8;
+// The first token at or past `from` that is not skipped (n_tokens: none).
+__device__ __forceinline__ int token_from(const Append8Args& a, int from) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (; from < (int)a.n_tokens; from += 64 * kSearchLoads) {
+    int64_t s[kSearchLoads];
+#pragma unroll
+    for (int k = 0; k < kSearchLoads; ++k)
+      s[k] = a.slots[min(from + 64 * k + lane, (int)a.n_tokens - 1)];
+#pragma unroll
+    for (int k = 0; k < kSearchLoads; ++k) {
+      const int t = from + 64 * k;
+      const uint64_t in = __builtin_amdgcn_ballot_w64(t + lane < (int)a.n_tokens && s[k] >= 0 &&
+                                                      s[k] < a.n_slots);
+      if (in) return t + __builtin_ctzll(in);
+    }
+  }
+  return (int)a.n_tokens;
+}
+// The block of the last token before `end` that is not skipped (-1: none).
+__device__ __forceinline__ int block_before(const Append8Args& a, int end) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (; end > 0; end -= 64 * kSearchLoads) {
+    int64_t s[kSearchLoads];
+#pragma unroll
+    for (int k = 0; k < kSearchLoads; ++k) s[k] = a.slots[max(end - 64 * (k + 1) + lane, 0)];
+#pragma unroll
+    for (int k = 0; k < kSearchLoads; ++k) {
+      const uint64_t in = __builtin_amdgcn_ballot_w64(end - 64 * (k + 1) + lane >= 0 && s[k] >= 0 &&
+                                                      s[k] < a.n_slots);
+      if (in)
+        return __builtin_amdgcn_readlane((int)(s[k] / kKv8Tokens), 63 - __builtin_clzll(in));
+    }
+  }
+  return -1;
+}
+// The bits of `mine` below the first one of `others`.
+__device__ __forceinline__ uint64_t up_to(uint64_t mine, uint64_t others) {
+  return mine & ((others & -others) - 1);  // (no others: all of them)
+}
+
 // A wave of the cache's writers: a head and side of the runs that begin in its
-// window of tokens.  A run is tokens next to each other in the call whose slots lie
-// in one block.
+// window of tokens.  A run is tokens of one block with no other block's between them in
+// the call.
 template <int DT, int D, int TURN>
 __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id) {
   const bool value = id & 1;
@@ -350,18 +398,31 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
   const uint32_t win = rest % a.n_windows, layer = rest / a.n_windows;
   const int lane = threadIdx.x & 63, g = lane >> 4;
   // lane i: token `first` + i, the one before the window in lane 0
-  const int64_t first = (int64_t)win * a.window - 1, tok = first + lane;
+  const int first = (int)(win * a.window) - 1, tok = first + lane;  // (below 2^30: append_args)
   int64_t s = -1;
-  if (tok >= 0 && tok < a.n_tokens) s = a.slots[tok];
+  if (tok >= 0 && tok < (int)a.n_tokens) s = a.slots[tok];
   const bool in = s >= 0 && s < a.n_slots;
   const int blk = in ? (int)(s / kKv8Tokens) : -1, off = (int)(s & (kKv8Tokens - 1));
-  const int before = __shfl_up(blk, 1), behind = __shfl_down(blk, 1);  // (every lane active)
+  const uint64_t held = __builtin_amdgcn_ballot_w64(in);
+  // the blocks of the nearest tokens before the lane's and behind it that are not skipped
+  // (before: -1, none; behind: its own where it is not among the wave's)
+  int before = __shfl_up(blk, 1), behind = __shfl_down(blk, 1);  // (every lane active)
+  const bool whole = held == __builtin_amdgcn_ballot_w64(tok >= 0 && tok < (int)a.n_tokens);
+  if (__builtin_expect(!whole, 0)) {  // uniform: some are skipped
+    const uint64_t below = held & ((1ull << lane) - 1), above = held >> lane >> 1;
+    before = __shfl(blk, below ? 63 - __builtin_clzll(below) : lane);
+    behind = __shfl(blk, above ? lane + 1 + __builtin_ctzll(above) : lane);
+    int back = -1;
+    if (!(held & 1) && held & 0x1fffe && first > 0) back = block_before(a, first);  // uniform
+    if (!below) before = back;
+    if (!above && first + 64 >= (int)a.n_tokens) behind = -1;
+  }
   const bool begins = lane > 0 && lane <= (int)a.window && in && blk != before;
-  uint64_t heads = __builtin_amdgcn_ballot_w64(begins);
+  uint32_t heads = (uint32_t)__builtin_amdgcn_ballot_w64(begins);  // (lanes 1 .. 16)
   if (!heads) return;  // uniform
   const Side side = side_of(a, layer, head, value, D);
   if (a.window > 1 && __builtin_amdgcn_ballot_w64(begins && blk == behind) == 0) {
-    int64_t at[4];
+    int at[4];
     int b[4], o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -373,18 +434,19 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
     append_singles<DT, D, TURN>(a, side, at, b, o);
     return;
   }
+  const int step = whole ? off - lane : INT32_MAX;  // the same in places one after the other
   while (heads) {  // uniform
-    const int i = __builtin_ctzll(heads);
+    const int i = __builtin_ctz(heads);
     heads &= heads - 1;
     const int b = __builtin_amdgcn_readlane(blk, i);
     const uint64_t same = __builtin_amdgcn_ballot_w64(blk == b) >> i;
-    const int n = ~same ? __builtin_ctzll(~same) : 64;  // tokens of the run (i > 0: below 64)
+    const int n = __builtin_ctzll(~same);  // neighbours of one block (i > 0: bit 63 is clear)
     const int off0 = __builtin_amdgcn_readlane(off, i);
-    int64_t at[4];
+    int at[4];
     bool anew;
-    const uint64_t run = n < 64 ? (1ull << n) - 1 : ~0ull;
-    const uint64_t in_order = __builtin_amdgcn_ballot_w64(off == off0 + lane - i) >> i;
-    if ((in_order & run) == run) {  // one place after the other
+    const uint64_t run = (1ull << n) - 1;
+    const uint64_t in_order = __builtin_amdgcn_ballot_w64(step == off0 - i) >> i;
+    if (__builtin_expect((in_order & run) == run, 1)) {  // one place after the other
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 4 * g + k - off0;
@@ -395,23 +457,28 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
 #pragma unroll
       for (int k = 0; k < 4; ++k) at[k] = -1;
       anew = false;
-      int64_t base = first;
-      int place = off, x = i, end = i + n;
+      int base = first;
+      int place = off;
+      uint64_t todo = same << i;
+      uint64_t others = (__builtin_amdgcn_ballot_w64(blk >= 0) & ~todo) >> i << i;
+      todo = up_to(todo, others);
       while (true) {  // uniform
-        for (; x < end; ++x) {
-          const int o = __builtin_amdgcn_readlane(place, x);
+        for (; todo; todo &= todo - 1) {
+          const int x = __builtin_ctzll(todo), o = __builtin_amdgcn_readlane(place, x);
           anew |= o == 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) at[k] = o == 4 * g + k ? base + x : at[k];
         }
-        if (end < 64) break;
-        // the run goes past the wave's tokens (places given many times): the next 64
-        base += 64;
-        const int64_t next = base + lane < a.n_tokens ? a.slots[base + lane] : -1;
+        if (others) break;
+        // the run may go on past the wave's tokens: the next 64, from one not skipped
+        base = token_from(a, base + 64);
+        if (base >= (int)a.n_tokens) break;
+        const int64_t next = base + lane < (int)a.n_tokens ? a.slots[base + lane] : -1;
         place = (int)(next & (kKv8Tokens - 1));
-        const uint64_t on = __builtin_amdgcn_ballot_w64(next >= 0 && next / kKv8Tokens == b);
-        x = 0;
-        end = ~on ? __builtin_ctzll(~on) : 64;
+        const bool there = next >= 0 && next < a.n_slots;
+        const uint64_t on = __builtin_amdgcn_ballot_w64(there && next / kKv8Tokens == b);
+        others = __builtin_amdgcn_ballot_w64(there) & ~on;
+        todo = up_to(on, others);
       }
     }
     append_run<DT, D, TURN>(a, side, b, at, anew);
@@ -421,7 +488,7 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
 // (Four waves per SIMD asked for: a register too many left three, 15% slower for prompts
 // of heads of 64; five made the loads wait for registers, 10% slower for 4 x 1000 tokens.)
 template <int DT, int D, int TURN>
-__global__ __launch_bounds__(kAppend8Threads, D > 128 ? 2 : 4) void kv8_append_kernel(Append8Args a) {
+__global__ __launch_bounds__(kAppend8Threads, D > 128 ? 3 : 4) void kv8_append_kernel(Append8Args a) {
   uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (kAppend8Threads / 64) +
                                                (threadIdx.x >> 6));
   if (id >= a.n_tasks) return;

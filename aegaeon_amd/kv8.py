@@ -81,7 +81,9 @@ def reshape_and_cache_kv8(key: torch.Tensor, value: torch.Tensor, kv_cache: torc
     slots past the cache are skipped.  A row at a block's first token begins the
     block anew; others join what it holds, whose values are rounded once more
     where their size raises the block's exponent.  The rows of one block must
-    follow each other in the call; of several for one slot the last counts."""
+    follow each other in the call (skipped ones may lie between them, another block's
+    not: the block's values may be wrong then); of several for one slot the last
+    counts."""
     _check_new_rows(key, value, 3, "[T, Hkv, D]")
     _append(key, value, kv_cache, slot_mapping, False, "reshape_and_cache_kv8")
 

@@ -557,9 +557,10 @@ int64_t aegkv_kv8_block_bytes(int32_t n_kv_heads, int32_t head_dim);
 /* aegkv_kv_append into the 8-bit cache: key/value rows of `dtype` (strides in
  * elements, the heads of a token dense), slots as there (negative ones and those
  * past the pool are skipped).  The tokens of one block must follow each other in
- * the call (as those of a prompt do), in any order within it; of two for one slot
- * the later one counts.  (Tokens of a block that other tokens lie between may
- * leave the block's values wrong, not those of other blocks.) */
+ * the call (as those of a prompt do), in any order within it, with any skipped rows
+ * between them; of two for one slot the later one counts.  (Tokens of a block that
+ * another block's tokens lie between may leave the block's values wrong, not those of
+ * other blocks.) */
 int aegkv_kv8_append(const void* key, const void* value, int64_t key_token_stride,
                      int64_t value_token_stride, int64_t key_layer_stride,
                      int64_t value_layer_stride, const int64_t* slot_mapping, int64_t n_tokens,

@@ -10,6 +10,7 @@ textbook in float64 over the decoded rows.
 from __future__ import annotations
 
 from functools import lru_cache
+from itertools import groupby
 from typing import Tuple
 
 import numpy as np
@@ -68,23 +69,18 @@ def _index(side: int, dim: int) -> np.ndarray:
 def append(key: np.ndarray, value: np.ndarray, cache: np.ndarray, slots: np.ndarray,
            dtype: str) -> None:
     """Rows ``[L, T, Hkv, D]`` (float32 or float64) into the cache, in place;
-    slots outside the cache are skipped."""
+    slots outside the cache are skipped, and tokens of a block join it at once
+    where no other block's lie between them."""
     L, T, H, D = key.shape
     slots = [int(s) for s in slots]
-    t = 0
-    while t < T:
-        blk = slots[t] // BLOCK
-        end = t
-        while end < T and slots[end] // BLOCK == blk:
-            end += 1
-        if 0 <= slots[t] < cache.shape[0] * BLOCK:
-            place = {slots[i] % BLOCK: i for i in range(t, end)}  # the later of two
-            for layer in range(L):
-                for h in range(H):
-                    for side, x in enumerate((key, value)):
-                        _put(cache[blk, layer], side, H, D, h,
-                             {r: x[layer, i, h] for r, i in place.items()}, dtype)
-        t = end
+    written = [t for t in range(T) if 0 <= slots[t] < cache.shape[0] * BLOCK]
+    for blk, run in groupby(written, key=lambda t: slots[t] // BLOCK):
+        place = {slots[t] % BLOCK: t for t in run}  # the later of two
+        for layer in range(L):
+            for h in range(H):
+                for side, x in enumerate((key, value)):
+                    _put(cache[blk, layer], side, H, D, h,
+                         {r: x[layer, t, h] for r, t in place.items()}, dtype)
 
 
 def _put(layer_block, side, H, D, h, new, dtype):

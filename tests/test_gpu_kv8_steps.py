@@ -1,0 +1,116 @@
+"""GPU parity of the 8-bit cache's append where a call's rows are not a few prompts:
+rows that are skipped between the tokens of a block.  Every byte of the cache equals
+the oracle's."""
+import numpy as np
+import pytest
+import torch
+
+from aegaeon_amd import kv8, rotary
+from oracle import kv8_oracle as k8
+from oracle import kv_oracle as ko
+from tests.kvtest_utils import to_bits, to_device_bits
+
+pytestmark = pytest.mark.gpu
+
+
+def _rows(rng, shape, dtype):
+    """Rows whose channels and tokens differ much in size, as bits."""
+    x = rng.standard_normal(shape) * np.exp(rng.standard_normal(shape[-1])) \
+        * np.exp(rng.standard_normal(shape[:-1]))[..., None]
+    return ko.float_to_bits(x, dtype)
+
+
+def _filled(rng, n, layers, heads, dim, dtype):
+    """A cache whose every slot was written, as the oracle holds it."""
+    cache = np.full((n, layers, k8.block_bytes(heads, dim)), 0xFF, dtype=np.uint8)
+    x = ko.bits_to_float(_rows(rng, (2, layers, n * 16, heads, dim), dtype), dtype)
+    k8.append(x[0], x[1], cache, np.arange(n * 16), dtype)
+    return cache
+
+
+def _check_append(device, key, value, cache, slots, dtype):
+    dev = torch.from_numpy(cache).to(device)
+    slots = np.asarray(slots, dtype=np.int64)
+    kv8.append_kv8(to_device_bits(key, dtype, device), to_device_bits(value, dtype, device), dev,
+                   torch.from_numpy(slots).to(device))
+    k8.append(ko.bits_to_float(key, dtype), ko.bits_to_float(value, dtype), cache, slots, dtype)
+    assert np.array_equal(dev.cpu().numpy(), cache)
+
+
+# ---------------------------------------------------------------------------
+# skipped rows do not part a block's tokens
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("slots", [
+    [16, -1, 17], [17, 4 * 16, 16], [20, -1, -1, 21, -9, 22], [-1, 18, -1, 17, -1, 18, -1],
+    [31, -1, 32, -1, 30 - 16, -1, 15, -1, 48]])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_skipped_rows_between_the_tokens_of_a_block(device, slots, dtype):
+    rng = np.random.default_rng(len(slots))
+    cache = _filled(rng, 4, 2, 3, 128, dtype)
+    k, v = (_rows(rng, (2, len(slots), 3, 128), dtype) for _ in range(2))
+    _check_append(device, k, v, cache, slots, dtype)
+
+
+@pytest.mark.parametrize("gap", [1, 20, 30, 46, 47, 62, 63, 64, 65, 511, 512, 513, 575, 576, 1100])
+@pytest.mark.parametrize("before", [0, 15])
+@pytest.mark.parametrize("heads", [2, 40])
+def test_long_gaps(device, gap, before, heads):
+    """Gaps of every length about the 64 rows of a wave and the 512 of a search, in
+    order and not, behind tokens of another block or none, ended by another block's or
+    by the call."""
+    rng = np.random.default_rng(gap + before)
+    for places, behind in (([3, 4, 5], []), ([0, 9, 2], [33, 34]), ([7, 7], [-1] * 300)):
+        slots = [0] * before
+        for p in places:
+            slots += [16 + p] + [-1] * gap
+        slots += behind
+        cache = _filled(rng, 3, 1, heads, 64, "bf16")
+        k, v = (_rows(rng, (1, len(slots), heads, 64), "bf16") for _ in range(2))
+        _check_append(device, k, v, cache, slots, "bf16")
+
+
+@pytest.mark.parametrize("layers", [1, 9])
+def test_a_padded_batch(device, layers):
+    """Sequences of a batch padded to one length with skipped rows, single tokens
+    and prompts among them, in blocks that begin anywhere."""
+    rng = np.random.default_rng(layers)
+    lens, width = [1, 3, 40, 1, 17, 1, 1, 64, 2], 70
+    slots, block = np.full((len(lens), width), -1), 0
+    for b, n in enumerate(lens):
+        start = int(rng.integers(0, 16))
+        at = rng.permutation(width)[:n] if b % 2 else np.arange(n)  # spread, or to the left
+        slots[b, np.sort(at)] = block * 16 + start + np.arange(n)
+        block += -(-(start + n) // 16)
+    cache = _filled(rng, block, layers, 4, 128, "fp16")
+    k, v = (_rows(rng, (layers, slots.size, 4, 128), "fp16") for _ in range(2))
+    _check_append(device, k, v, cache, slots.reshape(-1), "fp16")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_skipped_rows_of_a_rotating_append(device, interleaved):
+    """Drafted tokens of some of a batch's sequences, the others' rows skipped; all
+    queries and kept keys are turned."""
+    rng = np.random.default_rng(5)
+    B, m, Hq, Hkv, D = 40, 4, 4, 2, 64
+    slots = np.full((B, m), -1)
+    for b in range(B):
+        n = int(rng.integers(0, m + 1))
+        slots[b, np.sort(rng.permutation(m)[:n])] = b * 16 + int(rng.integers(0, 16 - n)) + np.arange(n)
+    slots = slots.reshape(-1)
+    x = _rows(rng, (B * m, Hq + 2 * Hkv, D), "bf16")
+    q, k, v = (y.contiguous() for y in to_device_bits(x, "bf16", device).split([Hq, Hkv, Hkv], 1))
+    f = ko.bits_to_float(x, "bf16")
+    positions = rng.integers(0, 100, size=B * m)
+    table = rotary.rotary_table(100, D, device=device)
+    cache = _filled(rng, B, 1, Hkv, D, "bf16")
+    dev = torch.from_numpy(cache).to(device)
+    key = torch.empty_like(k)
+    out = kv8.rotary_and_cache_kv8(q, k, v, dev[:, 0], torch.from_numpy(slots).to(device),
+                                   torch.from_numpy(positions).to(device), table,
+                                   interleaved=interleaved, out_key=key)
+    turned = [k8.turned(y, positions, table.cpu().numpy(), interleaved)
+              for y in (f[:, :Hq], f[:, Hq:Hq + Hkv])]
+    k8.append(turned[1][None], f[None, :, Hq + Hkv:], cache, slots, "bf16")
+    assert np.array_equal(dev.cpu().numpy(), cache)
+    for got, want in ((out, turned[0]), (key, turned[1])):
+        assert np.array_equal(to_bits(got), ko.float_to_bits(want.astype(np.float64), "bf16"))
