@@ -1,6 +1,8 @@
 """GPU parity of the 8-bit cache's append where a call's rows are not a few prompts:
-rows that are skipped between the tokens of a block.  Every byte of the cache equals
-the oracle's."""
+rows that are skipped between the tokens of a block, and single tokens of many blocks,
+which a wave takes four at a time.  Every byte of the cache equals the oracle's."""
+from functools import lru_cache
+
 import numpy as np
 import pytest
 import torch
@@ -114,3 +116,131 @@ def test_skipped_rows_of_a_rotating_append(device, interleaved):
     assert np.array_equal(dev.cpu().numpy(), cache)
     for got, want in ((out, turned[0]), (key, turned[1])):
         assert np.array_equal(to_bits(got), ko.float_to_bits(want.astype(np.float64), "bf16"))
+
+
+# ---------------------------------------------------------------------------
+# decode steps: single tokens, several runs of a wave at once
+# ---------------------------------------------------------------------------
+def _window(waves):
+    """Tokens whose runs a wave takes, of so many (token, head, side, layer)."""
+    w = 1
+    while w < 16 and waves > 2048 * w:
+        w *= 2
+    return w
+
+
+def _windows_of_singles(slots, window, n_slots):
+    """The windows in which two tokens or more begin, each the only one of its block."""
+    held = [t for t, s in enumerate(slots) if 0 <= s < n_slots]
+    block = {t: slots[t] // 16 for t in held}
+    begins = [t for i, t in enumerate(held) if i == 0 or block[held[i - 1]] != block[t]]
+    alone = {t for t in begins if not any(block.get(x) == block[t] for x in held if x > t)}
+    found = 0
+    for w in range(0, len(slots), window):
+        here = [t for t in begins if w <= t < w + window]
+        found += len(here) > 1 and all(t in alone for t in here)
+    return found
+
+
+@lru_cache(maxsize=None)
+def _filled_once(n, layers, heads, dim, dtype):
+    return _filled(np.random.default_rng(n + heads + dim), n, layers, heads, dim, dtype)
+
+
+def _steps(rng, T, n_blocks):
+    """(slots, gains) of three calls for T sequences: single tokens at any place, a
+    tenth skipped; the next place, which may be a block's first; then the next one or
+    two.  Gains raise most blocks' exponents in the first call and few later."""
+    fresh = [int(b) for b in rng.permutation(n_blocks)]
+    at = np.array([fresh.pop() * 16 + int(rng.choice([0, 1, 5, 10, 14, 15])) for _ in range(T)])
+    for step in range(3):
+        slots = []
+        for b in range(T):
+            for _ in range(2 if step == 2 and b % 9 == 0 else 1):
+                if rng.random() < 0.1:
+                    slots.append(int(rng.choice([-1, n_blocks * 16, -50])))
+                    continue
+                slots.append(int(at[b]))
+                at[b] = at[b] + 1 if at[b] % 16 < 15 else fresh.pop() * 16
+        gains = 2.0 ** rng.integers(-9 if step else -4, 4 if step else 10, size=len(slots))
+        yield np.array(slots, dtype=np.int64), gains
+
+
+def _scaled(rng, shape, gains, dtype):
+    """Rows [.., T, H, D] times their tokens' gains, infinities and NaN in a few."""
+    x = ko.bits_to_float(_rows(rng, shape, dtype), dtype) * gains[:, None, None]
+    for _ in range(6):
+        at = tuple(int(rng.integers(0, n)) for n in shape)
+        x[at] = rng.choice([np.inf, -np.inf, np.nan])
+    with np.errstate(over="ignore"):
+        return ko.float_to_bits(x, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("layers,window", [(2, 2), (4, 4), (8, 8), (16, 16)])
+def test_steps_of_single_tokens(device, dtype, D, layers, window):
+    """Layers beyond the second take the rows of the first two."""
+    T, H, n = 131, 4, 300
+    assert _window(2 * layers * H * T) == window
+    rng = np.random.default_rng(D + layers)
+    cache = _filled_once(n, 2, H, D, dtype).copy()
+    dev = torch.from_numpy(cache).to(device).repeat(1, layers // 2, 1)
+    for step, (slots, gains) in enumerate(_steps(rng, T, n)):
+        # (the third call mixes windows of single tokens and of pairs, as they come)
+        assert step == 2 or _windows_of_singles(slots, window, n * 16) > 2
+        k, v = (_scaled(rng, (2, len(slots), H, D), gains, dtype) for _ in range(2))
+        dk, dv = (to_device_bits(x, dtype, device).repeat(layers // 2, 1, 1, 1) for x in (k, v))
+        kv8.append_kv8(dk, dv, dev, torch.from_numpy(slots).to(device))
+        k8.append(ko.bits_to_float(k, dtype), ko.bits_to_float(v, dtype), cache, slots, dtype)
+        want = torch.from_numpy(cache).to(device).repeat(1, layers // 2, 1)
+        assert torch.equal(dev, want), step
+
+
+def _rotating_step(device, rng, dev, cache, slots, gains, Hq, D, table, dtype, interleaved):
+    H, T = (cache.shape[2] // (32 * D)), len(slots)
+    q = _scaled(rng, (T, Hq, D), gains, dtype)
+    k, v = (_scaled(rng, (T, H, D), gains, dtype) for _ in range(2))
+    positions = rng.integers(0, 900, size=T)
+    dq, dk, dv = (to_device_bits(x, dtype, device) for x in (q, k, v))
+    kv8.rotary_and_cache_kv8(dq, dk, dv, dev[:, 0], torch.from_numpy(slots).to(device),
+                             torch.from_numpy(positions).to(device), table, out=dq,
+                             interleaved=interleaved)
+    t = table.cpu().numpy()
+    with np.errstate(invalid="ignore", over="ignore"):
+        turned = k8.turned(ko.bits_to_float(k, dtype), positions, t, interleaved)
+        want_q = k8.turned(ko.bits_to_float(q, dtype), positions, t, interleaved)
+        want = ko.bits_to_float(ko.float_to_bits(want_q.astype(np.float64), dtype), dtype)
+    k8.append(turned[None], ko.bits_to_float(v, dtype)[None], cache, slots, dtype)
+    assert np.array_equal(dev.cpu().numpy(), cache)
+    got = dq.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.nan_to_num(got), np.nan_to_num(want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,rot", [(64, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotating_steps_of_single_tokens(device, dtype, D, rot, interleaved):
+    T, H, n = 131, 8, 300
+    assert _window(2 * H * T) == 2
+    rng = np.random.default_rng(D + rot)
+    cache = _filled_once(n, 1, H, D, dtype).copy()
+    dev = torch.from_numpy(cache).to(device)
+    table = rotary.rotary_table(900, rot, device=device)
+    for step, (slots, gains) in enumerate(_steps(rng, T, n)):
+        assert _windows_of_singles(slots, 2, n * 16) > 10
+        _rotating_step(device, rng, dev, cache, slots, gains, 5, D, table, dtype, interleaved)
+
+
+@pytest.mark.parametrize("dtype,interleaved", [("bf16", False), ("fp16", True)])
+def test_rotating_steps_past_the_largest_window(device, dtype, interleaved):
+    T, H, D, n = 210, 40, 128, 300
+    assert _window(2 * H * T) == 16
+    rng = np.random.default_rng(6)
+    cache = np.zeros((n, 1, k8.block_bytes(H, D)), dtype=np.uint8)
+    dev = torch.from_numpy(cache).to(device)
+    table = rotary.rotary_table(900, D, device=device)
+    slots, gains = next(_steps(rng, T, n))
+    assert _windows_of_singles(slots, 16, n * 16) > 10
+    _rotating_step(device, rng, dev, cache, slots, gains, 40, D, table, dtype, interleaved)
