@@ -148,13 +148,28 @@ struct Codes4 {
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
   }
-  // The first of a block's tokens whose V group of dim d is NaN (16: none).
+  // NaN comes by groups of V's dims.
+  static __device__ __host__ constexpr int nan_entry(int dim) { return dim / kKv4Group * kKv4Group; }
+  // The lane's block (ok: it is one), of the 64 from b0 on: its groups' scale bytes, a
+  // group's 16 tokens in one load, and the first NaN of each.  (Group after group: with
+  // all of them in flight the eight-wave kernel is 2% slower where there is no NaN.)
   template <int D>
-  static __device__ int first_nan(const uint8_t* part, const HeadPart&, int d) {
-    const uint8_t* e = part + kv4_record_bytes(D) + kv4_code_bytes(D) + d / kKv4Group * kKv4Tokens;
-    int t = 0;
-    while (t < kKv4Tokens && e[t] != kKv4ScaleNan) ++t;
-    return t;
+  static __device__ void find_nan(const uint8_t* part, const HeadPart&, bool ok, int b0,
+                                  int32_t* first) {
+    if (!ok) return;
+    const u32x4* e = reinterpret_cast<const u32x4*>(part + kv4_record_bytes(D) + kv4_code_bytes(D));
+#pragma unroll 1
+    for (int g = 0; g < D / kKv4Group; ++g) {
+      const u32x4 x = ~e[g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // a byte of zero (255 was there): the lowest one's bit 7 is exact
+        const uint32_t at = (x[i] - 0x01010101u) & ~x[i] & 0x80808080u;
+        if (at)
+          first_key(first + kKv4Group * g, (b0 + (int)(threadIdx.x & 63)) * kKv4Tokens + 4 * i +
+                                   (__builtin_ctz(at) >> 3));
+      }
+    }
   }
 };
 

@@ -138,14 +138,33 @@ struct Codes8 {
     }
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
   }
-  // The first of a block's tokens whose V value of dim d is NaN (16: none).
+  static __device__ __host__ constexpr int nan_entry(int dim) { return dim; }
+  // Whether the lane's block (ok: it is one), of the 64 from b0 on, has a NaN in V; then
+  // the wave takes such blocks one by one, a lane 4 dims of 4 tokens.
   template <int D>
-  static __device__ int first_nan(const uint8_t* part, const HeadPart& h, int d) {
-    if (!part[h.scale + 2]) return kKv8Tokens;
-    const uint8_t* v = part + kv8_side_bytes(D) + d % 4 * 4;
-    int t = 0;
-    while (t < kKv8Tokens && (v[kv8_v_byte<D>(t >> 2, d / 4) + (t & 3)] & 0x7f) != 0x7f) ++t;
-    return t;
+  static __device__ void find_nan(const uint8_t* part, const HeadPart& h, bool ok, int b0,
+                                  int32_t* first) {
+    const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+    uint64_t bad = __builtin_amdgcn_ballot_w64(ok && part[h.scale + 2] != 0);
+    for (; bad; bad &= bad - 1) {  // uniform
+      const int u = __builtin_ctzll(bad);
+      const uint64_t p = (uint64_t)part;
+      const uint8_t* v = reinterpret_cast<const uint8_t*>(
+                             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), u) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane((int)p, u)) +
+                         kv8_side_bytes(D) + 16 * lane;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(v + 1024 * i);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint32_t at = ((x[d] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          if (at)
+            first_key(first + D / 16 * j + 4 * i + d,
+                      (b0 + u) * kKv8Tokens + 4 * g + (__builtin_ctz(at) >> 3));
+        }
+      }
+    }
   }
 };
 

@@ -567,22 +567,33 @@ struct RowUnit : WaveSoftmax<DT, D, true> {
 // A tile's V values that are NaN are stored as zeros, as a weight of zero does not
 // undo a NaN, and found at the end (rare): the rows that see one's token get NaN in
 // its dim.  Visible keys are a prefix, so each dim's first such key of the piece
-// decides; every thread of the workgroup comes here.
-template <class F, int D>
+// decides: first[dim], found as first[F::nan_entry(dim)] where dims are NaN together.
+// Each wave takes 64 blocks, a lane one of them, and their minima meet in LDS; every
+// thread of the workgroup comes here.  (2048 queries over 16001 tokens, 28/4 heads, with
+// one NaN, us and without any: 4 bits 488 and 462, of 8 bits 465 and 472; a dim per thread,
+// block after block, 1556 and 720.)
+template <class F, int D, int NT>
 __device__ void find_nan(const VarlenArgs& a, const int32_t* table, const HeadPart& h, int len,
                          int kt0, int kt1, int32_t* first) {
+  const int t = threadIdx.x, lane = t & 63;
   const int n_blk = min(kt1 * kTileBlocks, (len + kCacheTokens - 1) / kCacheTokens);
-  if (threadIdx.x < D) {
-    int at = INT32_MAX;
-    for (int b = kt0 * kTileBlocks; b < n_blk && at == INT32_MAX; ++b) {
-      const int id = table[b];
-      if (id < 0 || id >= a.n_blocks) continue;
-      const int t = F::template first_nan<D>(a.cache + (int64_t)id * a.blk_b + h.off, h, threadIdx.x);
-      if (b * kCacheTokens + t < len && t < kCacheTokens) at = b * kCacheTokens + t;
-    }
-    first[threadIdx.x] = at;
+  if (t < D) first[t] = INT32_MAX;
+  VARLEN_BARRIER();
+  for (int b0 = kt0 * kTileBlocks + (t & ~63); b0 < n_blk; b0 += NT) {  // uniform in a wave
+    const int b = b0 + lane, id = b < n_blk ? table[b] : -1;
+    const bool ok = id >= 0 && id < a.n_blocks;
+    F::template find_nan<D>(a.cache + (int64_t)(ok ? id : 0) * a.blk_b + h.off, h, ok, b0, first);
   }
   VARLEN_BARRIER();
+  if constexpr (F::nan_entry(1) == 0) {  // to the group's other dims
+    const int x = t < D ? first[F::nan_entry(t)] : 0;
+    VARLEN_BARRIER();
+    if (t < D) first[t] = x;
+    VARLEN_BARRIER();
+  }
+}
+__device__ __forceinline__ void first_key(int32_t* at, int key) {
+  __hip_atomic_fetch_min(at, key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
 // Four waves.  KS = 1: four units, and wave w converts block w of each key tile.
@@ -689,7 +700,7 @@ __global__ __launch_bounds__(64 * kShortWaves4, 2) void cache_varlen_kernel(Varl
 #pragma unroll
   for (int i = 0; i < NW; ++i) nan |= s_nan[i] != 0;
   if (__builtin_amdgcn_readfirstlane(nan)) {
-    find_nan<F, D>(a, table, head, s.len, kt0 * KS, kt1 * KS, s_first);
+    find_nan<F, D, 64 * NW>(a, table, head, s.len, kt0 * KS, kt1 * KS, s_first);
     unit.spoil(s_first);
   }
   if (part > 0) return;
@@ -820,7 +831,7 @@ __global__ __launch_bounds__(64 * kLongWaves4) void cache_varlen_long_kernel(Var
   if (__builtin_amdgcn_readfirstlane(nan)) {
     // (in the stages' memory: an array beside them cost the whole kernel 1%)
     int32_t* first = reinterpret_cast<int32_t*>(lds);
-    find_nan<F, D>(a, table, head, s.len, kt0, kt0 + n_kt, first);
+    find_nan<F, D, 64 * W>(a, table, head, s.len, kt0, kt0 + n_kt, first);
     unit.spoil(first);
     VARLEN_BARRIER();  // before the outputs go there
   }
