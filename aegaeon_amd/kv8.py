@@ -127,16 +127,20 @@ def rotary_and_cache_kv8(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     8-bit cache, with :func:`reshape_and_cache_kv8`'s slots and blocks: returns the
     turned queries.  The codes are those of the turned keys in fp32, without a
     rounding to 16 bits between; ``out_key``, in 16 bits, must not be ``key``."""
-    dev = kv_cache.device
+    if query.dim() == 0:
+        raise ValueError("query must be [T, Hq, D]")
+    dev, heads = kv_cache.device, _kv_heads(kv_cache, False, query.shape[-1])
+    N, R = kv_cache.shape
+    cp, block_stride = kv_cache.data_ptr(), kv_cache.stride(0)
     args, out, keep = _turn_args(query, key, value, slot_mapping, positions, table, interleaved,
-                                 out, out_key, dev, False)
-    if _kv_heads(kv_cache, False, args[12]) != args[11]:
+                                 out, out_key, dev, False,
+                                 (("kv_cache", cp, cp + ((N - 1) * block_stride + R if N else 0)),))
+    if heads != args[11]:
         raise ValueError("key/value and kv_cache disagree on the kv heads")
     if args[15] == 0:
         return out
     with device_guard(dev):
-        rc = _lib.load().aegkv_kv8_rotary_append(*args, kv_cache.data_ptr(), kv_cache.stride(0),
-                                                 kv_cache.size(0), _DTYPES[query.dtype],
+        rc = _lib.load().aegkv_kv8_rotary_append(*args, cp, block_stride, N, _DTYPES[query.dtype],
                                                  raw_stream(dev))
     _lib.check(rc, "rotary_and_cache_kv8")
     return out

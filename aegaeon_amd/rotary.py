@@ -55,11 +55,21 @@ def _check_apart(name: str, written, read, same: Tuple[str, ...]) -> None:
         raise ValueError(f"{name} overlaps {of}")
 
 
+def _check_clear(written, others) -> None:
+    """No row of ``written`` lies in a tensor of ``others``, whatever gaps its blocks
+    have; both (name, first byte, byte past the last)."""
+    for name, a, b in written:
+        for of, c, d in others:
+            if a < d and c < b:
+                raise ValueError(f"{name} overlaps {of}")
+
+
 def _turn_args(query, key, value, slot_mapping, positions, table, interleaved, out, out_key, dev,
-               key_in_place: bool):
-    """The checks that both caches' calls share: the leading arguments of the C
-    entries (kept to one look-up each: a decode step's call is bound by its host
-    time), the turned queries' tensor and what must outlive the call."""
+               key_in_place: bool, caches):
+    """The checks that both caches' calls share (``caches``: as :func:`_check_clear`'s
+    others): the leading arguments of the C entries (kept to one look-up each: a decode
+    step's call is bound by its host time), the turned queries' tensor and what must
+    outlive the call."""
     qs, ks, dtype = query.shape, key.shape, query.dtype
     if len(qs) != 3 or len(ks) != 3 or value.shape != ks or ks[0] != qs[0] or ks[2] != qs[2]:
         raise ValueError("query must be [T, Hq, D], key and value [T, Hkv, D] with its tokens "
@@ -87,7 +97,7 @@ def _turn_args(query, key, value, slot_mapping, positions, table, interleaved, o
                          f"rows of up to head_dim {D} entries")
     qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
     q_row, k_row = 2 * Hq * D, 2 * Hkv * D
-    given, read = out is not None, ()
+    given, read, rows = out is not None, (), ()
     if (given or out_key is not None) and T > 0:
         read = [("query", (qp, 2 * qt[0], q_row, qp + 2 * (T - 1) * qt[0] + q_row)),
                 ("key", (kp, 2 * kt[0], k_row, kp + 2 * (T - 1) * kt[0] + k_row)),
@@ -104,6 +114,7 @@ def _turn_args(query, key, value, slot_mapping, positions, table, interleaved, o
             written = (op, 2 * ot, q_row, op + 2 * (T - 1) * ot + q_row)
             _check_apart("out", written, read, ("query",))
             read.append(("out", written))
+            rows = (("out", op, written[3]),)
     else:
         out = query.new_empty(qs)
         op, ot = out.data_ptr(), Hq * D
@@ -117,12 +128,17 @@ def _turn_args(query, key, value, slot_mapping, positions, table, interleaved, o
         if T > 1 and 2 * okt < k_row:
             raise ValueError("out_key's rows overlap each other")
         if T > 0:
-            _check_apart("out_key", (okp, 2 * okt, k_row, okp + 2 * (T - 1) * okt + k_row), read,
+            end = okp + 2 * (T - 1) * okt + k_row
+            _check_apart("out_key", (okp, 2 * okt, k_row, end), read,
                          ("key",) if key_in_place else ())
+            rows += (("out_key", okp, end),)
     slots, positions = slot_mapping.contiguous(), positions.contiguous()
-    return (qp, qt[0], op, ot, Hq, kp, kt[0], vp, vt[0], okp, okt, Hkv, D, slots.data_ptr(),
-            positions.data_ptr(), T, table.data_ptr(), ts[0], ts[1], 1 if interleaved else 0), \
-        out, (slots, positions)
+    sp, pp, tp = slots.data_ptr(), positions.data_ptr(), table.data_ptr()
+    if rows:
+        _check_clear(rows, (("slot_mapping", sp, sp + 8 * T), ("positions", pp, pp + 8 * T),
+                            ("table", tp, tp + 4 * ts[0] * ts[1]), *caches))
+    return (qp, qt[0], op, ot, Hq, kp, kt[0], vp, vt[0], okp, okt, Hkv, D, sp, pp, T, tp, ts[0],
+            ts[1], 1 if interleaved else 0), out, (slots, positions)
 
 
 def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -139,27 +155,32 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     others stay.  Computed in fp32 and rounded once.  A position outside the
     table gives NaN.  Token strides are free, the heads of a token dense.
     ``out`` (default: a new tensor) may be ``query`` itself, ``out_key``, which
-    gets the turned keys (default: not kept), ``key``; all tokens of both are
-    written, also those whose slot is skipped (negative or past the cache).  Of two
+    gets the turned keys (default: not kept), ``key``; neither may overlap anything
+    else that the call takes.  All tokens of both are written, also those whose slot is
+    skipped (negative or past the cache).  Of two
     tokens for one slot either may be left there, in parts."""
     _check_cache_view(key_cache, "key_cache")
     _check_cache_view(value_cache, "value_cache")
     dev = key_cache.device
     _check_on(value_cache, "value_cache", dev)
-    args, out, keep = _turn_args(query, key, value, slot_mapping, positions, table, interleaved,
-                                 out, out_key, dev, True)
-    shape, dtype, block_stride = key_cache.shape, query.dtype, key_cache.stride(0)
+    shape, block_stride = key_cache.shape, key_cache.stride(0)
     if block_stride != value_cache.stride(0) or shape != value_cache.shape:
         raise ValueError("key_cache and value_cache must share shape and block stride")
+    N, bs, Hkv, D = shape
+    kp, vp = key_cache.data_ptr(), value_cache.data_ptr()
+    nbytes = 2 * ((N - 1) * block_stride + bs * Hkv * D) if N else 0
+    args, out, keep = _turn_args(query, key, value, slot_mapping, positions, table, interleaved,
+                                 out, out_key, dev, True, (("key_cache", kp, kp + nbytes),
+                                                           ("value_cache", vp, vp + nbytes)))
+    dtype = query.dtype
     if key_cache.dtype != dtype or value_cache.dtype != dtype:
         raise ValueError("the rows and the caches must share one 16-bit dtype")
-    N, bs, Hkv, D = shape
     if args[11] != Hkv or args[12] != D:
         raise ValueError("key/value must be [T, Hkv, D] matching the cache view")
     if args[15] == 0:
         return out
     with device_guard(dev):
-        rc = _lib.load().aegkv_rotary_append(*args, key_cache.data_ptr(), value_cache.data_ptr(),
-                                             block_stride, N, bs, _DTYPES[dtype], raw_stream(dev))
+        rc = _lib.load().aegkv_rotary_append(*args, kp, vp, block_stride, N, bs, _DTYPES[dtype],
+                                             raw_stream(dev))
     _lib.check(rc, "rotary_and_cache")
     return out

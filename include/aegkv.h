@@ -512,7 +512,8 @@ int aegkv_kv4_varlen_attention(void* out, int64_t out_token_stride, const void* 
  *     NaN.
  *   out_query: the turned queries, out_key (may be NULL) the turned keys (a
  *     prompt's own attention reads them); either may be its input (same pointer
- *     and stride).  All tokens are written, also those whose slot is skipped.
+ *     and stride), neither may overlap anything else that the call reads or writes.
+ *     All tokens are written, also those whose slot is skipped.
  *   The turned key rows and the value rows go to the cache as in
  *     aegkv_kv_append (one layer; slots < 0 and past the pool are skipped).
  * Token strides in elements, the heads of a token dense.  rotary_dim a multiple

@@ -244,3 +244,45 @@ def test_rotating_steps_past_the_largest_window(device, dtype, interleaved):
     slots, gains = next(_steps(rng, T, n))
     assert _windows_of_singles(slots, 16, n * 16) > 10
     _rotating_step(device, rng, dev, cache, slots, gains, 40, D, table, dtype, interleaved)
+
+
+def test_outputs_that_overlap_what_the_call_uses_are_refused(device):
+    """Slots, positions, the table and either cache, and nothing was written."""
+    T, H, D = 4, 2, 64
+    q, k, v = (torch.ones(T, H, D, dtype=torch.float16, device=device) for _ in range(3))
+    ids = torch.zeros(64 * T, dtype=torch.int64, device=device)
+    table = rotary.rotary_table(8, D, device=device)
+    c8 = kv8.kv8_cache(4, 2, H, D, device)
+    c16 = torch.zeros(4, 2, 16, H, D, dtype=torch.float16, device=device)
+
+    def rows(x):
+        return x.view(torch.float16).reshape(-1)[:T * H * D].view(T, H, D)
+
+    def call(eight, slots=ids[:T], positions=ids[:T], **kw):
+        if eight:
+            kv8.rotary_and_cache_kv8(q, k, v, c8[:, 1], slots, positions, table, **kw)
+        else:
+            rotary.rotary_and_cache(q, k, v, c16[:, 0], c16[:, 1], slots, positions, table, **kw)
+
+    before = [x.clone() for x in (ids, table, c8, c16)]
+    other = torch.zeros_like(ids)
+    for eight in (False, True):
+        for name in ("out", "out_key"):
+            with pytest.raises(ValueError, match=f"{name} overlaps slot_mapping"):
+                call(eight, positions=other[:T], **{name: rows(ids)})
+            with pytest.raises(ValueError, match=f"{name} overlaps positions"):
+                call(eight, slots=other[:T], **{name: rows(ids)})
+            with pytest.raises(ValueError, match=f"{name} overlaps table"):
+                call(eight, **{name: rows(table)})
+            if eight:
+                with pytest.raises(ValueError, match=f"{name} overlaps kv_cache"):
+                    call(True, **{name: rows(c8[2, 1])})
+            else:
+                for side in (0, 1):
+                    with pytest.raises(ValueError, match=f"{name} overlaps (key|value)_cache"):
+                        call(False, **{name: rows(c16[3, side])})
+    for x, y in zip((ids, table, c8, c16), before):
+        assert torch.equal(x, y)
+    whole = torch.zeros(3 * T * H * D, dtype=torch.float16, device=device)  # touching is clear
+    a, b, c = whole.view(3, T, H, D)
+    rotary.rotary_and_cache(b, k, v, c16[:, 0], c16[:, 1], ids[:T], ids[:T], table, out=a, out_key=c)
