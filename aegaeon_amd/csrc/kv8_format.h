@@ -4,16 +4,22 @@
 // an exponent e: the least integer with max|x| <= 448 * 2^e over the block's finite
 // values, within [-117, 119] (bf16) or [-15, 7] (fp16).  A value's code is the
 // 8-bit float (four exponent and three mantissa bits, largest 448) nearest to
-// x / 2^e, ties to even; an infinity or a NaN gets the code 0xff, a NaN.  An element is
-// off by 2^-4 of itself at most, or by 2^-10 * 2^e.  The bounds keep code * 2^e
+// x / 2^e, ties to even; an infinity or a NaN gets the code 0xff, a NaN.  An element
+// rounded once is off by at most 2^-4 of itself or 2^-10 * 2^e, half a step of the
+// codes or of the least of them, whichever is more.  The bounds keep code * 2^e
 // exact in the rows' 16-bit type (2^TOP * 448 finite, its least step a number of
 // the type), so that everything past the conversion is the 16-bit operators'
-// arithmetic; values past 448 * 2^TOP are stored as that.
+// arithmetic; values past 448 * 2^TOP are stored as that (fp16: 65504 as 57344).
 //   Tokens that join a block in which earlier ones are (none of them at the block's
 // first place) take e = max(the block's, their own).  When that rises, the earlier
 // tokens' values are rounded once more, to the codes of the new exponent: as the
-// scale is a power of two, only what falls below 2^-6 of it loses bits.  A token at
-// a block's first place begins the block anew, the tokens not written read as 0.
+// scale is a power of two, only what falls below 2^-6 of it loses bits, and an element
+// is off by less than 2^-9 * 2^e, or 2^-4 of itself, after any number of rises: each
+// rounding there is off by 2^-10 of its own 2^e, at most half of the next one's, and the
+// one before them by at most half of the first's.  No append lowers an exponent but
+// at a block's first place: a token written over another leaves the block as coarse as
+// that one made it.  A token at a block's first place begins the block anew, the tokens
+// not written read as 0.
 //
 // Bytes.  A block of one layer: per kv head the 16 D codes of K, then V's; then 4
 // bytes per head: K's e + 127, V's, 1 where V holds a NaN, 0; padded to a whole

@@ -1,5 +1,5 @@
-"""The 8-bit cache's rules without a GPU: which tokens join a block at once, and what
-the outputs of a rotating append may not share."""
+"""The 8-bit cache's rules without a GPU: which tokens join a block at once, how far
+a held value may be off, and what the outputs of a rotating append may not share."""
 import numpy as np
 import pytest
 
@@ -21,6 +21,48 @@ def test_skipped_rows_do_not_part_a_blocks_tokens(skipped):
     got = np.zeros_like(want)
     k8.append(rows, -rows, got, slots, "bf16")
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rises", [0, 1, 2, 5])
+def test_how_far_a_held_value_is_off(dtype, rises):
+    """Rounded once: 2^-4 of itself or 2^-10 of the scale.  After rises of the block's
+    exponent: 2^-4 of itself or less than 2^-9 of the scale, as roundings at scales
+    that double add up to less than twice the last one's.  (Exact in 64 bits.)"""
+    rng = np.random.default_rng(rises)
+    D, past = 64, 0
+    for trial in range(60):
+        cache = np.zeros((1, 1, k8.block_bytes(1, D)), dtype=np.uint8)
+        x = np.exp(rng.uniform(-10, 0, size=(1, 1, 1, D))) * rng.choice([-1, 1], size=(1, 1, 1, D))
+        x[..., 0] = 1.0
+        x *= 2.0 ** -6
+        k8.append(x, x, cache, np.array([0]), dtype)
+        for i in range(rises):
+            y = np.full((1, 1, 1, D), 2.0 ** -6 * 2.0 ** (i + 1))
+            k8.append(y, y, cache, np.array([1 + i]), dtype)
+        e = int(cache[0, 0, 32 * D]) - 127
+        assert e == -14 + rises
+        held = k8.rows(cache[:, 0], 1, D)[0][0, 0, 0]
+        off, own = np.abs(held - x[0, 0, 0]), 2.0 ** -4 * np.abs(x[0, 0, 0])
+        past += int((off > np.maximum(own, 2.0 ** (e - 10))).sum())
+        assert (np.maximum(off - own, 0) == 0)[off >= 2.0 ** (e - 9)].all()
+    assert (past > 0) == (rises > 0)  # the bound of one rounding does not hold for several
+
+
+def test_values_past_the_largest_are_held_as_that():
+    cache = np.zeros((1, 1, k8.block_bytes(1, 64)), dtype=np.uint8)
+    x = np.full((1, 1, 1, 64), 65504.0)
+    k8.append(x, -x, cache, np.array([0]), "fp16")
+    k, v = k8.rows(cache[:, 0], 1, 64)
+    assert (k[0, 0] == 57344.0).all() and (v[0, 0] == -57344.0).all()
+
+
+def test_a_token_written_over_leaves_the_blocks_exponent():
+    cache = np.zeros((1, 1, k8.block_bytes(1, 64)), dtype=np.uint8)
+    for place, size in ((0, 1.0), (1, 1000.0), (1, 1.0)):
+        x = np.full((1, 1, 1, 64), size)
+        k8.append(x, x, cache, np.array([place]), "bf16")
+    assert int(cache[0, 0, 32 * 64]) - 127 == 2   # 1000 <= 448 * 2^2, where 1.0 alone has -8
 
 
 def test_outputs_of_a_rotation_lie_clear_of_what_the_call_uses():
