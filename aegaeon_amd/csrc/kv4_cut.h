@@ -41,11 +41,13 @@ constexpr int ranges_of(int n_kt, int span) {
 // one of average length, so that only longer ones are cut), and the average work of a
 // place at least; a piece costs kPieceStart steps beside its own (its start, its
 // partials).  Sequences of more steps get more pieces of `span`.  `cost`: key steps of
-// all tiles.  Us a pass of the 8-bit cache, uncut and so (28/4 heads of 128, bf16): 1250
-// queries over 16000 tokens (140 tiles) 463 and 341, 1500 (168) 464 and 376, 2048 (224)
-// 477 and 458 (a step takes 2.1 us with every CU at work, 1.85 with 224), 3 x 700 over
-// 6000 on average, ragged (240) 226 and 190, 8/8 heads, 14 x 512 over 8000 (224) 254 and
-// 257.
+// all tiles.  Us a pass of the 8-bit cache, uncut and so (bf16, D = 128; one session):
+// 28/4 heads, 1250 queries over 16000 tokens (140 tiles) 470 and 342, 1500 (168) 471 and
+// 379, 2048 (224) 473 and 450 (a step takes 2.1 us with every CU at work, 1.85 with 224),
+// 3 x 700 over 4100 to 7400 (240) 229 and 215; 8/8 heads, 14 x 512 over 4258 to 7471 (224)
+// 228 and 200, over 8000 each 245 and 251.  So tiles of one length on 7/8 of the CUs gain
+// nothing and pay the merge; they are cut all the same, as the host does not know the
+// lengths and uneven ones gain more than that.
 constexpr int kPieceStart = 8;
 constexpr int uneven_span(int64_t cost, int64_t tiles, int64_t places, int least) {
   if (tiles <= 0 || places <= 0) return INT32_MAX;

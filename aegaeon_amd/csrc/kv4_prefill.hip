@@ -4,8 +4,8 @@
 //
 // Bounds and measured.  Per cached token and kv head 17 D / 16 bytes are read
 // and 4 D G flops done per query, so past some 10 queries at G = 7 the products
-// bound it: 2048 queries over 16001 tokens (28/4 heads, D = 128) 453 us, 972
-// TFLOP/s (224 of 256 CUs hold a tile, at 92% of the rate of a large matrix
+// bound it: 2048 queries over 16001 tokens (28/4 heads, D = 128) 453 to 462 us by the
+// session, 972 to 952 TFLOP/s (224 of 256 CUs hold a tile, at 92% of the rate of a large matrix
 // product each); 4 x 512 over 3800 tokens each 137 us, the longest sequence's;
 // two whole prompts of 2048 81 us, 747 TFLOP/s.  Few queries are bound by the latency
 // of their steps, 1.7 us each of a lone workgroup (conversion, products and softmax

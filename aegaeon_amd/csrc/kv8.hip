@@ -9,11 +9,14 @@
 // further): a block's maximum is a reduction within the wave, and V's words, four
 // tokens of a dim, come together in one lane's registers.
 //   Both are bound by memory once they are large.  4 kv heads of 128, bf16:
-//   append    28 layers of a decode step of 128 tokens 12.5 us, of 256 20.0: latency of
-//             the chain slot, scale byte, new scale, and of the lines that V's bytes
-//             touch.  8 layers of 4 x 1024 tokens 21.7 us (100 MB, 4.6 TB/s).
-//   rotating  one layer beside 28 query heads: 128 tokens 5.5 us, 4000 of four prompts
-//             19.2 (71 MB, 3.7 TB/s: the keys' waves load partners and angles too).
+//   append    28 layers of a decode step of 128 tokens 10.9 us: latency of the chain
+//             slot, scale byte, new scale, and lines written in part.  Of 256 tokens 15.9:
+//             a token's K is 16 bytes in each of eight lines per head and layer, its V
+//             one byte in four of another four, so 128 tokens touch 24 MB of lines for
+//             3.7 MB of codes, beside 7.3 MB of rows.  8 layers of 4 x 1024 tokens 21.2 us
+//             (100 MB, 4.7 TB/s).
+//   rotating  one layer beside 28 query heads: 128 tokens 5.0 us, 4000 of four prompts
+//             18.3 (71 MB, 3.9 TB/s: the keys' waves load partners and angles too).
 //   gather    128 sequences of 400 tokens on average 25.4 us (155 MB, 6.1 TB/s).
 #include <algorithm>
 
@@ -722,7 +725,7 @@ uint32_t window_of(uint64_t waves_of_one) {
 }
 
 // The part of a call that both appends share: checks of the cache and the rows, and
-// the waves that write.  (1: nothing to do)
+// the waves that write.  A status; AEGKV_OK without tokens too, with `a` as it was.
 int append_args(Append8Args& a, const void* key, const void* value, int64_t key_token_stride,
                 int64_t value_token_stride, int64_t key_layer_stride, int64_t value_layer_stride,
                 const int64_t* slot_mapping, int64_t n_tokens, void* cache,

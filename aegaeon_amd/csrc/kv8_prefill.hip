@@ -5,7 +5,7 @@
 // 8 bytes of a dim's four tokens, and the operand V^T[32 dims x 16 keys] is one
 // ordinary 16-byte read per lane, without a transposing read.
 //   Bound by the products where rows are many (2048 queries over 16001 tokens, 28/4
-// heads, bf16: 464 us a pass, 950 TFLOP/s) and by the latency of a piece's start and
+// heads, bf16: 450 to 464 us a pass by the session, 977 to 948 TFLOP/s) and by the latency of a piece's start and
 // steps where they are few (48 x 5 over 1000 tokens, 32/4 heads: 22.4 us and the merge's
 // 4.4; 52 MB).  Measured and no better: V^T's rows permuted by
 // one more bit (0 to +1.5%), reads four ahead (0), left to the compiler's order (+2%),

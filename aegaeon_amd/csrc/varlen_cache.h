@@ -210,9 +210,10 @@ __device__ __forceinline__ bool locate(const VarlenArgs& a, LocateLds& x, Piece&
   p.tile = p.s.tiles - 1 - p.tile;
   return true;
 }
-// As locate, of an uneven cut (its number of pieces r is the sequence's; a tile may have
-// fewer, uneven_tile).  The first pieces of all tiles come first, in the order above,
-// then the others.
+// As locate, of an uneven cut.  The number of pieces r is the sequence's: a tile whose
+// own key steps give fewer (uneven_ranges, in cache_varlen_long_kernel) leaves the rest
+// of its workgroups without work, and they return there.  The first pieces of all tiles
+// come first, in the order above, then the others.
 template <int W, int NT>
 __device__ __forceinline__ bool locate_uneven(const VarlenArgs& a, LocateLds& x, Piece& p) {
   constexpr int NW = NT / 64;
