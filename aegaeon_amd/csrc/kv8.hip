@@ -246,9 +246,9 @@ __device__ __forceinline__ void append_run(const Append8Args& a, const Side& s, 
 
 // Up to 16 runs of one token each, as a decode step's: the lanes 16 g .. take the
 // window's tokens 4 k + g, every load of the four in flight together (28 layers of
-// 128 tokens of 4 heads of 128: 12.6 us, one run after the other 27.4; V's words read
-// and written whole instead of their bytes 12.1, but prompts, whose waves it leaves
-// fewer registers, 5-15% slower).  tok[k] (-1: none) goes to place off[k] of block
+// 128 tokens of 4 heads of 128, of the same first form of the kernel: 12.6 us, one run
+// after the other 27.4; V's words read and written whole instead of their bytes 12.1, but
+// prompts, whose waves it leaves fewer registers, 5-15% slower).  tok[k] (-1: none) goes to place off[k] of block
 // blk[k].
 template <int DT, int D, int TURN>
 __device__ __forceinline__ void append_singles(const Append8Args& a, const Side& s,
@@ -489,7 +489,8 @@ __device__ __forceinline__ void append_window(const Append8Args& a, uint32_t id)
 }
 
 // (Four waves per SIMD asked for: a register too many left three, 15% slower for prompts
-// of heads of 64; five made the loads wait for registers, 10% slower for 4 x 1000 tokens.)
+// of heads of 64; five made the loads wait for registers, 10% slower for 4 x 1000 tokens.
+// Three for heads of 256, whose rotating form in fp16 needs all of those 168 registers.)
 template <int DT, int D, int TURN>
 __global__ __launch_bounds__(kAppend8Threads, D > 128 ? 3 : 4) void kv8_append_kernel(Append8Args a) {
   uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (kAppend8Threads / 64) +
